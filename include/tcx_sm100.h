@@ -455,6 +455,76 @@ int tcx_sm100_topk(tcx_stream_t stream, int dtype, const void* input, void* valu
 int tcx_sm100_embedding(tcx_stream_t stream, const int32_t* indices, int64_t rows, const float* weight,
                         int64_t vocabulary, int64_t width, float* output, int* invalid_flag);
 
+/* ----------------------------------------------------------------- training --- */
+/* Operators that a model learns with; the reference, an inference runtime, has no
+ * counterpart of them. float32; statistics, sums and states are held in 32 bits.
+ * Outputs must not overlap inputs unless a declaration says so.
+ *
+ * Random masks: element e of a call takes place offset + e of the seed's uniform stream
+ * (tcx_sm100_random, UNIFORM on [0, 1)) and is kept when its value is at least p, a
+ * comparison made exactly on the 24 random bits. The mask is a function of (seed, place)
+ * and is not stored: the backward pass gets the same seed and offset and makes it again.
+ * p in [0, 1]; p = 0 keeps everything, p = 1 nothing. A kept element is multiplied by
+ * 1 / (1 - p) rounded to float32; a dropped one counts as 0 even when it is inf or NaN.
+ * step_offset, when not NULL, is a device int64 that is read when the kernels run and
+ * added to offset (modulo 2^64): a captured graph whose counter is advanced between
+ * replays gets a new mask every time. */
+
+/* output = dropout(input), or residual + dropout(input) with a residual (the product and
+ * the sum rounded one after the other). The gradient with respect to input is the same
+ * call on the output's gradient, without the residual. output may be input or residual. */
+int tcx_sm100_dropout(tcx_stream_t stream, const float* input, const float* residual, float* output, int64_t count,
+                      double p, uint64_t seed, uint64_t offset, const int64_t* step_offset);
+
+/* Layer norm over the last axis of [rows, cols] that keeps what its backward pass needs:
+ *   total = residual + dropout(input)        (total may be NULL without both: it is input)
+ *   mean[r] = mean of row r,  rstd[r] = 1 / sqrt(variance of row r + epsilon)
+ *   output = (total - mean) * rstd * weight + bias      (weight, bias [cols] or NULL)
+ * The variance is the biased one, computed about the mean. A constant finite row whose
+ * values' differences are 0 gives exactly 0 * weight + bias (NaN when epsilon is 0). */
+int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* input, const float* residual, const float* weight,
+                                const float* bias, float* output, float* total, float* mean, float* rstd,
+                                int64_t rows, int64_t cols, float epsilon, double p, uint64_t seed, uint64_t offset,
+                                const int64_t* step_offset);
+
+/* Its gradients. With xhat = (total - mean) * rstd and g = dy * weight:
+ *   dresidual = dtotal + rstd * (g - mean(g) - xhat * mean(g * xhat))
+ *   dx = dresidual through the dropout      (dx may be NULL when p is 0: it is dresidual)
+ *   dweight[c] = sum over rows of dy * xhat,  dbias[c] = sum over rows of dy
+ * dtotal (the gradient that reaches total by other ways) may be NULL; dweight and dbias
+ * are both given or both NULL. Sums over rows are added in a fixed order: the same inputs
+ * give the same bits. The workspace holds partial column sums. */
+size_t tcx_sm100_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy, const float* total, const float* mean,
+                                 const float* rstd, const float* weight, const float* dtotal, float* dresidual,
+                                 float* dx, float* dweight, float* dbias, int64_t rows, int64_t cols, double p,
+                                 uint64_t seed, uint64_t offset, const int64_t* step_offset, void* workspace,
+                                 size_t workspace_bytes);
+
+/* Gated linear recurrence over [batch, time, channels], each channel by itself:
+ *   DECAY:    h_t = gate_t * h_(t-1) + x_t
+ *   SIGMOID:  h_t = s_t * h_(t-1) + (1 - s_t) * x_t,  s_t = 1 / (1 + exp(-gate_t))
+ * from initial [batch, channels] (NULL: zeros). lengths (NULL, or batch device int32, taken
+ * as clamped to [0, time]): steps at and beyond a sequence's length hold its state,
+ * h_t = h_(t-1), whatever gate and x hold there. h receives every state; state (NULL or
+ * [batch, channels]) the last one. Long sequences are cut into parts that are joined by
+ * (product of gates, state from zero): the products must be representable, as they are
+ * for gates of magnitude up to 1. */
+enum { TCX_RECURRENCE_DECAY = 0, TCX_RECURRENCE_SIGMOID = 1 };
+size_t tcx_sm100_recurrence_workspace_bytes(int64_t batch, int64_t time, int64_t channels);
+int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const float* gate, const float* x,
+                                 const float* initial, const int32_t* lengths, float* h, float* state, int64_t batch,
+                                 int64_t time, int64_t channels, void* workspace, size_t workspace_bytes);
+
+/* Its gradients from dh (of every h_t) and dstate (of the last state; NULL: zeros), given
+ * the forward pass's h: dgate and dx [batch, time, channels], dinitial [batch, channels]
+ * (or NULL). x is read in the SIGMOID form only (NULL otherwise). dgate and dx are 0 at
+ * steps that a sequence does not have. */
+int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, const float* dh, const float* gate, const float* x,
+                                  const float* h, const float* initial, const int32_t* lengths, const float* dstate,
+                                  float* dgate, float* dx, float* dinitial, int64_t batch, int64_t time,
+                                  int64_t channels, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

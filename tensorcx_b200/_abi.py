@@ -22,8 +22,10 @@ OP = dict(add=1, multiply=2, matmul=3, sum=4, max=5, mean=6, exp=7, gelu=8, silu
 ACT = dict(none=0, silu=1, relu=2)
 MATMUL_PATH = dict(auto=0, ffma=1, tensor=2)
 RANDOM = dict(normal=0, uniform=1)
+RECURRENCE = dict(decay=0, sigmoid=1)
 
 _vp, _i64, _sz, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_size_t, ctypes.c_int32, ctypes.c_float
+_f64, _u64 = ctypes.c_double, ctypes.c_uint64
 _i64p = ctypes.POINTER(ctypes.c_int64)
 
 
@@ -92,6 +94,17 @@ SIGNATURES = {
     "tcx_sm100_matmul_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, ctypes.c_int]),
     "tcx_sm100_matmul": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i32,
                                         _vp, ctypes.c_int, ctypes.c_int, _vp, _sz]),
+    "tcx_sm100_dropout": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _f64, _u64, _u64, _vp]),
+    "tcx_sm100_layernorm_forward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _f64,
+                                                   _u64, _u64, _vp]),
+    "tcx_sm100_layernorm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "tcx_sm100_layernorm_backward": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                                    _f64, _u64, _u64, _vp, _vp, _sz]),
+    "tcx_sm100_recurrence_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "tcx_sm100_recurrence_forward": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                                    _vp, _sz]),
+    "tcx_sm100_recurrence_backward": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                     _vp, _i64, _i64, _i64, _vp, _sz]),
 }
 
 _lib = None

@@ -33,39 +33,15 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "philox.cuh"
 
 namespace tcx {
 namespace {
 
-constexpr uint32_t kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u;  // round multipliers
-constexpr uint32_t kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;  // key schedule (Weyl)
+using namespace philox;
+
 constexpr float kTwoPow24Inv = 5.9604644775390625e-08f;               // 2^-24
 constexpr float kPi = 3.14159265358979323846f, kTwoPi = 6.28318530717958647692f;
-
-// The ten round keys of `key` (the Weyl sequence), computed once per thread.
-struct RoundKeys {
-  uint32_t x[10], y[10];
-};
-__device__ __forceinline__ RoundKeys round_keys(uint2 k) {
-  RoundKeys rk;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    rk.x[r] = k.x + static_cast<uint32_t>(r) * kPhiloxW0;
-    rk.y[r] = k.y + static_cast<uint32_t>(r) * kPhiloxW1;
-  }
-  return rk;
-}
-
-__device__ __forceinline__ uint4 philox4x32_10(uint4 c, const RoundKeys& rk) {
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t p0 = static_cast<uint64_t>(kPhiloxM0) * c.x, p1 = static_cast<uint64_t>(kPhiloxM1) * c.z;
-    const uint32_t hi0 = static_cast<uint32_t>(p0 >> 32), lo0 = static_cast<uint32_t>(p0);
-    const uint32_t hi1 = static_cast<uint32_t>(p1 >> 32), lo1 = static_cast<uint32_t>(p1);
-    c = make_uint4(hi1 ^ c.y ^ rk.x[r], lo1, hi0 ^ c.w ^ rk.y[r], lo0);
-  }
-  return c;
-}
 
 // -ln u for u in (0, 1] as described above (v = 1 - u is exact for u >= 1/2).
 __device__ __forceinline__ float neg_ln(float u) {
@@ -112,10 +88,6 @@ __device__ __forceinline__ float4 block_values(uint4 w, float a, float b) {
     v.w = __fmaf_rn(span, __fmul_rn(static_cast<float>(w.w >> 8), kTwoPow24Inv), a);
   }
   return v;
-}
-
-__device__ __forceinline__ uint4 block_words(uint64_t blk, const RoundKeys& rk) {
-  return philox4x32_10(make_uint4(static_cast<uint32_t>(blk), static_cast<uint32_t>(blk >> 32), 0u, 0u), rk);
 }
 
 // Elements [offset, offset + count) of the stream into out[0, count); element e is word

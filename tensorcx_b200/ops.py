@@ -21,12 +21,13 @@ import numpy as np
 import torch
 
 from . import plan
-from ._abi import ACT, FLOAT32, INT32, MATMUL_PATH, OP, Partial, check, i64_array, lib
+from ._abi import ACT, FLOAT32, INT32, MATMUL_PATH, OP, RECURRENCE, Partial, check, i64_array, lib
 
 __all__ = ["matmul", "sum", "max", "mean", "min", "argmax", "softmax", "rmsnorm", "layernorm",
            "exp", "gelu", "silu", "add", "subtract", "multiply", "divide", "clip", "relu",
            "bias_act", "linear", "attention", "scaled_dot_product_attention", "attention_softmax",
-           "reduce_partial", "reduce_combine", "Partial", "randn", "rand_uniform"]
+           "reduce_partial", "reduce_combine", "Partial", "randn", "rand_uniform", "dropout", "dropout_backward",
+           "layernorm_forward", "layernorm_backward", "gated_recurrence", "gated_recurrence_backward"]
 
 
 def _dtype(t: torch.Tensor) -> int:
@@ -684,3 +685,179 @@ def rand_uniform(shape, low: float = 0.0, high: float = 1.0, device="cuda", seed
     """Uniform float32 on [low, high) from the same counter-based stream (24 random
     bits per value)."""
     return _generate(1, shape, seed, offset, float(low), float(high), device)
+
+
+# ------------------------------------------------------------------- training
+# Operators that a model learns with (no counterpart in the reference, an inference
+# runtime). Backward passes are functions of their own: the caller keeps what the forward
+# pass returned and hands it over.
+def _check_floats(shape, device, **tensors) -> None:
+    """Each tensor that is not None: a contiguous float32 CUDA tensor of `shape`."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _check_tensor(t, name)
+        if t.dtype != torch.float32:
+            raise ValueError(f"{name} must be a float32 tensor")
+        if t.shape != shape:
+            raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+        if t.device != device:
+            raise ValueError(f"device mismatch: {name} is on {t.device}, not {device}")
+
+
+def _dropout_stream(p, seed, offset, device):
+    """(p, seed, offset, pointer of a device-side offset) as the C ABI takes them."""
+    if isinstance(p, (bool, np.bool_)) or not isinstance(p, (int, float, np.integer, np.floating)):
+        raise TypeError("dropout probability must be a real number")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("dropout probability must be in [0, 1]")
+    if p == 0.0:
+        return p, 0, 0, None  # nothing is drawn
+    if seed is None:
+        raise ValueError("dropout needs a seed: the backward pass makes the same mask from it")
+    seed = _seed_of(seed)
+    if isinstance(offset, torch.Tensor):
+        if offset.dtype != torch.int64 or offset.numel() != 1 or not offset.is_cuda or offset.device != device:
+            raise ValueError(f"a tensor offset must hold one int64 on {device}")
+        return p, seed, 0, _ptr(offset)
+    if isinstance(offset, (bool, np.bool_)) or not isinstance(offset, (int, np.integer)) or not 0 <= offset < 2**64:
+        raise ValueError("offset must be an integer in [0, 2**64), or an int64 tensor")
+    return p, seed, int(offset), None
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, *, offset=0, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """dropout(x), or residual + dropout(x) in one pass. Element i is kept when element
+    offset + i of rand_uniform's stream of `seed` is at least p, and then multiplied by
+    1 / (1 - p); a dropped element is 0 even when it is inf or NaN. The mask is never
+    stored: dropout_backward makes it again from the same seed and offset. `offset` is an
+    integer, or a CUDA int64 tensor of one element that is read when the kernel runs
+    (advance it between the replays of a captured graph)."""
+    _check_floats(getattr(x, "shape", None), getattr(x, "device", None), x=x, residual=residual)
+    p, seed, offset, step = _dropout_stream(p, seed, offset, x.device)
+    out = torch.empty_like(x)
+    check(lib().tcx_sm100_dropout(_stream(), _ptr(x), _ptr(residual), _ptr(out), x.numel(), p, seed, offset, step))
+    return out
+
+
+def dropout_backward(dy: torch.Tensor, p: float, seed: int, *, offset=0) -> torch.Tensor:
+    """The gradient of dropout with respect to x (the residual's is dy itself)."""
+    return dropout(dy, p, seed, offset=offset)
+
+
+def layernorm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                      eps: float = 1.0e-5, *, residual: torch.Tensor | None = None, p: float = 0.0,
+                      seed: int | None = None, offset=0):
+    """Layer norm over the last axis for training, in one pass with what stands in front of
+    it: total = residual + dropout(x), y = (total - mean) * rstd * weight + bias. Returns
+    (y, total, mean, rstd); mean and rstd have x's shape without its last axis, and total
+    is x itself without a residual and with p = 0. p, seed and offset as for dropout."""
+    _check_tensor(x, "x")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("layernorm_forward requires a non-empty last axis")
+    _check_floats(x.shape, x.device, x=x, residual=residual)
+    cols = x.shape[-1]
+    _check_floats((cols,), x.device, weight=weight, bias=bias)
+    e = plan.epsilon(eps)
+    p, seed, offset, step = _dropout_stream(p, seed, offset, x.device)
+    y = torch.empty_like(x)
+    total = torch.empty_like(x) if residual is not None or p > 0.0 else None
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    check(lib().tcx_sm100_layernorm_forward(
+        _stream(), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y), _ptr(total), _ptr(mean), _ptr(rstd),
+        x.numel() // cols, cols, e, p, seed, offset, step))
+    return y, x if total is None else total, mean, rstd
+
+
+def layernorm_backward(dy: torch.Tensor, total: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                       weight: torch.Tensor | None = None, *, dtotal: torch.Tensor | None = None, p: float = 0.0,
+                       seed: int | None = None, offset=0):
+    """The gradients of layernorm_forward from what it returned: (dx, dresidual, dweight,
+    dbias). dresidual is the gradient of total (dtotal, what reaches total by other ways,
+    added), and dx the same through the dropout: with p = 0 both are one tensor. Without a
+    weight dweight and dbias are None. Sums over rows have a fixed order."""
+    _check_tensor(total, "total")
+    if total.dim() == 0 or total.shape[-1] == 0:
+        raise ValueError("layernorm_backward requires a non-empty last axis")
+    _check_floats(total.shape, total.device, total=total, dy=dy, dtotal=dtotal)
+    cols = total.shape[-1]
+    _check_floats(total.shape[:-1], total.device, mean=mean, rstd=rstd)
+    _check_floats((cols,), total.device, weight=weight)
+    p, seed, offset, step = _dropout_stream(p, seed, offset, total.device)
+    rows = total.numel() // cols
+    dresidual = torch.empty_like(total)
+    dx = torch.empty_like(total) if p > 0.0 else None
+    dweight = dbias = keep = ws = None
+    ws_bytes = 0
+    if weight is not None:
+        dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
+        ws_bytes = lib().tcx_sm100_layernorm_backward_workspace_bytes(rows, cols)
+        keep, ws = _workspace(ws_bytes, total.device)
+    check(lib().tcx_sm100_layernorm_backward(
+        _stream(), _ptr(dy), _ptr(total), _ptr(mean), _ptr(rstd), _ptr(weight), _ptr(dtotal), _ptr(dresidual),
+        _ptr(dx), _ptr(dweight), _ptr(dbias), rows, cols, p, seed, offset, step, ws, ws_bytes))
+    del keep
+    return dresidual if dx is None else dx, dresidual, dweight, dbias
+
+
+def _recurrence_args(gate, form, lengths, **tensors):
+    if form not in RECURRENCE:
+        raise ValueError(f"recurrence form must be one of {sorted(RECURRENCE)}")
+    _check_tensor(gate, "gate")
+    if gate.dim() != 3:
+        raise ValueError("a recurrence runs over [batch, time, channels]")
+    _check_floats(gate.shape, gate.device, gate=gate, **tensors)
+    batch, time, channels = gate.shape
+    if lengths is not None:
+        _check_tensor(lengths, "lengths")
+        if lengths.dtype != torch.int32 or lengths.shape != (batch,) or lengths.device != gate.device:
+            raise ValueError(f"lengths must be an int32 tensor of shape ({batch},) on {gate.device}")
+    ws_bytes = lib().tcx_sm100_recurrence_workspace_bytes(batch, time, channels)
+    keep, ws = _workspace(ws_bytes, gate.device)
+    return batch, time, channels, keep, ws, ws_bytes
+
+
+def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, initial: torch.Tensor | None = None, *,
+                     form: str = "decay", lengths: torch.Tensor | None = None):
+    """A gated linear recurrence over [batch, time, channels], each channel by itself:
+    form "decay": h_t = gate_t * h_(t-1) + x_t; form "sigmoid": h_t = s_t * h_(t-1) +
+    (1 - s_t) * x_t with s = sigmoid(gate). It starts from `initial` [batch, channels]
+    (zeros without one). `lengths` (int32 [batch], clamped to [0, time]): steps that a
+    sequence does not have hold its state, whatever gate and x hold there. Returns (h,
+    state): every state, and the last one to go on from. With one step (a token of each
+    running sequence) state is a view of h."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a tensor")
+    batch, time, channels, keep, ws, ws_bytes = _recurrence_args(gate, form, lengths, x=x)
+    _check_floats((batch, channels), gate.device, initial=initial)
+    h = torch.empty_like(gate)
+    state = h.view(batch, channels) if time == 1 else torch.empty((batch, channels), dtype=torch.float32,
+                                                                  device=gate.device)
+    check(lib().tcx_sm100_recurrence_forward(
+        _stream(), RECURRENCE[form], _ptr(gate), _ptr(x), _ptr(initial), _ptr(lengths), _ptr(h),
+        None if time == 1 else _ptr(state), batch, time, channels, ws, ws_bytes))
+    del keep
+    return h, state
+
+
+def gated_recurrence_backward(dh: torch.Tensor, gate: torch.Tensor, x: torch.Tensor | None, h: torch.Tensor,
+                              initial: torch.Tensor | None = None, *, form: str = "decay",
+                              lengths: torch.Tensor | None = None, dstate: torch.Tensor | None = None):
+    """The gradients of gated_recurrence, (dgate, dx, dinitial), from dh (of every h_t),
+    dstate (of the state it returned; None: zeros), its arguments and its h. The decay form
+    does not read x (None will do). dinitial is None without an initial state."""
+    for name, t in (("dh", dh), ("h", h)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+    if form == "sigmoid" and x is None:
+        raise ValueError("the sigmoid form's gradient needs x")
+    batch, time, channels, keep, ws, ws_bytes = _recurrence_args(gate, form, lengths, dh=dh, x=x, h=h)
+    _check_floats((batch, channels), gate.device, initial=initial, dstate=dstate)
+    dgate, dx = torch.empty_like(gate), torch.empty_like(gate)
+    dinitial = None if initial is None else torch.empty_like(initial)
+    check(lib().tcx_sm100_recurrence_backward(
+        _stream(), RECURRENCE[form], _ptr(dh), _ptr(gate), _ptr(x), _ptr(h), _ptr(initial), _ptr(lengths),
+        _ptr(dstate), _ptr(dgate), _ptr(dx), _ptr(dinitial), batch, time, channels, ws, ws_bytes))
+    del keep
+    return dgate, dx, dinitial
