@@ -67,27 +67,6 @@ __device__ __forceinline__ void store(float* p, const float (&v)[VEC]) {
   else __stcs(p, v[0]);
 }
 
-// Loads and stores of values that other blocks of the grid write or read (L2, never L1).
-template <int VEC>
-__device__ __forceinline__ void load_shared(float (&v)[VEC], const float* p) {
-  if constexpr (VEC == 4) {
-    const float4 t = __ldcg(reinterpret_cast<const float4*>(p));
-    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-  } else if constexpr (VEC == 2) {
-    const float2 t = __ldcg(reinterpret_cast<const float2*>(p));
-    v[0] = t.x, v[1] = t.y;
-  } else {
-    v[0] = __ldcg(p);
-  }
-}
-
-template <int VEC>
-__device__ __forceinline__ void store_shared(float* p, const float (&v)[VEC]) {
-  if constexpr (VEC == 4) __stcg(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
-  else if constexpr (VEC == 2) __stcg(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
-  else __stcg(p, v[0]);
-}
-
 template <int VEC>
 __device__ __forceinline__ void start_of(float (&v)[VEC], const float* p, int64_t at) {
 #pragma unroll
@@ -177,235 +156,376 @@ __global__ void __launch_bounds__(256) walk_backward_kernel(Args a) {
 }
 
 // --------------------------------------------------------- scan over parts of the time
-// A sequence of one batch entry and 32 VEC channels (a chain) is cut into chunks of
-// kWarps * kSteps steps, a block to a chunk: each warp holds kSteps steps of its 32 VEC
-// channels in registers, so memory is read once and written once. A part's effect on a
-// state is (A, B): the product of its gates and its last state from zero. The warps' parts
-// meet in shared memory; the chunks' in the workspace: a block publishes its (A, B), walks
-// back over its chain's published parts to the nearest chunk whose last state is known,
-// advances that state through the parts between, and publishes its own. Chunks are handed
-// out in order of a ticket, so what a block waits for has always begun; the waits are
-// bounded all the same.
+// A sequence of one batch entry and 32 channels (a chain) is cut into chunks of time, a block
+// to a chunk at a time. A row of a chunk is 128 bytes: 32 / VEC lanes of a warp read it, so a
+// warp's lanes form VEC groups, and each group of each warp takes kSteps steps of its own.
+// Memory is read once and written once. A part's effect on a state is (A, B): the product of
+// its gates and its last state from zero. The groups' parts meet by shuffles, the warps' in
+// shared memory and the chunks' in the workspace: a block publishes its (A, B), walks back
+// over its chain's published parts to the nearest chunk whose last state is known, advances
+// that state through the parts between, and publishes its own. Blocks stay on their SM and
+// take chunks in order of a ticket, each in the order it got them, so what a block waits for
+// has always begun; the waits are bounded all the same. The next chunk's data come into
+// shared memory (cp.async; a thread copies and reads its own places only, so that needs no
+// barrier) as soon as the values there have been taken into registers or used.
 //
 // The state that enters a chunk is always the previous chunk's entering state advanced by
 // that chunk's (A, B), whether a published state or the parts themselves bring it: the
 // result does not depend on the order in which blocks run.
 //
 // Backward the same scan runs from the last step to the first, on c_t = a_t (c_(t+1) + dh_t).
-constexpr int kWarps = 8, kSteps = 8, kChunk = kWarps * kSteps;
-constexpr int64_t kWalkSteps = 16;  // up to so many steps a thread walks through time alone
+constexpr int kWide = 32;            // channels of a chain
+constexpr int64_t kWalkSteps = 16;   // up to so many steps a thread walks through time alone
+constexpr int kLeastChunk = 64;      // no shape has shorter chunks (the workspace is sized by it)
+
+template <int VEC, bool SIGMOID, bool BACK>
+struct Shape {
+  static constexpr int kWarps = 4, kPerSm = 3;
+  static constexpr int kSteps = 32 / VEC;      // of one group
+  static constexpr int kRing = BACK ? 1 : 2;   // chunks whose data are on their way
+  static constexpr int kChunk = kWarps * VEC * kSteps;
+  static constexpr int kArrays = BACK ? (SIGMOID ? 4 : 3) : 2;  // gate, x | gate, dh, the state before, x
+  static constexpr int kArray = kChunk * kWide, kPlace = kArrays * kArray, kBytes = kRing * kPlace * 4;
+  static_assert(kChunk >= kLeastChunk, "the workspace is sized for chunks of kLeastChunk steps or more");
+  static_assert(kBytes * kPerSm <= 216 * 1024, "the blocks of an SM share its memory");
+};
+
+// What a chunk tells the later ones about one channel, written and read in one 128-bit access.
+struct __align__(16) Record {
+  float A, B;      // its part's effect
+  float state;     // its last state
+  unsigned known;  // 0: nothing yet, 1: A and B, 2: the state
+};
 
 struct Scan {
   unsigned* ticket;
-  unsigned* flags;  // per chunk: 0 nothing, 1 parts, 2 the last state
-  float* parts;     // per chunk: A, then B
-  float* states;    // per chunk
-  int32_t blocks;   // channel blocks
-  int64_t chains, chunks;
+  Record* records;                         // [chain, chunk, kWide], zero at the start
+  unsigned blocks, chains, chunks, tiles;  // channel blocks; batch * blocks; per chain; in all
 };
 
-__device__ __forceinline__ unsigned load_flag(const unsigned* p) {
-  unsigned v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
+__device__ __forceinline__ void put(Record* p, float A, float B, float state, unsigned known) {
+  asm volatile("{\n .reg .b64 lo, hi;\n .reg .b128 v;\n mov.b64 lo, {%1, %2};\n mov.b64 hi, {%3, %4};\n"
+               " mov.b128 v, {lo, hi};\n st.relaxed.gpu.global.b128 [%0], v;\n}\n" ::"l"(p), "f"(A), "f"(B), "f"(state),
+               "r"(known)
+               : "memory");
+}
+__device__ __forceinline__ Record get(const Record* p) {
+  Record r;
+  asm volatile("{\n .reg .b64 lo, hi;\n .reg .b128 v;\n ld.relaxed.gpu.global.b128 v, [%4];\n mov.b128 {lo, hi}, v;\n"
+               " mov.b64 {%0, %1}, lo;\n mov.b64 {%2, %3}, hi;\n}\n"
+               : "=f"(r.A), "=f"(r.B), "=f"(r.state), "=r"(r.known)
+               : "l"(p)
+               : "memory");
+  return r;
 }
 
-// By one warp, after its lanes' store_shared.
-__device__ __forceinline__ void publish(unsigned* flag, unsigned value, int lane) {
-  __threadfence();
-  __syncwarp();
-  if (lane == 0) asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(value) : "memory");
-}
-
-// How many chunks before `chunk` have to be advanced through to reach it from a known state
-// (that of chunk - 1 - result, or the sequence's start when that is -1). One warp.
-__device__ int64_t walk_back(const unsigned* flags, int64_t chunk, int lane, int* err) {
-  int64_t depth = 0;
+// The state that enters chunk `chunk` > 0 of a chain, a lane to a channel; `start` is the
+// sequence's, `mine` the lane's record of the chunk. Looks at kLook chunks at a time.
+constexpr int kLook = 8;
+__device__ float enter(const Record* mine, int chunk, float start, int lane, int* err) {
   uint64_t began = 0;
-  for (;;) {
-    const int64_t at = chunk - 1 - depth - lane;
-    const unsigned f = at < 0 ? 2u : load_flag(flags + at);
-    const unsigned known = __ballot_sync(0xffffffffu, f == 2u), there = __ballot_sync(0xffffffffu, f != 0u);
-    if (known) {
-      const int j = __ffs(known) - 1;
-      const unsigned need = (1u << j) - 1u;
-      if ((there & need) == need) return depth + j;
-    } else if (there == 0xffffffffu) {
-      depth += 32;
-      continue;
+  for (int depth = 0;;) {  // chunks that are known to have parts, nearest first
+    Record r[kLook];
+#pragma unroll
+    for (int j = 0; j < kLook; ++j) {
+      const int back = depth + j + 1;
+      r[j].known = 2u, r[j].state = start, r[j].A = 1.0f, r[j].B = 0.0f;
+      if (back <= chunk) r[j] = get(mine - static_cast<int64_t>(back) * kWide);
+    }
+    unsigned known = 0, there = 0;  // bit j: every lane sees it
+#pragma unroll
+    for (int j = 0; j < kLook; ++j) {
+      known |= (__all_sync(0xffffffffu, r[j].known == 2u) ? 1u : 0u) << j;
+      there |= (__all_sync(0xffffffffu, r[j].known != 0u) ? 1u : 0u) << j;
+    }
+    const int at = __ffs(known) - 1;
+    const unsigned need = known ? (1u << at) - 1u : (1u << kLook) - 1u;
+    if ((there & need) == need) {
+      if (!known) {
+        depth += kLook;
+        continue;
+      }
+      float h = 0.0f;
+#pragma unroll
+      for (int j = kLook - 1; j >= 0; --j) {
+        if (j == at) h = r[j].state;
+        if (j < at) h = advance(h, r[j].A, r[j].B);
+      }
+#pragma unroll 4
+      for (int back = depth; back > 0; --back) {
+        const Record q = get(mine - static_cast<int64_t>(back) * kWide);
+        h = advance(h, q.A, q.B);
+      }
+      return h;
     }
     const uint64_t now = ptx::globaltimer();
     if (!began) began = now;
     if (__any_sync(0xffffffffu, now - began > ptx::kWaitLimitNs)) {
       if (lane == 0) record_device_error(err, 0x501);
-      return 0;
+      return start;
     }
   }
 }
 
-template <int VEC, bool SIGMOID, bool BACK>
-__global__ void __launch_bounds__(kWarps * 32, 2) scan_kernel(Args a, Scan sc, int* err) {
-  constexpr int kWide = 32 * VEC;
-  __shared__ __align__(16) float part[kWarps][2][kWide];
-  __shared__ __align__(16) float entry[kWide], ended[kWide];
-  __shared__ unsigned mine;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) mine = atomicAdd(sc.ticket, 1u);
-  __syncthreads();
-  const int64_t chain = mine % sc.chains, chunk = mine / sc.chains;
-  const int64_t b = chain / sc.blocks, c0 = (chain % sc.blocks) * kWide + lane * VEC;
-  const bool inside = c0 < a.channels;
-  const int64_t n = length_of(a, b);
-  const int64_t first = chunk * kChunk + warp * kSteps;  // in the scan's own order
-  const int64_t base = b * a.time * a.channels + c0;
-  auto step_of = [&](int s) { return BACK ? a.time - 1 - (first + s) : first + s; };
+// Copies VEC floats to shared memory, or zeros.
+template <int VEC>
+__device__ __forceinline__ void copy_async(uint32_t to, const float* from, bool there) {
+  const int bytes = there ? 4 * VEC : 0;
+  if constexpr (VEC == 4)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+  else if constexpr (VEC == 2)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
 
-  float g[kSteps][VEC], v[kSteps][VEC];  // gate and x, or gate and dh
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const int64_t t = step_of(s);
-    const bool in = inside && first + s < a.time;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) g[s][i] = BACK && SIGMOID ? 0.0f : 1.0f, v[s][i] = 0.0f;
-    if (in && t < n) load<VEC>(g[s], a.gate + base + t * a.channels);
-    if (in && (BACK || t < n)) load<VEC>(v[s], (BACK ? a.dh : a.x) + base + t * a.channels);
+template <int VEC>
+__device__ __forceinline__ void load_place(float (&v)[VEC], const float* p) {
+  if constexpr (VEC == 4) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+  } else if constexpr (VEC == 2) {
+    const float2 t = *reinterpret_cast<const float2*>(p);
+    v[0] = t.x, v[1] = t.y;
+  } else {
+    v[0] = *p;
   }
-  float A[VEC], B[VEC];
+}
+
+// A thread's share of a chunk: kSteps steps of VEC channels.
+struct Share {
+  unsigned tile, chain, chunk;
+  int64_t b, c;      // batch entry, first channel
+  int64_t n, first;  // the sequence's length, the first step in the scan's own order
+  int64_t at;        // of the first step in the arrays
+  bool inside, full;  // the channels exist; so do all the steps
+};
+
+template <int VEC, bool SIGMOID, bool BACK>
+__device__ __forceinline__ Share share_of(const Args& a, const Scan& sc, unsigned tile, int column, int before_me) {
+  using Sh = Shape<VEC, SIGMOID, BACK>;
+  Share m;
+  m.tile = tile;
+  m.chunk = tile / sc.chains;
+  m.chain = tile - m.chunk * sc.chains;
+  const unsigned b = m.chain / sc.blocks;
+  m.b = b;
+  m.c = static_cast<int64_t>(m.chain - b * sc.blocks) * kWide + column;
+  m.n = length_of(a, m.b);
+  m.first = static_cast<int64_t>(m.chunk) * Sh::kChunk + before_me;
+  const int64_t t = BACK ? a.time - 1 - m.first : m.first;
+  m.at = (m.b * a.time + t) * a.channels + m.c;
+  m.inside = m.c < a.channels;
+  m.full = m.inside && m.first + Sh::kSteps <= a.time && (BACK ? t < m.n : t + Sh::kSteps <= m.n);
+  return m;
+}
+
+template <int VEC, bool SIGMOID, bool BACK>
+__global__ void __launch_bounds__(Shape<VEC, SIGMOID, BACK>::kWarps * 32, Shape<VEC, SIGMOID, BACK>::kPerSm)
+scan_kernel(Args a, Scan sc, int* err) {
+  using Sh = Shape<VEC, SIGMOID, BACK>;
+  constexpr int kWarps = Sh::kWarps, kSteps = Sh::kSteps, kChunk = Sh::kChunk, kArray = Sh::kArray, kRing = Sh::kRing;
+  constexpr int kRow = 32 / VEC;       // lanes of a row
+  constexpr int kNext = 32 * VEC;      // from one step's place in shared memory to the next one's
+  extern __shared__ __align__(16) float stage[];
+  __shared__ float parts[kWarps][2][kWide];
+  __shared__ __align__(16) float entries[kWarps][kWide], ended[kWide];
+  __shared__ unsigned queue[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = lane / kRow;
+  const int column = (lane % kRow) * VEC;              // within the chain
+  const int before_me = (warp * VEC + group) * kSteps;  // steps of the chunk
+  float* const place = stage + (warp * kSteps * 32 + lane) * VEC;
+  const uint32_t place_at = ptx::smem_u32(place);
+  const int64_t stride = BACK ? -a.channels : a.channels;
+
+  // Step s of the share exists; the sequence has it.
+  auto exists = [&](const Share& m, int s) { return m.full || (m.inside && m.first + s < a.time); };
+  auto lives = [&](const Share& m, int s) {
+    return m.full || (m.first + s < a.time && (BACK ? a.time - 1 - (m.first + s) : m.first + s) < m.n);
+  };
+  // What the parts are made from: gate and x, or gate and dh.
+  auto fetch = [&](const Share& m, unsigned turn) {
+    if (m.tile < sc.tiles) {
+      const uint32_t to = place_at + (turn % kRing) * (Sh::kPlace * 4);
+      const float *p = a.gate + m.at, *q = (BACK ? a.dh : a.x) + m.at;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) A[i] = 1.0f, B[i] = 0.0f;
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    const bool live = first + s < a.time && step_of(s) < n;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      if (BACK) {
-        float s1 = g[s][i], rest;
-        if (SIGMOID) sigmoid_pair(s1, s1, rest);
-        if (!live) s1 = 1.0f;
-        A[i] *= s1;
-        B[i] = s1 * (B[i] + v[s][i]);
-      } else {
-        if (SIGMOID && live) {
-          float rest;
-          sigmoid_pair(g[s][i], g[s][i], rest);
-          v[s][i] *= rest;
-        }
-        A[i] *= g[s][i];
-        B[i] = fmaf(g[s][i], B[i], v[s][i]);
+      for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
+        const bool live = m.inside && lives(m, s);
+        copy_async<VEC>(to + 4 * s * kNext, live ? p : a.gate, live);
+        const bool has = BACK ? exists(m, s) : live;
+        copy_async<VEC>(to + 4 * (kArray + s * kNext), has ? q : a.gate, has);
       }
     }
-  }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // What a backward chunk needs besides once its entering state is known.
+  auto fetch_rest = [&](const Share& m) {
+    if (m.tile < sc.tiles) {
+      const float *p = a.hs + m.at - a.channels, *q = SIGMOID ? a.x + m.at : nullptr;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) part[warp][0][lane * VEC + i] = A[i], part[warp][1][lane * VEC + i] = B[i];
-  __syncthreads();
+      for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
+        const bool live = m.inside && lives(m, s), opening = m.first + s == a.time - 1;  // t = 0
+        const bool has = live && (!opening || a.initial);
+        copy_async<VEC>(place_at + 4 * (2 * kArray + s * kNext),
+                        !has ? a.gate : opening ? a.initial + m.b * a.channels + m.c : p, has);
+        if constexpr (SIGMOID) copy_async<VEC>(place_at + 4 * (3 * kArray + s * kNext), live ? q : a.gate, live);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 
-  // A forward chunk in which the sequence ends: what is held after it is the state itself,
-  // not one advanced by (A, B), so this chunk publishes that state alone.
-  const bool ends = !BACK && n < a.time && n > chunk * kChunk && n <= chunk * kChunk + kChunk;
-  const int64_t row = chain * sc.chunks + chunk;
-  unsigned* flag = sc.flags + row;
-  if (warp == 0) {
-    float h[VEC];
+  Share line[kRing];  // this chunk and those whose data are on their way
+#pragma unroll
+  for (int k = 0; k < kRing; ++k) {
+    if (threadIdx.x == 0) queue[k & 1] = atomicAdd(sc.ticket, 1u);
+    __syncthreads();
+    line[k] = share_of<VEC, SIGMOID, BACK>(a, sc, queue[k & 1], column, before_me);
+    fetch(line[k], k);
+  }
+  if (BACK) fetch_rest(line[0]);
+  unsigned later = threadIdx.x == 0 ? atomicAdd(sc.ticket, 1u) : 0;
+  __syncthreads();
+  for (unsigned turn = 0; line[0].tile < sc.tiles; ++turn) {  // tickets past the end stay past it
+    const Share m = line[0];
+    const float* const here = place + (turn % kRing) * Sh::kPlace;
+    asm volatile("cp.async.wait_group %0;" ::"n"(BACK ? 1 : kRing - 1) : "memory");
+    float g[kSteps][VEC], v[kSteps][VEC];  // gate and x, or gate and dh
+    float A[VEC], B[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) A[i] = 1.0f, B[i] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w)
+    for (int s = 0; s < kSteps; ++s) {
+      load_place<VEC>(g[s], here + s * kNext);
+      load_place<VEC>(v[s], here + kArray + s * kNext);
+      const bool live = lives(m, s);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float wa = part[w][0][lane * VEC + i];
-        A[i] *= wa;
-        B[i] = fmaf(wa, B[i], part[w][1][lane * VEC + i]);
-      }
-    int64_t depth = 0;
-    if (chunk > 0) {
-      if (!ends && load_flag(flag - 1) != 2u) {
-        store_shared<VEC>(sc.parts + row * 2 * kWide + lane * VEC, A);
-        store_shared<VEC>(sc.parts + row * 2 * kWide + kWide + lane * VEC, B);
-        publish(flag, 1u, lane);
-      }
-      depth = walk_back(flag - chunk, chunk, lane, err);
-    }
-    if (chunk - depth > 0) {
-      load_shared<VEC>(h, sc.states + (row - 1 - depth) * kWide + lane * VEC);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[i] = 0.0f;
-      if (inside) start_of<VEC>(h, BACK ? a.dstate : a.initial, b * a.channels + c0);
-    }
-#pragma unroll 4
-    for (int64_t q = row - depth; q < row; ++q) {
-      float qa[VEC], qb[VEC];
-      load_shared<VEC>(qa, sc.parts + q * 2 * kWide + lane * VEC);
-      load_shared<VEC>(qb, sc.parts + q * 2 * kWide + kWide + lane * VEC);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[i] = advance(h[i], qa[i], qb[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) entry[lane * VEC + i] = h[i];
-    if (chunk + 1 < sc.chunks && !ends) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[i] = advance(h[i], A[i], B[i]);
-      store_shared<VEC>(sc.states + row * kWide + lane * VEC, h);
-      publish(flag, 2u, lane);
-    }
-  }
-  __syncthreads();
-  float h[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) h[i] = entry[lane * VEC + i];
-  for (int w = 0; w < warp; ++w)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) h[i] = advance(h[i], part[w][0][lane * VEC + i], part[w][1][lane * VEC + i]);
-
-  if constexpr (BACK) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int64_t t = step_of(s);
-      if (!inside || first + s >= a.time) continue;
-      const int64_t at = base + t * a.channels;
-      Reads<VEC, SIGMOID> r = {};
-      if (t < n) {
-        if (t) load<VEC>(r.before, a.hs + at - a.channels);
-        else start_of<VEC>(r.before, a.initial, b * a.channels + c0);
-        if constexpr (SIGMOID) load<VEC>(r.x, a.x + at);
-      }
-      float dgate[VEC], dx[VEC];
-      backward_step<VEC, SIGMOID>(g[s], v[s], r, t < n, h, dgate, dx);
-      store<VEC>(a.dgate + at, dgate);
-      store<VEC>(a.dx + at, dx);
-    }
-  } else {
-    auto write = [&](int s) {
-      const int64_t t = first + s;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[i] = fmaf(g[s][i], h[i], v[s][i]);
-      if (inside && t < a.time) store<VEC>(a.h + base + t * a.channels, h);
-    };
-    const bool held = ends && first >= n;  // this warp's steps come after the end
-    if (!held) {
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) write(s);
-    }
-    if (ends) {
-      if (n > first && n <= first + kSteps) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) ended[lane * VEC + i] = h[i];
-        if (chunk + 1 < sc.chunks) {
-          store_shared<VEC>(sc.states + row * kWide + lane * VEC, h);
-          publish(flag, 2u, lane);
+        if (BACK) {
+          float s1 = g[s][i], rest;
+          if (SIGMOID) sigmoid_pair(s1, s1, rest);
+          if (!live) s1 = 1.0f;
+          A[i] *= s1;
+          B[i] = s1 * (B[i] + v[s][i]);
+        } else {
+          if (SIGMOID) {
+            float rest;
+            sigmoid_pair(g[s][i], g[s][i], rest);
+            v[s][i] *= rest;
+          }
+          if (!live) g[s][i] = 1.0f;  // and v is 0
+          A[i] *= g[s][i];
+          B[i] = fmaf(g[s][i], B[i], v[s][i]);
         }
       }
-      __syncthreads();
-      if (held) {
+    }
+    // the groups before this one, then with it; the last group has the warp's part
+    float eA[VEC], eB[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) h[i] = ended[lane * VEC + i];
+    for (int i = 0; i < VEC; ++i) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) write(s);
+      for (int off = 1; off < VEC; off *= 2) {
+        const float pa = __shfl_up_sync(0xffffffffu, A[i], off * kRow), pb = __shfl_up_sync(0xffffffffu, B[i], off * kRow);
+        if (group >= off) {
+          B[i] = fmaf(A[i], pb, B[i]);
+          A[i] *= pa;
+        }
+      }
+      eA[i] = eB[i] = 0.0f;
+      if (VEC > 1) {
+        eA[i] = __shfl_up_sync(0xffffffffu, A[i], kRow);
+        eB[i] = __shfl_up_sync(0xffffffffu, B[i], kRow);
+      }
+      if (group == VEC - 1) parts[warp][0][column + i] = A[i], parts[warp][1][column + i] = B[i];
+    }
+    if (threadIdx.x == 0) queue[0] = later;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k + 1 < kRing; ++k) line[k] = line[k + 1];
+    line[kRing - 1] = share_of<VEC, SIGMOID, BACK>(a, sc, queue[0], column, before_me);
+
+    // A forward chunk in which the sequence ends: what is held after it is the state itself,
+    // not one advanced by (A, B), so this chunk publishes that state alone.
+    const int64_t opens = m.first - before_me;
+    const bool ends = !BACK && m.n < a.time && m.n > opens && m.n <= opens + kChunk;
+    Record* const record = sc.records + (static_cast<int64_t>(m.chain) * sc.chunks + m.chunk) * kWide;
+    if (warp == 0) {  // a lane to a channel
+      float wA = 1.0f, wB = 0.0f, state = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        wB = fmaf(parts[w][0][lane], wB, parts[w][1][lane]);
+        wA *= parts[w][0][lane];
+      }
+      const int64_t channel = m.c - column + lane;
+      const float* start = BACK ? a.dstate : a.initial;
+      if (start && channel < a.channels) state = __ldg(start + m.b * a.channels + channel);
+      const bool goes_on = m.chunk + 1 < sc.chunks && !ends;
+      if (m.chunk > 0) {
+        if (goes_on) put(record + lane, wA, wB, 0.0f, 1u);
+        state = enter(record + lane, static_cast<int>(m.chunk), state, lane, err);
+      }
+      if (goes_on) put(record + lane, wA, wB, advance(state, wA, wB), 2u);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        entries[w][lane] = state;
+        state = advance(state, parts[w][0][lane], parts[w][1][lane]);
       }
     }
+    fetch(line[kRing - 1], turn);
+    if (threadIdx.x == 0) later = atomicAdd(sc.ticket, 1u);
+    __syncthreads();
+    float h[VEC];
+    load_place<VEC>(h, &entries[warp][column]);
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[i] = advance(h[i], eA[i], eB[i]);
+    }
+
+    if constexpr (BACK) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      float *p = a.dgate + m.at, *q = a.dx + m.at;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
+        Reads<VEC, SIGMOID> r;
+        load_place<VEC>(r.before, place + 2 * kArray + s * kNext);
+        if constexpr (SIGMOID) load_place<VEC>(r.x, place + 3 * kArray + s * kNext);
+        if (!exists(m, s)) continue;
+        float dgate[VEC], dx[VEC];
+        backward_step<VEC, SIGMOID>(g[s], v[s], r, lives(m, s), h, dgate, dx);
+        store<VEC>(p, dgate);
+        store<VEC>(q, dx);
+      }
+      fetch_rest(line[0]);
+    } else {
+      auto write = [&]() {
+        float* p = a.h + m.at;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s, p += stride) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) h[i] = fmaf(g[s][i], h[i], v[s][i]);
+          if (exists(m, s)) store<VEC>(p, h);
+        }
+      };
+      const bool held = ends && m.first >= m.n;  // this group's steps come after the end
+      if (!held) write();
+      if (ends) {
+        if (m.n > m.first && m.n <= m.first + kSteps) {  // the group that has the last step
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            ended[column + i] = h[i];
+            if (m.chunk + 1 < sc.chunks) put(record + column + i, 1.0f, 0.0f, h[i], 2u);
+          }
+        }
+        __syncthreads();
+        if (held) {
+          load_place<VEC>(h, ended + column);
+          write();
+        }
+      }
+    }
+    float* last = BACK ? a.dinitial : a.state;
+    if (last && m.inside && m.first < a.time && m.first + kSteps >= a.time)
+      store<VEC>(last + m.b * a.channels + m.c, h);
   }
-  float* last = BACK ? a.dinitial : a.state;
-  if (last && inside && first < a.time && first + kSteps >= a.time) store<VEC>(last + b * a.channels + c0, h);
 }
 
 // ------------------------------------------------------------------------- launches
@@ -413,17 +533,14 @@ bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) 
 
 // Channels per thread: as wide as the channel count and every buffer's alignment allow.
 int width_of(const Args& a) {
-  const void* all[] = {a.gate, a.x, a.h, a.state, a.dh, a.hs, a.dgate, a.dx, a.dinitial};
+  const void* all[] = {a.gate, a.x, a.initial, a.h, a.state, a.dh, a.hs, a.dstate, a.dgate, a.dx, a.dinitial};
   for (int vec = 4; vec > 1; vec /= 2) {
     bool fits = a.channels % vec == 0;
     for (const void* p : all) fits = fits && aligned(p, 4 * vec);
-    // half a warp's lanes would stand idle: take narrower ones
-    if (fits && (a.channels > 16 * vec || vec == 1)) return vec;
+    if (fits) return vec;
   }
   return 1;
 }
-
-int64_t chains_of(int64_t batch, int64_t channels, int vec) { return batch * ceil_div(channels, 32 * vec); }
 
 template <int VEC, bool SIGMOID, bool BACK>
 int launch(cudaStream_t s, const Args& a, void* workspace) {
@@ -434,20 +551,30 @@ int launch(cudaStream_t s, const Args& a, void* workspace) {
     else walk_forward_kernel<VEC, SIGMOID><<<grid, 256, 0, s>>>(a);
     return launch_status("recurrence");
   }
-  Scan sc;
-  sc.blocks = static_cast<int32_t>(ceil_div(a.channels, 32 * VEC));
-  sc.chains = a.batch * sc.blocks;
-  sc.chunks = ceil_div(a.time, kChunk);
-  const int64_t tiles = sc.chains * sc.chunks;
+  using Sh = Shape<VEC, SIGMOID, BACK>;
+  const int64_t blocks = ceil_div(a.channels, kWide), chunks = ceil_div(a.time, Sh::kChunk);
+  const int64_t tiles = a.batch * blocks * chunks;
   if (tiles > INT32_MAX) return invalid("recurrence is too large for one call");
-  float* f = static_cast<float*>(workspace);
-  sc.parts = f;
-  sc.states = f + tiles * 64 * VEC;
-  sc.flags = reinterpret_cast<unsigned*>(sc.states + tiles * 32 * VEC);
-  sc.ticket = sc.flags + tiles;
-  cudaMemsetAsync(sc.flags, 0, (tiles + 1) * sizeof(unsigned), s);
+  Scan sc;
+  sc.blocks = static_cast<unsigned>(blocks);
+  sc.chains = static_cast<unsigned>(a.batch * blocks);
+  sc.chunks = static_cast<unsigned>(chunks);
+  sc.tiles = static_cast<unsigned>(tiles);
+  sc.records = static_cast<Record*>(workspace);
+  sc.ticket = reinterpret_cast<unsigned*>(sc.records + tiles * kWide);
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+    if (cudaFuncSetAttribute(scan_kernel<VEC, SIGMOID, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Sh::kBytes) != cudaSuccess)
+      return launch_status("recurrence shared memory attribute");
+    attr_done[dev] = true;
+  }
+  cudaMemsetAsync(workspace, 0, tiles * kWide * sizeof(Record) + sizeof(unsigned), s);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, Sh::kPerSm * sm_count()));
   TimedLaunch timer(BACK ? "recurrence_scan_backward" : "recurrence_scan", s);
-  scan_kernel<VEC, SIGMOID, BACK><<<static_cast<unsigned>(tiles), kWarps * 32, 0, s>>>(a, sc, device_error_word());
+  scan_kernel<VEC, SIGMOID, BACK><<<grid, Sh::kWarps * 32, Sh::kBytes, s>>>(a, sc, device_error_word());
   return launch_status("recurrence");
 }
 
@@ -483,11 +610,9 @@ using namespace tcx;
 
 extern "C" size_t tcx_sm100_recurrence_workspace_bytes(int64_t batch, int64_t time, int64_t channels) {
   if (check_recurrence(TCX_RECURRENCE_DECAY, batch, time, channels) || time <= kWalkSteps) return 0;
-  // three values per channel and chunk, and a flag per chunk: the narrowest blocks have the
-  // most flags, the widest the most channels past the end
-  const int64_t chunks = ceil_div(time, kChunk);
-  return static_cast<size_t>(chains_of(batch, channels, 4) * 128 * 3 * chunks + chains_of(batch, channels, 1) * chunks +
-                             1) * sizeof(float);
+  // a record per channel for each chunk, and the ticket
+  const int64_t tiles = batch * ceil_div(channels, kWide) * ceil_div(time, kLeastChunk);
+  return static_cast<size_t>(tiles) * kWide * sizeof(Record) + sizeof(unsigned);
 }
 
 extern "C" int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const float* gate, const float* x,
