@@ -17,6 +17,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -180,7 +181,7 @@ constexpr int kLeastChunk = 64;      // no shape has shorter chunks (the workspa
 
 template <int VEC, bool SIGMOID, bool BACK>
 struct Shape {
-  static constexpr int kWarps = 4, kPerSm = 3;
+  static constexpr int kWarps = 4, kPerSm = 3, kThreads = kWarps * 32;
   static constexpr int kSteps = 32 / VEC;      // of one group
   static constexpr int kRing = BACK ? 1 : 2;   // chunks whose data are on their way
   static constexpr int kChunk = kWarps * VEC * kSteps;
@@ -290,6 +291,13 @@ __device__ __forceinline__ void load_place(float (&v)[VEC], const float* p) {
   } else {
     v[0] = *p;
   }
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_place(float* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else if constexpr (VEC == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+  else *p = v[0];
 }
 
 // A thread's share of a chunk: kSteps steps of VEC channels.
@@ -528,6 +536,294 @@ scan_kernel(Args a, Scan sc, int* err) {
   }
 }
 
+// ---------------------------------------------------------------- the forward scan
+// The same scan with the walk back taken out of the blocks' way: kWarps warps make the parts
+// of chunk i + 1 and then write the states of chunk i, while two more warps publish the parts
+// (the teller) and bring the state that enters chunk i + 1 (the carrier). The values wait in
+// shared memory between the two uses, in the places that the next chunks' data come into.
+template <int VEC>
+struct Forward {
+  static constexpr int kWarps = 4, kRing = 3, kPerSm = 2;
+  static constexpr int kSteps = 32 / VEC;  // of one group
+  static constexpr int kChunk = kWarps * VEC * kSteps;
+  static constexpr int kArray = kChunk * kWide, kPlace = 2 * kArray, kBytes = kRing * kPlace * 4;  // gate, x
+  static constexpr int kThreads = (kWarps + 2) * 32;
+  static_assert(kChunk >= kLeastChunk, "the workspace is sized for chunks of kLeastChunk steps or more");
+  static_assert(kBytes * kPerSm <= 216 * 1024, "the blocks of an SM share its memory");
+};
+
+// A chunk as its block sees it.
+struct Tile {
+  int64_t at;            // of its first step and channel in the arrays
+  int64_t edge;          // of its first channel in the states
+  int channels, steps;   // that exist, of kWide and kChunk; no channels: there is no such chunk
+  int live;              // steps that the sequence has
+  unsigned row, chunk;   // its records; its place in the chain
+  int ends, last;        // the sequence ends in it, before time does; no chunk comes after it
+};
+
+// The block's chunk number i. With records: the one that a ticket names. Without: whole chains,
+// chunk after chunk.
+template <int VEC, bool WHOLE>
+__device__ Tile next_tile(const Args& a, const Scan& sc, unsigned i) {
+  using F = Forward<VEC>;
+  Tile m = {};
+  unsigned chain;
+  if (!WHOLE) {
+    const unsigned tile = atomicAdd(sc.ticket, 1u);
+    if (tile >= sc.tiles) return m;
+    m.chunk = tile / sc.chains;
+    chain = tile - m.chunk * sc.chains;
+  } else {
+    const unsigned turn = i / sc.chunks;
+    m.chunk = i - turn * sc.chunks;
+    chain = blockIdx.x + turn * gridDim.x;
+    if (chain >= sc.chains) return m;
+  }
+  const unsigned b = chain / sc.blocks, block = chain - b * sc.blocks;
+  const int64_t n = length_of(a, b), opens = static_cast<int64_t>(m.chunk) * F::kChunk;
+  const int64_t c = static_cast<int64_t>(block) * kWide;
+  m.at = (b * a.time + opens) * a.channels + c;
+  m.edge = b * a.channels + c;
+  m.channels = static_cast<int>(min(a.channels - c, static_cast<int64_t>(kWide)));
+  m.steps = static_cast<int>(min(a.time - opens, static_cast<int64_t>(F::kChunk)));
+  m.live = static_cast<int>(max(min(n - opens, static_cast<int64_t>(F::kChunk)), static_cast<int64_t>(0)));
+  m.row = chain * sc.chunks + m.chunk;
+  m.ends = n < a.time && n > opens && n <= opens + F::kChunk;
+  m.last = m.chunk + 1 == sc.chunks;
+  return m;
+}
+
+// Barriers between the warps that work and the carrier, two of each by the chunk's parity.
+enum { kPartsMade = 1, kEntryKnown = 3, kEndKnown = 5, kEndTold = 6, kPartsTold = 7 };
+__device__ __forceinline__ void meet(int barrier, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void signal(int barrier, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+}
+
+template <int VEC, bool SIGMOID, bool WHOLE>
+__global__ void __launch_bounds__(Forward<VEC>::kThreads, Forward<VEC>::kPerSm)
+scan_forward_kernel(Args a, Scan sc, int* err) {
+  using F = Forward<VEC>;
+  constexpr int kWarps = F::kWarps, kSteps = F::kSteps, kRing = F::kRing, kArray = F::kArray;
+  constexpr int kAll = (kWarps + 1) * 32;  // the warps that work, and one of the two others
+  constexpr int kRow = 32 / VEC, kNext = 32 * VEC;
+  extern __shared__ __align__(16) float stage[];
+  __shared__ float parts[2][kWarps][2][kWide], joined[2][2][kWide];  // the warps' and the chunk's
+  __shared__ __align__(16) float entries[2][kWarps][kWide], ended[kWide];
+  // Chunk i's at i % 8. The carrier sets i's in its turn i - kRing, before it signals that
+  // turn's entry. The warps that work see that signal before they make chunk i - 1's parts
+  // (kRing >= 3), and the teller reads i's after those were made; the slots in use at a time
+  // are those from one chunk behind the carrier's to kRing beyond it.
+  __shared__ Tile line[8];
+  static_assert(kRing >= 3 && kRing + 3 <= 8, "a chunk's line is set before it is read, and kept until it is done");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  if (warp == kWarps + 1) {  // the teller
+    for (int k = 0; k < kRing; ++k) __syncthreads();
+    for (unsigned i = 0;; ++i) {
+      const Tile& m = line[i & 7];
+      if (m.channels == 0) return;
+      meet(kPartsMade + (i & 1), kAll);
+      const float (*part)[2][kWide] = parts[i & 1];
+      float A = 1.0f, B = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        B = fmaf(part[w][0][lane], B, part[w][1][lane]);
+        A *= part[w][0][lane];
+      }
+      joined[i & 1][0][lane] = A;
+      joined[i & 1][1][lane] = B;
+      if (!WHOLE && m.chunk > 0 && !m.last && !m.ends)
+        put(sc.records + static_cast<int64_t>(m.row) * kWide + lane, A, B, 0.0f, 1u);
+      signal(kPartsTold + (i & 1), 64);
+    }
+  }
+  if (warp == kWarps) {  // the carrier
+    for (int k = 0; k < kRing; ++k) {
+      if (lane == 0) line[k] = next_tile<VEC, WHOLE>(a, sc, k);
+      __syncthreads();
+    }
+    float state = 0.0f;
+    bool ended_before = false;
+    for (unsigned i = 0;; ++i) {
+      const Tile m = line[i & 7];
+      if (m.channels == 0) return;
+      if (lane == 0) line[(i + kRing) & 7] = next_tile<VEC, WHOLE>(a, sc, i + kRing);
+      const float start = a.initial && lane < m.channels ? __ldg(a.initial + m.edge + lane) : 0.0f;
+      meet(kPartsTold + (i & 1), 64);
+      const float (*part)[2][kWide] = parts[i & 1];
+      const float A = joined[i & 1][0][lane], B = joined[i & 1][1][lane];
+      if (!WHOLE) {
+        Record* const record = sc.records + static_cast<int64_t>(m.row) * kWide + lane;
+        state = m.chunk > 0 ? enter(record, static_cast<int>(m.chunk), start, lane, err) : start;
+        if (!m.last && !m.ends) put(record, A, B, advance(state, A, B), 2u);
+      } else {
+        if (ended_before) {
+          meet(kEndTold, kAll);
+          state = ended[lane];
+        }
+        if (m.chunk == 0) state = start;
+        ended_before = m.ends && !m.last;
+      }
+      float h = state;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        entries[i & 1][w][lane] = h;
+        h = advance(h, part[w][0][lane], part[w][1][lane]);
+      }
+      state = advance(state, A, B);
+      __syncwarp();
+      signal(kEntryKnown + (i & 1), kAll);
+    }
+  }
+
+  const int group = lane / kRow, column = (lane % kRow) * VEC;
+  const int before_me = (warp * VEC + group) * kSteps;  // steps of the chunk
+  float* const places = stage + (warp * kSteps * 32 + lane) * VEC;
+  const uint32_t places_at = ptx::smem_u32(places);
+  const int64_t mine = before_me * a.channels + column;
+
+  auto fetch = [&](unsigned i) {
+    const Tile& m = line[i & 7];
+    if (m.channels) {
+      const float *p = a.gate + m.at + mine, *q = a.x + m.at + mine;
+      const uint32_t to = places_at + (i % kRing) * (F::kPlace * 4);
+      if (column < m.channels && before_me + kSteps <= m.live) {
+#pragma unroll 8
+        for (int s = 0; s < kSteps; ++s, p += a.channels, q += a.channels) {
+          copy_async<VEC>(to + 4 * s * kNext, p, true);
+          copy_async<VEC>(to + 4 * (kArray + s * kNext), q, true);
+        }
+      } else {
+#pragma unroll 4
+        for (int s = 0; s < kSteps; ++s, p += a.channels, q += a.channels) {
+          const bool live = column < m.channels && before_me + s < m.live;
+          copy_async<VEC>(to + 4 * s * kNext, live ? p : a.gate, live);
+          copy_async<VEC>(to + 4 * (kArray + s * kNext), live ? q : a.x, live);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // The parts of chunk i; the effect of the groups before this one into (eA, eB).
+  auto make = [&](unsigned i, float (&eA)[VEC], float (&eB)[VEC]) {
+    float* const place = places + (i % kRing) * F::kPlace;
+    const int live = line[i & 7].live - before_me;
+    float A[VEC], B[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[j] = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < kSteps; ++s) {
+      float g[VEC], v[VEC];
+      load_place<VEC>(g, place + s * kNext);
+      load_place<VEC>(v, place + kArray + s * kNext);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if (SIGMOID) {
+          float rest;
+          sigmoid_pair(g[j], g[j], rest);
+          v[j] *= rest;
+        }
+        if (s >= live) g[j] = 1.0f;  // and v is 0
+        A[j] *= g[j];
+        B[j] = fmaf(g[j], B[j], v[j]);
+      }
+      if (SIGMOID) {
+        store_place<VEC>(place + s * kNext, g);
+        store_place<VEC>(place + kArray + s * kNext, v);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+#pragma unroll
+      for (int off = 1; off < VEC; off *= 2) {
+        const float pa = __shfl_up_sync(0xffffffffu, A[j], off * kRow), pb = __shfl_up_sync(0xffffffffu, B[j], off * kRow);
+        if (group >= off) {
+          B[j] = fmaf(A[j], pb, B[j]);
+          A[j] *= pa;
+        }
+      }
+      eA[j] = eB[j] = 0.0f;
+      if (VEC > 1) {
+        eA[j] = __shfl_up_sync(0xffffffffu, A[j], kRow);
+        eB[j] = __shfl_up_sync(0xffffffffu, B[j], kRow);
+      }
+      if (group == VEC - 1) parts[i & 1][warp][0][column + j] = A[j], parts[i & 1][warp][1][column + j] = B[j];
+    }
+    signal(kPartsMade + (i & 1), kAll);
+  };
+
+#pragma unroll
+  for (int k = 0; k < kRing; ++k) {
+    __syncthreads();
+    fetch(k);
+  }
+  float eA[VEC], eB[VEC], nA[VEC], nB[VEC];
+  if (line[0].channels) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+    make(0, eA, eB);
+  }
+  for (unsigned i = 0; line[i & 7].channels; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    if (line[(i + 1) & 7].channels) make(i + 1, nA, nB);
+    const Tile& m = line[i & 7];
+    meet(kEntryKnown + (i & 1), kAll);
+    float h[VEC];
+    load_place<VEC>(h, &entries[i & 1][warp][column]);
+    if (group > 0) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) h[j] = advance(h[j], eA[j], eB[j]);
+    }
+    const float* const place = places + (i % kRing) * F::kPlace;
+    const bool inside = column < m.channels;
+    auto write = [&](bool whole) {
+      float* p = a.h + m.at + mine;
+#pragma unroll 8
+      for (int s = 0; s < kSteps; ++s, p += a.channels) {
+        float g[VEC], v[VEC];
+        load_place<VEC>(g, place + s * kNext);
+        load_place<VEC>(v, place + kArray + s * kNext);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if (!SIGMOID && !whole && before_me + s >= m.live) g[j] = 1.0f;
+          h[j] = fmaf(g[j], h[j], v[j]);
+        }
+        if (whole || (inside && before_me + s < m.steps)) store<VEC>(p, h);
+      }
+    };
+    if (inside && before_me + kSteps <= m.live) {
+      write(true);
+    } else if (!(m.ends && before_me >= m.live)) {
+      write(false);
+    }
+    if (m.ends) {
+      // what is held after the end is the state itself, not one advanced by (A, B): this
+      // chunk publishes that state alone
+      if (m.live > before_me && m.live <= before_me + kSteps) {  // the group that has the last step
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          ended[column + j] = h[j];
+          if (!WHOLE && !m.last) put(sc.records + static_cast<int64_t>(m.row) * kWide + column + j, 1.0f, 0.0f, h[j], 2u);
+        }
+      }
+      meet(kEndKnown, kWarps * 32);
+      if (WHOLE && !m.last) signal(kEndTold, kAll);
+      if (before_me >= m.live) {
+        load_place<VEC>(h, ended + column);
+        write(false);
+      }
+    }
+    if (a.state && inside && before_me < m.steps && m.last && before_me + kSteps >= m.steps)
+      store<VEC>(a.state + m.edge + column, h);
+    fetch(i + kRing);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) eA[j] = nA[j], eB[j] = nB[j];
+  }
+}
+
 // ------------------------------------------------------------------------- launches
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
@@ -542,6 +838,31 @@ int width_of(const Args& a) {
   return 1;
 }
 
+// Whole chains to a block, where the last of their rounds leaves few blocks idle.
+bool walks(int64_t chains, int64_t blocks) { return chains * 10 >= ceil_div(chains, blocks) * blocks * 8; }
+
+// `whole`: a block takes whole chains, and there are no records.
+template <typename Sh>
+int launch_scan(cudaStream_t s, const Args& a, void (*kernel)(Args, Scan, int*), bool whole, void* workspace) {
+  const int64_t blocks = ceil_div(a.channels, kWide), chunks = ceil_div(a.time, Sh::kChunk);
+  const int64_t tiles = a.batch * blocks * chunks;
+  if (tiles > INT32_MAX) return invalid("recurrence is too large for one call");
+  Scan sc;
+  sc.blocks = static_cast<unsigned>(blocks);
+  sc.chains = static_cast<unsigned>(a.batch * blocks);
+  sc.chunks = static_cast<unsigned>(chunks);
+  sc.tiles = static_cast<unsigned>(tiles);
+  sc.records = whole ? nullptr : static_cast<Record*>(workspace);
+  sc.ticket = whole ? nullptr : reinterpret_cast<unsigned*>(sc.records + tiles * kWide);
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kBytes) != cudaSuccess)
+    return launch_status("recurrence shared memory attribute");
+  if (!whole) cudaMemsetAsync(workspace, 0, tiles * kWide * sizeof(Record) + sizeof(unsigned), s);
+  const int64_t grid = std::min<int64_t>(whole ? sc.chains : tiles, Sh::kPerSm * sm_count());
+  TimedLaunch timer("recurrence_scan", s);
+  kernel<<<static_cast<unsigned>(grid), Sh::kThreads, Sh::kBytes, s>>>(a, sc, device_error_word());
+  return launch_status("recurrence");
+}
+
 template <int VEC, bool SIGMOID, bool BACK>
 int launch(cudaStream_t s, const Args& a, void* workspace) {
   if (a.time <= kWalkSteps) {
@@ -551,31 +872,14 @@ int launch(cudaStream_t s, const Args& a, void* workspace) {
     else walk_forward_kernel<VEC, SIGMOID><<<grid, 256, 0, s>>>(a);
     return launch_status("recurrence");
   }
-  using Sh = Shape<VEC, SIGMOID, BACK>;
-  const int64_t blocks = ceil_div(a.channels, kWide), chunks = ceil_div(a.time, Sh::kChunk);
-  const int64_t tiles = a.batch * blocks * chunks;
-  if (tiles > INT32_MAX) return invalid("recurrence is too large for one call");
-  Scan sc;
-  sc.blocks = static_cast<unsigned>(blocks);
-  sc.chains = static_cast<unsigned>(a.batch * blocks);
-  sc.chunks = static_cast<unsigned>(chunks);
-  sc.tiles = static_cast<unsigned>(tiles);
-  sc.records = static_cast<Record*>(workspace);
-  sc.ticket = reinterpret_cast<unsigned*>(sc.records + tiles * kWide);
-  static bool attr_done[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-    if (cudaFuncSetAttribute(scan_kernel<VEC, SIGMOID, BACK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             Sh::kBytes) != cudaSuccess)
-      return launch_status("recurrence shared memory attribute");
-    attr_done[dev] = true;
+  const int64_t chains = a.batch * ceil_div(a.channels, kWide);
+  if constexpr (BACK) {
+    return launch_scan<Shape<VEC, SIGMOID, true>>(s, a, scan_kernel<VEC, SIGMOID, true>, false, workspace);
+  } else {
+    if (walks(chains, Forward<VEC>::kPerSm * sm_count()))
+      return launch_scan<Forward<VEC>>(s, a, scan_forward_kernel<VEC, SIGMOID, true>, true, workspace);
+    return launch_scan<Forward<VEC>>(s, a, scan_forward_kernel<VEC, SIGMOID, false>, false, workspace);
   }
-  cudaMemsetAsync(workspace, 0, tiles * kWide * sizeof(Record) + sizeof(unsigned), s);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, Sh::kPerSm * sm_count()));
-  TimedLaunch timer(BACK ? "recurrence_scan_backward" : "recurrence_scan", s);
-  scan_kernel<VEC, SIGMOID, BACK><<<grid, Sh::kWarps * 32, Sh::kBytes, s>>>(a, sc, device_error_word());
-  return launch_status("recurrence");
 }
 
 template <bool SIGMOID, bool BACK>
