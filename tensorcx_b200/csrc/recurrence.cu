@@ -17,7 +17,6 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -48,14 +47,12 @@ __device__ __forceinline__ int64_t length_of(const Args& a, int64_t b) {
   return n < 0 ? 0 : n > a.time ? a.time : n;
 }
 
+// VEC = 4 channels or 1 of global memory that is read or written once, and of shared memory.
 template <int VEC>
 __device__ __forceinline__ void load(float (&v)[VEC], const float* p) {
   if constexpr (VEC == 4) {
     const float4 t = __ldcs(reinterpret_cast<const float4*>(p));
     v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-  } else if constexpr (VEC == 2) {
-    const float2 t = __ldcs(reinterpret_cast<const float2*>(p));
-    v[0] = t.x, v[1] = t.y;
   } else {
     v[0] = __ldcs(p);
   }
@@ -64,10 +61,26 @@ __device__ __forceinline__ void load(float (&v)[VEC], const float* p) {
 template <int VEC>
 __device__ __forceinline__ void store(float* p, const float (&v)[VEC]) {
   if constexpr (VEC == 4) __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
-  else if constexpr (VEC == 2) __stcs(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
   else __stcs(p, v[0]);
 }
 
+template <int VEC>
+__device__ __forceinline__ void load_shared(float (&v)[VEC], const float* p) {
+  if constexpr (VEC == 4) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+  } else {
+    v[0] = *p;
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_shared(float* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else *p = v[0];
+}
+
+// The state that a sequence starts from (or the gradient that reaches its last one).
 template <int VEC>
 __device__ __forceinline__ void start_of(float (&v)[VEC], const float* p, int64_t at) {
 #pragma unroll
@@ -78,16 +91,10 @@ __device__ __forceinline__ void start_of(float (&v)[VEC], const float* p, int64_
 // From a zero state it is B alone: a product that overflowed says nothing about it.
 __device__ __forceinline__ float advance(float h, float A, float B) { return h == 0.0f ? B : fmaf(A, h, B); }
 
-// What the second half of a backward step needs from memory.
-template <int VEC, bool SIGMOID>
-struct Reads {
-  float before[VEC], x[SIGMOID ? VEC : 1];
-};
-
 template <int VEC, bool SIGMOID>
 __device__ __forceinline__ void backward_step(const float (&gate)[VEC], const float (&dh)[VEC],
-                                              const Reads<VEC, SIGMOID>& r, bool live, float (&c)[VEC],
-                                              float (&dgate)[VEC], float (&dx)[VEC]) {
+                                              const float (&before)[VEC], const float (&x)[VEC], bool live,
+                                              float (&c)[VEC], float (&dgate)[VEC], float (&dx)[VEC]) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     const float g = dh[i] + c[i];
@@ -95,14 +102,16 @@ __device__ __forceinline__ void backward_step(const float (&gate)[VEC], const fl
     if (SIGMOID) sigmoid_pair(s, s, rest);
     const float d = SIGMOID ? g * rest : g;
     dx[i] = live ? d : 0.0f;
-    dgate[i] = live ? (SIGMOID ? d * s * (r.before[i] - r.x[SIGMOID ? i : 0]) : d * r.before[i]) : 0.0f;
+    dgate[i] = live ? (SIGMOID ? d * s * (before[i] - x[i]) : d * before[i]) : 0.0f;
     c[i] = live ? s * g : g;
   }
 }
 
 // ------------------------------------------------------- one thread per VEC channels
-// Walks through time by itself. For short sequences: a token of each running sequence is
-// one step of this kernel.
+// Walks through time by itself, the loads of kAhead steps at a time. For short sequences (a
+// token of each running sequence is one step of this kernel) and for batches wide enough.
+constexpr int kAhead = 4;
+
 template <int VEC, bool SIGMOID>
 __global__ void __launch_bounds__(256) walk_forward_kernel(Args a) {
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * VEC;
@@ -111,22 +120,31 @@ __global__ void __launch_bounds__(256) walk_forward_kernel(Args a) {
   float h[VEC];
   start_of<VEC>(h, a.initial, i);
   int64_t at = b * (a.time - 1) * a.channels + i;
-  for (int64_t t = 0; t < a.time; ++t, at += a.channels) {
-    if (t < n) {
-      float g[VEC], x[VEC];
-      load<VEC>(g, a.gate + at);
-      load<VEC>(x, a.x + at);
+  for (int64_t t0 = 0; t0 < a.time; t0 += kAhead) {
+    float g[kAhead][VEC], x[kAhead][VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        if (SIGMOID) {
-          float rest;
-          sigmoid_pair(g[j], g[j], rest);
-          x[j] *= rest;
-        }
-        h[j] = fmaf(g[j], h[j], x[j]);
+    for (int s = 0; s < kAhead; ++s) {
+      if (t0 + s < n) {
+        load<VEC>(g[s], a.gate + at + s * a.channels);
+        load<VEC>(x[s], a.x + at + s * a.channels);
       }
     }
-    store<VEC>(a.h + at, h);
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s, at += a.channels) {
+      if (t0 + s >= a.time) break;
+      if (t0 + s < n) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if (SIGMOID) {
+            float rest;
+            sigmoid_pair(g[s][j], g[s][j], rest);
+            x[s][j] *= rest;
+          }
+          h[j] = fmaf(g[s][j], h[j], x[s][j]);
+        }
+      }
+      store<VEC>(a.h + at, h);
+    }
   }
   if (a.state) store<VEC>(a.state + i, h);
 }
@@ -139,57 +157,52 @@ __global__ void __launch_bounds__(256) walk_backward_kernel(Args a) {
   float c[VEC];
   start_of<VEC>(c, a.dstate, i);
   int64_t at = b * (a.time - 1) * a.channels + i + (a.time - 1) * a.channels;
-  for (int64_t t = a.time - 1; t >= 0; --t, at -= a.channels) {
-    float gate[VEC] = {}, dh[VEC], dgate[VEC], dx[VEC];
-    Reads<VEC, SIGMOID> r = {};
-    load<VEC>(dh, a.dh + at);
-    if (t < n) {
-      load<VEC>(gate, a.gate + at);
-      if (t) load<VEC>(r.before, a.hs + at - a.channels);
-      else start_of<VEC>(r.before, a.initial, i);
-      if constexpr (SIGMOID) load<VEC>(r.x, a.x + at);
+  for (int64_t t0 = a.time - 1; t0 >= 0; t0 -= kAhead) {
+    float gate[kAhead][VEC], dh[kAhead][VEC], before[kAhead][VEC], x[kAhead][VEC];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const int64_t t = t0 - s, here = at - s * a.channels;
+      if (t < 0) break;
+      load<VEC>(dh[s], a.dh + here);
+      if (t < n) {
+        load<VEC>(gate[s], a.gate + here);
+        if (t) load<VEC>(before[s], a.hs + here - a.channels);
+        else start_of<VEC>(before[s], a.initial, i);
+        if (SIGMOID) load<VEC>(x[s], a.x + here);
+      }
     }
-    backward_step<VEC, SIGMOID>(gate, dh, r, t < n, c, dgate, dx);
-    store<VEC>(a.dgate + at, dgate);
-    store<VEC>(a.dx + at, dx);
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s, at -= a.channels) {
+      if (t0 - s < 0) break;
+      float dgate[VEC], dx[VEC];
+      backward_step<VEC, SIGMOID>(gate[s], dh[s], before[s], x[s], t0 - s < n, c, dgate, dx);
+      store<VEC>(a.dgate + at, dgate);
+      store<VEC>(a.dx + at, dx);
+    }
   }
   if (a.dinitial) store<VEC>(a.dinitial + i, c);
 }
 
 // --------------------------------------------------------- scan over parts of the time
-// A sequence of one batch entry and 32 channels (a chain) is cut into chunks of time, a block
-// to a chunk at a time. A row of a chunk is 128 bytes: 32 / VEC lanes of a warp read it, so a
-// warp's lanes form VEC groups, and each group of each warp takes kSteps steps of its own.
-// Memory is read once and written once. A part's effect on a state is (A, B): the product of
-// its gates and its last state from zero. The groups' parts meet by shuffles, the warps' in
-// shared memory and the chunks' in the workspace: a block publishes its (A, B), walks back
-// over its chain's published parts to the nearest chunk whose last state is known, advances
-// that state through the parts between, and publishes its own. Blocks stay on their SM and
-// take chunks in order of a ticket, each in the order it got them, so what a block waits for
-// has always begun; the waits are bounded all the same. The next chunk's data come into
-// shared memory (cp.async; a thread copies and reads its own places only, so that needs no
-// barrier) as soon as the values there have been taken into registers or used.
+// A sequence of one batch entry and 32 channels (a chain) is cut into chunks of kChunk steps,
+// which blocks take one at a time. Memory is read once and written once: a chunk's rows of
+// 128 bytes come into shared memory (cp.async) while the block works on earlier chunks. With
+// VEC = 4, 8 lanes hold a row, so that a warp's lanes form 4 groups; with VEC = 1 all 32 do.
+// Each group of each warp takes kSteps steps of its own. A part's effect on a state is (A, B):
+// the product of its gates and its last state from zero. The groups' parts meet by shuffles,
+// the warps' in shared memory and the chunks' in the workspace, as records: a block publishes
+// its chunk's (A, B), walks back over its chain's published parts to the nearest chunk whose
+// last state is known, advances that state through the parts between, and publishes its own.
+// Blocks stay on their SM and take chunks in order of a ticket, each in the order it got
+// them, so what a block waits for has always begun; the waits are bounded all the same.
 //
 // The state that enters a chunk is always the previous chunk's entering state advanced by
 // that chunk's (A, B), whether a published state or the parts themselves bring it: the
 // result does not depend on the order in which blocks run.
 //
 // Backward the same scan runs from the last step to the first, on c_t = a_t (c_(t+1) + dh_t).
-constexpr int kWide = 32;            // channels of a chain
-constexpr int64_t kWalkSteps = 16;   // up to so many steps a thread walks through time alone
-constexpr int kLeastChunk = 64;      // no shape has shorter chunks (the workspace is sized by it)
-
-template <int VEC, bool SIGMOID, bool BACK>
-struct Shape {
-  static constexpr int kWarps = 4, kPerSm = 3, kThreads = kWarps * 32;
-  static constexpr int kSteps = 32 / VEC;      // of one group
-  static constexpr int kRing = BACK ? 1 : 2;   // chunks whose data are on their way
-  static constexpr int kChunk = kWarps * VEC * kSteps;
-  static constexpr int kArrays = BACK ? (SIGMOID ? 4 : 3) : 2;  // gate, x | gate, dh, the state before, x
-  static constexpr int kArray = kChunk * kWide, kPlace = kArrays * kArray, kBytes = kRing * kPlace * 4;
-  static_assert(kChunk >= kLeastChunk, "the workspace is sized for chunks of kLeastChunk steps or more");
-  static_assert(kBytes * kPerSm <= 216 * 1024, "the blocks of an SM share its memory");
-};
+constexpr int kWide = 32;   // channels of a chain
+constexpr int kChunk = 128;
 
 // What a chunk tells the later ones about one channel, written and read in one 128-bit access.
 struct __align__(16) Record {
@@ -268,333 +281,192 @@ __device__ float enter(const Record* mine, int chunk, float start, int lane, int
   }
 }
 
-// Copies VEC floats to shared memory, or zeros.
-template <int VEC>
-__device__ __forceinline__ void copy_async(uint32_t to, const float* from, bool there) {
-  const int bytes = there ? 4 * VEC : 0;
-  if constexpr (VEC == 4)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-  else if constexpr (VEC == 2)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-
-template <int VEC>
-__device__ __forceinline__ void load_place(float (&v)[VEC], const float* p) {
-  if constexpr (VEC == 4) {
-    const float4 t = *reinterpret_cast<const float4*>(p);
-    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-  } else if constexpr (VEC == 2) {
-    const float2 t = *reinterpret_cast<const float2*>(p);
-    v[0] = t.x, v[1] = t.y;
-  } else {
-    v[0] = *p;
-  }
-}
-
-template <int VEC>
-__device__ __forceinline__ void store_place(float* p, const float (&v)[VEC]) {
-  if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  else if constexpr (VEC == 2) *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
-  else *p = v[0];
-}
-
-// A thread's share of a chunk: kSteps steps of VEC channels.
-struct Share {
-  unsigned tile, chain, chunk;
-  int64_t b, c;      // batch entry, first channel
-  int64_t n, first;  // the sequence's length, the first step in the scan's own order
-  int64_t at;        // of the first step in the arrays
-  bool inside, full;  // the channels exist; so do all the steps
-};
-
-template <int VEC, bool SIGMOID, bool BACK>
-__device__ __forceinline__ Share share_of(const Args& a, const Scan& sc, unsigned tile, int column, int before_me) {
-  using Sh = Shape<VEC, SIGMOID, BACK>;
-  Share m;
-  m.tile = tile;
-  m.chunk = tile / sc.chains;
-  m.chain = tile - m.chunk * sc.chains;
-  const unsigned b = m.chain / sc.blocks;
-  m.b = b;
-  m.c = static_cast<int64_t>(m.chain - b * sc.blocks) * kWide + column;
-  m.n = length_of(a, m.b);
-  m.first = static_cast<int64_t>(m.chunk) * Sh::kChunk + before_me;
-  const int64_t t = BACK ? a.time - 1 - m.first : m.first;
-  m.at = (m.b * a.time + t) * a.channels + m.c;
-  m.inside = m.c < a.channels;
-  m.full = m.inside && m.first + Sh::kSteps <= a.time && (BACK ? t < m.n : t + Sh::kSteps <= m.n);
-  return m;
-}
-
-template <int VEC, bool SIGMOID, bool BACK>
-__global__ void __launch_bounds__(Shape<VEC, SIGMOID, BACK>::kWarps * 32, Shape<VEC, SIGMOID, BACK>::kPerSm)
-scan_kernel(Args a, Scan sc, int* err) {
-  using Sh = Shape<VEC, SIGMOID, BACK>;
-  constexpr int kWarps = Sh::kWarps, kSteps = Sh::kSteps, kChunk = Sh::kChunk, kArray = Sh::kArray, kRing = Sh::kRing;
-  constexpr int kRow = 32 / VEC;       // lanes of a row
-  constexpr int kNext = 32 * VEC;      // from one step's place in shared memory to the next one's
-  extern __shared__ __align__(16) float stage[];
-  __shared__ float parts[kWarps][2][kWide];
-  __shared__ __align__(16) float entries[kWarps][kWide], ended[kWide];
-  __shared__ unsigned queue[2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = lane / kRow;
-  const int column = (lane % kRow) * VEC;              // within the chain
-  const int before_me = (warp * VEC + group) * kSteps;  // steps of the chunk
-  float* const place = stage + (warp * kSteps * 32 + lane) * VEC;
-  const uint32_t place_at = ptx::smem_u32(place);
-  const int64_t stride = BACK ? -a.channels : a.channels;
-
-  // Step s of the share exists; the sequence has it.
-  auto exists = [&](const Share& m, int s) { return m.full || (m.inside && m.first + s < a.time); };
-  auto lives = [&](const Share& m, int s) {
-    return m.full || (m.first + s < a.time && (BACK ? a.time - 1 - (m.first + s) : m.first + s) < m.n);
-  };
-  // What the parts are made from: gate and x, or gate and dh.
-  auto fetch = [&](const Share& m, unsigned turn) {
-    if (m.tile < sc.tiles) {
-      const uint32_t to = place_at + (turn % kRing) * (Sh::kPlace * 4);
-      const float *p = a.gate + m.at, *q = (BACK ? a.dh : a.x) + m.at;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
-        const bool live = m.inside && lives(m, s);
-        copy_async<VEC>(to + 4 * s * kNext, live ? p : a.gate, live);
-        const bool has = BACK ? exists(m, s) : live;
-        copy_async<VEC>(to + 4 * (kArray + s * kNext), has ? q : a.gate, has);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  // What a backward chunk needs besides once its entering state is known.
-  auto fetch_rest = [&](const Share& m) {
-    if (m.tile < sc.tiles) {
-      const float *p = a.hs + m.at - a.channels, *q = SIGMOID ? a.x + m.at : nullptr;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
-        const bool live = m.inside && lives(m, s), opening = m.first + s == a.time - 1;  // t = 0
-        const bool has = live && (!opening || a.initial);
-        copy_async<VEC>(place_at + 4 * (2 * kArray + s * kNext),
-                        !has ? a.gate : opening ? a.initial + m.b * a.channels + m.c : p, has);
-        if constexpr (SIGMOID) copy_async<VEC>(place_at + 4 * (3 * kArray + s * kNext), live ? q : a.gate, live);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-
-  Share line[kRing];  // this chunk and those whose data are on their way
-#pragma unroll
-  for (int k = 0; k < kRing; ++k) {
-    if (threadIdx.x == 0) queue[k & 1] = atomicAdd(sc.ticket, 1u);
-    __syncthreads();
-    line[k] = share_of<VEC, SIGMOID, BACK>(a, sc, queue[k & 1], column, before_me);
-    fetch(line[k], k);
-  }
-  if (BACK) fetch_rest(line[0]);
-  unsigned later = threadIdx.x == 0 ? atomicAdd(sc.ticket, 1u) : 0;
-  __syncthreads();
-  for (unsigned turn = 0; line[0].tile < sc.tiles; ++turn) {  // tickets past the end stay past it
-    const Share m = line[0];
-    const float* const here = place + (turn % kRing) * Sh::kPlace;
-    asm volatile("cp.async.wait_group %0;" ::"n"(BACK ? 1 : kRing - 1) : "memory");
-    float g[kSteps][VEC], v[kSteps][VEC];  // gate and x, or gate and dh
-    float A[VEC], B[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) A[i] = 1.0f, B[i] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      load_place<VEC>(g[s], here + s * kNext);
-      load_place<VEC>(v[s], here + kArray + s * kNext);
-      const bool live = lives(m, s);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (BACK) {
-          float s1 = g[s][i], rest;
-          if (SIGMOID) sigmoid_pair(s1, s1, rest);
-          if (!live) s1 = 1.0f;
-          A[i] *= s1;
-          B[i] = s1 * (B[i] + v[s][i]);
-        } else {
-          if (SIGMOID) {
-            float rest;
-            sigmoid_pair(g[s][i], g[s][i], rest);
-            v[s][i] *= rest;
-          }
-          if (!live) g[s][i] = 1.0f;  // and v is 0
-          A[i] *= g[s][i];
-          B[i] = fmaf(g[s][i], B[i], v[s][i]);
-        }
-      }
-    }
-    // the groups before this one, then with it; the last group has the warp's part
-    float eA[VEC], eB[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-      for (int off = 1; off < VEC; off *= 2) {
-        const float pa = __shfl_up_sync(0xffffffffu, A[i], off * kRow), pb = __shfl_up_sync(0xffffffffu, B[i], off * kRow);
-        if (group >= off) {
-          B[i] = fmaf(A[i], pb, B[i]);
-          A[i] *= pa;
-        }
-      }
-      eA[i] = eB[i] = 0.0f;
-      if (VEC > 1) {
-        eA[i] = __shfl_up_sync(0xffffffffu, A[i], kRow);
-        eB[i] = __shfl_up_sync(0xffffffffu, B[i], kRow);
-      }
-      if (group == VEC - 1) parts[warp][0][column + i] = A[i], parts[warp][1][column + i] = B[i];
-    }
-    if (threadIdx.x == 0) queue[0] = later;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k + 1 < kRing; ++k) line[k] = line[k + 1];
-    line[kRing - 1] = share_of<VEC, SIGMOID, BACK>(a, sc, queue[0], column, before_me);
-
-    // A forward chunk in which the sequence ends: what is held after it is the state itself,
-    // not one advanced by (A, B), so this chunk publishes that state alone.
-    const int64_t opens = m.first - before_me;
-    const bool ends = !BACK && m.n < a.time && m.n > opens && m.n <= opens + kChunk;
-    Record* const record = sc.records + (static_cast<int64_t>(m.chain) * sc.chunks + m.chunk) * kWide;
-    if (warp == 0) {  // a lane to a channel
-      float wA = 1.0f, wB = 0.0f, state = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        wB = fmaf(parts[w][0][lane], wB, parts[w][1][lane]);
-        wA *= parts[w][0][lane];
-      }
-      const int64_t channel = m.c - column + lane;
-      const float* start = BACK ? a.dstate : a.initial;
-      if (start && channel < a.channels) state = __ldg(start + m.b * a.channels + channel);
-      const bool goes_on = m.chunk + 1 < sc.chunks && !ends;
-      if (m.chunk > 0) {
-        if (goes_on) put(record + lane, wA, wB, 0.0f, 1u);
-        state = enter(record + lane, static_cast<int>(m.chunk), state, lane, err);
-      }
-      if (goes_on) put(record + lane, wA, wB, advance(state, wA, wB), 2u);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        entries[w][lane] = state;
-        state = advance(state, parts[w][0][lane], parts[w][1][lane]);
-      }
-    }
-    fetch(line[kRing - 1], turn);
-    if (threadIdx.x == 0) later = atomicAdd(sc.ticket, 1u);
-    __syncthreads();
-    float h[VEC];
-    load_place<VEC>(h, &entries[warp][column]);
-    if (group > 0) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[i] = advance(h[i], eA[i], eB[i]);
-    }
-
-    if constexpr (BACK) {
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      float *p = a.dgate + m.at, *q = a.dx + m.at;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
-        Reads<VEC, SIGMOID> r;
-        load_place<VEC>(r.before, place + 2 * kArray + s * kNext);
-        if constexpr (SIGMOID) load_place<VEC>(r.x, place + 3 * kArray + s * kNext);
-        if (!exists(m, s)) continue;
-        float dgate[VEC], dx[VEC];
-        backward_step<VEC, SIGMOID>(g[s], v[s], r, lives(m, s), h, dgate, dx);
-        store<VEC>(p, dgate);
-        store<VEC>(q, dx);
-      }
-      fetch_rest(line[0]);
-    } else {
-      auto write = [&]() {
-        float* p = a.h + m.at;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s, p += stride) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) h[i] = fmaf(g[s][i], h[i], v[s][i]);
-          if (exists(m, s)) store<VEC>(p, h);
-        }
-      };
-      const bool held = ends && m.first >= m.n;  // this group's steps come after the end
-      if (!held) write();
-      if (ends) {
-        if (m.n > m.first && m.n <= m.first + kSteps) {  // the group that has the last step
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            ended[column + i] = h[i];
-            if (m.chunk + 1 < sc.chunks) put(record + column + i, 1.0f, 0.0f, h[i], 2u);
-          }
-        }
-        __syncthreads();
-        if (held) {
-          load_place<VEC>(h, ended + column);
-          write();
-        }
-      }
-    }
-    float* last = BACK ? a.dinitial : a.state;
-    if (last && m.inside && m.first < a.time && m.first + kSteps >= a.time)
-      store<VEC>(last + m.b * a.channels + m.c, h);
-  }
-}
-
-// ---------------------------------------------------------------- the forward scan
-// The same scan with the walk back taken out of the blocks' way: kWarps warps make the parts
-// of chunk i + 1 and then write the states of chunk i, while two more warps publish the parts
-// (the teller) and bring the state that enters chunk i + 1 (the carrier). The values wait in
-// shared memory between the two uses, in the places that the next chunks' data come into.
-template <int VEC>
-struct Forward {
-  static constexpr int kWarps = 4, kRing = 3, kPerSm = 2;
-  static constexpr int kSteps = 32 / VEC;  // of one group
-  static constexpr int kChunk = kWarps * VEC * kSteps;
-  static constexpr int kArray = kChunk * kWide, kPlace = 2 * kArray, kBytes = kRing * kPlace * 4;  // gate, x
-  static constexpr int kThreads = (kWarps + 2) * 32;
-  static_assert(kChunk >= kLeastChunk, "the workspace is sized for chunks of kLeastChunk steps or more");
-  static_assert(kBytes * kPerSm <= 216 * 1024, "the blocks of an SM share its memory");
-};
-
-// A chunk as its block sees it.
+// A chunk as its block sees it; steps are numbered in the scan's own order.
 struct Tile {
-  int64_t at;            // of its first step and channel in the arrays
-  int64_t edge;          // of its first channel in the states
-  int channels, steps;   // that exist, of kWide and kChunk; no channels: there is no such chunk
-  int live;              // steps that the sequence has
-  unsigned row, chunk;   // its records; its place in the chain
-  int ends, last;        // the sequence ends in it, before time does; no chunk comes after it
+  int64_t at;           // of its first step and channel in the arrays
+  int64_t edge;         // of its first channel in the states
+  int channels, steps;  // that exist, of kWide and kChunk; no channels: there is no such chunk
+  int from, to;         // steps that the sequence has
+  unsigned row, chunk;  // its records; its place in the chain
+  int ends, last;       // the sequence ends in it, before time does; no chunk comes after it
 };
 
-// The block's chunk number i. With records: the one that a ticket names. Without: whole chains,
-// chunk after chunk.
-template <int VEC, bool WHOLE>
-__device__ Tile next_tile(const Args& a, const Scan& sc, unsigned i) {
-  using F = Forward<VEC>;
+// The chunk that a ticket names; WHOLE: the block's chunk number i, where it takes whole
+// chains, chunk after chunk.
+template <bool BACK, bool WHOLE>
+__device__ Tile tile_of(const Args& a, const Scan& sc, unsigned i) {
   Tile m = {};
   unsigned chain;
-  if (!WHOLE) {
-    const unsigned tile = atomicAdd(sc.ticket, 1u);
-    if (tile >= sc.tiles) return m;
-    m.chunk = tile / sc.chains;
-    chain = tile - m.chunk * sc.chains;
-  } else {
+  if (WHOLE) {
     const unsigned turn = i / sc.chunks;
     m.chunk = i - turn * sc.chunks;
     chain = blockIdx.x + turn * gridDim.x;
     if (chain >= sc.chains) return m;
+  } else {
+    if (i >= sc.tiles) return m;
+    m.chunk = i / sc.chains;
+    chain = i - m.chunk * sc.chains;
   }
   const unsigned b = chain / sc.blocks, block = chain - b * sc.blocks;
-  const int64_t n = length_of(a, b), opens = static_cast<int64_t>(m.chunk) * F::kChunk;
+  const int64_t n = length_of(a, b), opens = static_cast<int64_t>(m.chunk) * kChunk;
   const int64_t c = static_cast<int64_t>(block) * kWide;
-  m.at = (b * a.time + opens) * a.channels + c;
+  auto local = [&](int64_t v) {
+    return static_cast<int>(max(min(v - opens, static_cast<int64_t>(kChunk)), static_cast<int64_t>(0)));
+  };
+  m.at = (b * a.time + (BACK ? a.time - 1 - opens : opens)) * a.channels + c;
   m.edge = b * a.channels + c;
   m.channels = static_cast<int>(min(a.channels - c, static_cast<int64_t>(kWide)));
-  m.steps = static_cast<int>(min(a.time - opens, static_cast<int64_t>(F::kChunk)));
-  m.live = static_cast<int>(max(min(n - opens, static_cast<int64_t>(F::kChunk)), static_cast<int64_t>(0)));
+  m.steps = local(a.time);
+  m.from = BACK ? local(a.time - n) : 0;
+  m.to = BACK ? m.steps : local(n);
   m.row = chain * sc.chunks + m.chunk;
-  m.ends = n < a.time && n > opens && n <= opens + F::kChunk;
+  m.ends = !BACK && n < a.time && n > opens && n <= opens + kChunk;
   m.last = m.chunk + 1 == sc.chunks;
   return m;
 }
 
-// Barriers between the warps that work and the carrier, two of each by the chunk's parity.
+// A thread's rows of an array of a chunk in shared memory. VEC = 4: each thread copies and
+// reads places of its own (16 bytes of a row). VEC = 1: rows start at any element, so a warp
+// copies the 16-byte words that hold its rows, 9 to a row, and a lane reads its channel at the
+// row's own distance from the word's start; rows that begin before the array itself does are
+// copied element by element.
+template <int VEC>
+struct Rows {
+  static constexpr int kWarps = VEC == 4 ? 4 : 8;           // that work on a chunk
+  static constexpr int kSteps = kChunk / (kWarps * VEC);    // of one group
+  static constexpr int kGroup = 32 / VEC;                   // lanes of a group
+  static constexpr int kNext = VEC == 4 ? 128 : 36;         // floats from one step's place to the next one's
+  static constexpr int kArray = kWarps * kSteps * kNext;    // floats of an array
+  static_assert(kWarps * VEC * kSteps == kChunk, "");
+  int lane, warp, column, mine;  // its first channel within the chain, its first step of the chunk
+  float* place;                  // its first place in the first array
+
+  __device__ explicit Rows(float* stage) {
+    lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    column = (lane % kGroup) * VEC;
+    mine = (warp * VEC + lane / kGroup) * kSteps;
+    place = stage + warp * kSteps * kNext + (VEC == 4 ? lane * VEC : 0);
+  }
+  __device__ int group() const { return lane / kGroup; }
+
+  // Copies steps [from, to) of `channels` channels; `row` points at the chunk's first channel
+  // and step, `all` at the array of `count` elements, and a step is `stride` elements.
+  __device__ __forceinline__ void copy(int array, const float* all, int64_t count, const float* row, int64_t stride,
+                                       int channels, int from, int to) const {
+    const uint32_t dst = ptx::smem_u32(place + array * kArray);
+    if constexpr (VEC == 4) {
+      const float* p = row + mine * stride + column;
+      if (column < channels && mine >= from && mine + kSteps <= to) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s, p += stride)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * s * kNext), "l"(p) : "memory");
+      } else {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s, p += stride) {
+          const bool in = column < channels && mine + s >= from && mine + s < to;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 4 * s * kNext), "l"(in ? p : all),
+                       "r"(in ? 16 : 0)
+                       : "memory");
+        }
+      }
+    } else {
+      const float* const end = all + count;
+      const float* const word = reinterpret_cast<const float*>(reinterpret_cast<uintptr_t>(all) & ~uintptr_t(15));
+      if (lane >= 27) return;  // 9 lanes to a row, 3 rows at a time
+      int r = lane / 9;
+      const int q4 = 4 * (lane - 9 * r);
+      const float* start = row + (mine + r) * stride;
+      uint32_t to_at = dst + 4 * (r * kNext + q4);
+#pragma unroll
+      for (int k = 0; k < kSteps; k += 3, r += 3, start += 3 * stride, to_at += 12 * kNext) {
+        if (r >= kSteps) break;
+        const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(start) >> 2) & 3;
+        const bool in = mine + r >= from && mine + r < to && q4 - shift < channels;
+        const float* const p = start + (q4 - shift);
+        if (in && p < all) {
+          for (int j = 0; j < 4; ++j)
+            if (p + j >= all && p + j < end)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to_at + 4 * j), "l"(p + j) : "memory");
+        } else {
+          const int bytes = in ? static_cast<int>(min(end - p, static_cast<int64_t>(4))) * 4 : 0;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to_at), "l"(in ? p : word), "r"(bytes)
+                       : "memory");
+        }
+      }
+    }
+  }
+  // Where this thread's step 0 lies; a step on, at(s) of a later one.
+  __device__ __forceinline__ int shift(const float* row, int64_t stride) const {
+    if (VEC == 4) return 0;
+    return static_cast<int>(reinterpret_cast<uintptr_t>(row + mine * stride) >> 2) & 3;
+  }
+  __device__ __forceinline__ float* at(int array, int s, int shift, int stride) const {
+    float* const p = place + array * kArray + s * kNext;
+    return VEC == 4 ? p : p + ((shift + s * stride) & 3) + lane;
+  }
+  // The copies of this thread's warp, all but the last N groups, are there.
+  template <int N>
+  __device__ __forceinline__ void arrived() const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    if (VEC == 1) __syncwarp();
+  }
+  // Its places may be copied into again.
+  __device__ __forceinline__ void done() const {
+    if (VEC == 1) __syncwarp();
+  }
+};
+
+// Joins the groups' parts of a warp: (A, B) becomes the effect of the groups up to this one,
+// (eA, eB) that of the groups before it; the last group writes the warp's to `part`.
+template <int VEC>
+__device__ __forceinline__ void join_groups(float (&A)[VEC], float (&B)[VEC], float (&eA)[VEC], float (&eB)[VEC],
+                                            int group, int column, float (*part)[kWide]) {
+  constexpr int kGroup = 32 / VEC;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+    for (int off = 1; off < VEC; off *= 2) {
+      const float pa = __shfl_up_sync(0xffffffffu, A[i], off * kGroup);
+      const float pb = __shfl_up_sync(0xffffffffu, B[i], off * kGroup);
+      if (group >= off) {
+        B[i] = fmaf(A[i], pb, B[i]);
+        A[i] *= pa;
+      }
+    }
+    eA[i] = eB[i] = 0.0f;
+    if (VEC > 1) {
+      eA[i] = __shfl_up_sync(0xffffffffu, A[i], kGroup);
+      eB[i] = __shfl_up_sync(0xffffffffu, B[i], kGroup);
+    }
+    if (group == VEC - 1) part[0][column + i] = A[i], part[1][column + i] = B[i];
+  }
+}
+
+// The state that enters this thread's steps, from the one that enters its warp's.
+template <int VEC>
+__device__ __forceinline__ void enter_group(float (&h)[VEC], const float* entry, const float (&eA)[VEC],
+                                            const float (&eB)[VEC], int group, int column) {
+  load_shared<VEC>(h, entry + column);
+  if (group > 0) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) h[i] = advance(h[i], eA[i], eB[i]);
+  }
+}
+
+// ---------------------------------------------------------------- the forward scan
+// kWarps warps make the parts of chunk i + 1 and then write the states of chunk i, while two
+// more warps publish the parts (the teller) and bring the state that enters a chunk (the
+// carrier): the walk back does not stand between a chunk's loads and its stores. The values
+// wait in shared memory between their two uses. A block that takes whole chains (WHOLE) has
+// the entering state from its own last chunk, and there are no records.
+template <int VEC>
+struct Forward {
+  static constexpr int kRing = 3, kPerSm = 2, kThreads = (Rows<VEC>::kWarps + 2) * 32;
+  static constexpr int kBytes = kRing * 2 * Rows<VEC>::kArray * 4;  // gate, x
+};
+
+// Barriers of the working warps with the teller and with the carrier, and of those two; two
+// of a kind go by the chunk's parity.
 enum { kPartsMade = 1, kEntryKnown = 3, kEndKnown = 5, kEndTold = 6, kPartsTold = 7 };
 __device__ __forceinline__ void meet(int barrier, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
@@ -606,13 +478,13 @@ __device__ __forceinline__ void signal(int barrier, int threads) {
 template <int VEC, bool SIGMOID, bool WHOLE>
 __global__ void __launch_bounds__(Forward<VEC>::kThreads, Forward<VEC>::kPerSm)
 scan_forward_kernel(Args a, Scan sc, int* err) {
-  using F = Forward<VEC>;
-  constexpr int kWarps = F::kWarps, kSteps = F::kSteps, kRing = F::kRing, kArray = F::kArray;
+  using R = Rows<VEC>;
+  constexpr int kRing = Forward<VEC>::kRing, kSteps = R::kSteps, kWarps = R::kWarps;
   constexpr int kAll = (kWarps + 1) * 32;  // the warps that work, and one of the two others
-  constexpr int kRow = 32 / VEC, kNext = 32 * VEC;
   extern __shared__ __align__(16) float stage[];
-  __shared__ float parts[2][kWarps][2][kWide], joined[2][2][kWide];  // the warps' and the chunk's
-  __shared__ __align__(16) float entries[2][kWarps][kWide], ended[kWide];
+  // The warps' parts. The teller puts the whole chunk's in the place of the last warp's, which
+  // nothing else needs; the carrier puts the state that enters a warp's steps in that of A.
+  __shared__ __align__(16) float parts[2][kWarps][2][kWide], ended[kWide];
   // Chunk i's at i % 8. The carrier sets i's in its turn i - kRing, before it signals that
   // turn's entry. The warps that work see that signal before they make chunk i - 1's parts
   // (kRing >= 3), and the teller reads i's after those were made; the slots in use at a time
@@ -627,15 +499,15 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
       const Tile& m = line[i & 7];
       if (m.channels == 0) return;
       meet(kPartsMade + (i & 1), kAll);
-      const float (*part)[2][kWide] = parts[i & 1];
+      float (*const part)[2][kWide] = parts[i & 1];
       float A = 1.0f, B = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         B = fmaf(part[w][0][lane], B, part[w][1][lane]);
         A *= part[w][0][lane];
       }
-      joined[i & 1][0][lane] = A;
-      joined[i & 1][1][lane] = B;
+      part[kWarps - 1][0][lane] = A;
+      part[kWarps - 1][1][lane] = B;
       if (!WHOLE && m.chunk > 0 && !m.last && !m.ends)
         put(sc.records + static_cast<int64_t>(m.row) * kWide + lane, A, B, 0.0f, 1u);
       signal(kPartsTold + (i & 1), 64);
@@ -643,7 +515,7 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
   }
   if (warp == kWarps) {  // the carrier
     for (int k = 0; k < kRing; ++k) {
-      if (lane == 0) line[k] = next_tile<VEC, WHOLE>(a, sc, k);
+      if (lane == 0) line[k] = tile_of<false, WHOLE>(a, sc, WHOLE ? k : atomicAdd(sc.ticket, 1u));
       __syncthreads();
     }
     float state = 0.0f;
@@ -651,11 +523,12 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
     for (unsigned i = 0;; ++i) {
       const Tile m = line[i & 7];
       if (m.channels == 0) return;
-      if (lane == 0) line[(i + kRing) & 7] = next_tile<VEC, WHOLE>(a, sc, i + kRing);
+      if (lane == 0)
+        line[(i + kRing) & 7] = tile_of<false, WHOLE>(a, sc, WHOLE ? i + kRing : atomicAdd(sc.ticket, 1u));
       const float start = a.initial && lane < m.channels ? __ldg(a.initial + m.edge + lane) : 0.0f;
       meet(kPartsTold + (i & 1), 64);
-      const float (*part)[2][kWide] = parts[i & 1];
-      const float A = joined[i & 1][0][lane], B = joined[i & 1][1][lane];
+      float (*const part)[2][kWide] = parts[i & 1];
+      const float A = part[kWarps - 1][0][lane], B = part[kWarps - 1][1][lane];
       if (!WHOLE) {
         Record* const record = sc.records + static_cast<int64_t>(m.row) * kWide + lane;
         state = m.chunk > 0 ? enter(record, static_cast<int>(m.chunk), start, lane, err) : start;
@@ -671,8 +544,9 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
       float h = state;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        entries[i & 1][w][lane] = h;
+        const float before = h;
         h = advance(h, part[w][0][lane], part[w][1][lane]);
+        part[w][0][lane] = before;
       }
       state = advance(state, A, B);
       __syncwarp();
@@ -680,46 +554,35 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
     }
   }
 
-  const int group = lane / kRow, column = (lane % kRow) * VEC;
-  const int before_me = (warp * VEC + group) * kSteps;  // steps of the chunk
-  float* const places = stage + (warp * kSteps * 32 + lane) * VEC;
-  const uint32_t places_at = ptx::smem_u32(places);
-  const int64_t mine = before_me * a.channels + column;
+  const R rows(stage);
+  const int group = rows.group(), column = rows.column, mine = rows.mine;
+  const int64_t count = a.batch * a.time * a.channels;
+  const int turn_by = static_cast<int>(a.channels & 3);
 
   auto fetch = [&](unsigned i) {
     const Tile& m = line[i & 7];
     if (m.channels) {
-      const float *p = a.gate + m.at + mine, *q = a.x + m.at + mine;
-      const uint32_t to = places_at + (i % kRing) * (F::kPlace * 4);
-      if (column < m.channels && before_me + kSteps <= m.live) {
-#pragma unroll 8
-        for (int s = 0; s < kSteps; ++s, p += a.channels, q += a.channels) {
-          copy_async<VEC>(to + 4 * s * kNext, p, true);
-          copy_async<VEC>(to + 4 * (kArray + s * kNext), q, true);
-        }
-      } else {
-#pragma unroll 4
-        for (int s = 0; s < kSteps; ++s, p += a.channels, q += a.channels) {
-          const bool live = column < m.channels && before_me + s < m.live;
-          copy_async<VEC>(to + 4 * s * kNext, live ? p : a.gate, live);
-          copy_async<VEC>(to + 4 * (kArray + s * kNext), live ? q : a.x, live);
-        }
-      }
+      const int first = 2 * (i % kRing);  // array
+      rows.copy(first, a.gate, count, a.gate + m.at, a.channels, m.channels, m.from, m.to);
+      rows.copy(first + 1, a.x, count, a.x + m.at, a.channels, m.channels, m.from, m.to);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // The parts of chunk i; the effect of the groups before this one into (eA, eB).
   auto make = [&](unsigned i, float (&eA)[VEC], float (&eB)[VEC]) {
-    float* const place = places + (i % kRing) * F::kPlace;
-    const int live = line[i & 7].live - before_me;
+    const Tile& m = line[i & 7];
+    const int first = 2 * (i % kRing), live = m.to - mine;
+    const int gs = rows.shift(a.gate + m.at, a.channels), xs = rows.shift(a.x + m.at, a.channels);
     float A[VEC], B[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[j] = 0.0f;
 #pragma unroll 8
     for (int s = 0; s < kSteps; ++s) {
+      float* const gp = rows.at(first, s, gs, turn_by);
+      float* const xp = rows.at(first + 1, s, xs, turn_by);
       float g[VEC], v[VEC];
-      load_place<VEC>(g, place + s * kNext);
-      load_place<VEC>(v, place + kArray + s * kNext);
+      load_shared<VEC>(g, gp);
+      load_shared<VEC>(v, xp);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         if (SIGMOID) {
@@ -732,27 +595,11 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
         B[j] = fmaf(g[j], B[j], v[j]);
       }
       if (SIGMOID) {
-        store_place<VEC>(place + s * kNext, g);
-        store_place<VEC>(place + kArray + s * kNext, v);
+        store_shared<VEC>(gp, g);
+        store_shared<VEC>(xp, v);
       }
     }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-#pragma unroll
-      for (int off = 1; off < VEC; off *= 2) {
-        const float pa = __shfl_up_sync(0xffffffffu, A[j], off * kRow), pb = __shfl_up_sync(0xffffffffu, B[j], off * kRow);
-        if (group >= off) {
-          B[j] = fmaf(A[j], pb, B[j]);
-          A[j] *= pa;
-        }
-      }
-      eA[j] = eB[j] = 0.0f;
-      if (VEC > 1) {
-        eA[j] = __shfl_up_sync(0xffffffffu, A[j], kRow);
-        eB[j] = __shfl_up_sync(0xffffffffu, B[j], kRow);
-      }
-      if (group == VEC - 1) parts[i & 1][warp][0][column + j] = A[j], parts[i & 1][warp][1][column + j] = B[j];
-    }
+    join_groups<VEC>(A, B, eA, eB, group, column, parts[i & 1][warp]);
     signal(kPartsMade + (i & 1), kAll);
   };
 
@@ -763,46 +610,43 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
   }
   float eA[VEC], eB[VEC], nA[VEC], nB[VEC];
   if (line[0].channels) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+    rows.template arrived<kRing - 1>();
     make(0, eA, eB);
   }
   for (unsigned i = 0; line[i & 7].channels; ++i) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+    rows.template arrived<kRing - 2>();
     if (line[(i + 1) & 7].channels) make(i + 1, nA, nB);
     const Tile& m = line[i & 7];
     meet(kEntryKnown + (i & 1), kAll);
     float h[VEC];
-    load_place<VEC>(h, &entries[i & 1][warp][column]);
-    if (group > 0) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) h[j] = advance(h[j], eA[j], eB[j]);
-    }
-    const float* const place = places + (i % kRing) * F::kPlace;
+    enter_group<VEC>(h, parts[i & 1][warp][0], eA, eB, group, column);
+    const int first = 2 * (i % kRing);
+    const int gs = rows.shift(a.gate + m.at, a.channels), xs = rows.shift(a.x + m.at, a.channels);
     const bool inside = column < m.channels;
     auto write = [&](bool whole) {
-      float* p = a.h + m.at + mine;
+      float* p = a.h + m.at + mine * a.channels + column;
 #pragma unroll 8
       for (int s = 0; s < kSteps; ++s, p += a.channels) {
         float g[VEC], v[VEC];
-        load_place<VEC>(g, place + s * kNext);
-        load_place<VEC>(v, place + kArray + s * kNext);
+        load_shared<VEC>(g, rows.at(first, s, gs, turn_by));
+        load_shared<VEC>(v, rows.at(first + 1, s, xs, turn_by));
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          if (!SIGMOID && !whole && before_me + s >= m.live) g[j] = 1.0f;
+          if (!SIGMOID && !whole && mine + s >= m.to) g[j] = 1.0f;
           h[j] = fmaf(g[j], h[j], v[j]);
         }
-        if (whole || (inside && before_me + s < m.steps)) store<VEC>(p, h);
+        if (whole || (inside && mine + s < m.steps)) store<VEC>(p, h);
       }
     };
-    if (inside && before_me + kSteps <= m.live) {
+    if (inside && mine + kSteps <= m.to) {
       write(true);
-    } else if (!(m.ends && before_me >= m.live)) {
+    } else if (!(m.ends && mine >= m.to)) {
       write(false);
     }
     if (m.ends) {
       // what is held after the end is the state itself, not one advanced by (A, B): this
       // chunk publishes that state alone
-      if (m.live > before_me && m.live <= before_me + kSteps) {  // the group that has the last step
+      if (m.to > mine && m.to <= mine + kSteps) {  // the group that has the last step
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           ended[column + j] = h[j];
@@ -811,40 +655,167 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
       }
       meet(kEndKnown, kWarps * 32);
       if (WHOLE && !m.last) signal(kEndTold, kAll);
-      if (before_me >= m.live) {
-        load_place<VEC>(h, ended + column);
+      if (mine >= m.to) {
+        load_shared<VEC>(h, ended + column);
         write(false);
       }
     }
-    if (a.state && inside && before_me < m.steps && m.last && before_me + kSteps >= m.steps)
+    if (a.state && inside && m.last && mine < m.steps && mine + kSteps >= m.steps)
       store<VEC>(a.state + m.edge + column, h);
+    rows.done();
     fetch(i + kRing);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) eA[j] = nA[j], eB[j] = nB[j];
   }
 }
 
-// ------------------------------------------------------------------------- launches
-bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+// --------------------------------------------------------------- the backward scan
+// A chunk is twice the forward one's bytes, so three blocks to an SM hide each other's walk
+// back: gate and dh go into registers for the parts, their places take the next chunk's, and
+// the state before each step and x are read when the entering gradient is known.
+template <int VEC, bool SIGMOID>
+struct Backward {
+  static constexpr int kPerSm = VEC == 4 ? 3 : 2, kThreads = Rows<VEC>::kWarps * 32;
+  static constexpr int kBytes = (SIGMOID ? 4 : 3) * Rows<VEC>::kArray * 4;  // gate, dh, the state before, x
+};
 
-// Channels per thread: as wide as the channel count and every buffer's alignment allow.
-int width_of(const Args& a) {
-  const void* all[] = {a.gate, a.x, a.initial, a.h, a.state, a.dh, a.hs, a.dstate, a.dgate, a.dx, a.dinitial};
-  for (int vec = 4; vec > 1; vec /= 2) {
-    bool fits = a.channels % vec == 0;
-    for (const void* p : all) fits = fits && aligned(p, 4 * vec);
-    if (fits) return vec;
+template <int VEC, bool SIGMOID>
+__global__ void __launch_bounds__(Backward<VEC, SIGMOID>::kThreads, Backward<VEC, SIGMOID>::kPerSm)
+scan_backward_kernel(Args a, Scan sc, int* err) {
+  using R = Rows<VEC>;
+  constexpr int kSteps = R::kSteps, kWarps = R::kWarps;
+  extern __shared__ __align__(16) float stage[];
+  __shared__ float parts[kWarps][2][kWide];
+  __shared__ __align__(16) float entries[kWarps][kWide];
+  __shared__ Tile line[2];  // this chunk and the next one, by the turn's parity
+  const R rows(stage);
+  const int lane = rows.lane, warp = rows.warp, group = rows.group(), column = rows.column, mine = rows.mine;
+  const int64_t count = a.batch * a.time * a.channels, stride = -a.channels;
+  const int turn_by = static_cast<int>(stride & 3);
+
+  auto fetch = [&](const Tile& m) {
+    if (m.channels) {
+      rows.copy(0, a.gate, count, a.gate + m.at, stride, m.channels, m.from, m.to);
+      rows.copy(1, a.dh, count, a.dh + m.at, stride, m.channels, 0, m.steps);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto fetch_rest = [&](const Tile& m) {
+    if (m.channels) {
+      // the first step of all has no state before it in h
+      rows.copy(2, a.hs, count, a.hs + m.at - a.channels, stride, m.channels, m.from, m.last ? m.to - 1 : m.to);
+      if (SIGMOID) rows.copy(3, a.x, count, a.x + m.at, stride, m.channels, m.from, m.to);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  if (threadIdx.x == 0) line[0] = tile_of<true, false>(a, sc, atomicAdd(sc.ticket, 1u));
+  __syncthreads();
+  fetch(line[0]);
+  fetch_rest(line[0]);
+  unsigned later = threadIdx.x == 0 ? atomicAdd(sc.ticket, 1u) : 0;
+  for (unsigned turn = 0; line[turn & 1].channels; ++turn) {
+    const Tile m = line[turn & 1];
+    const Tile& next = line[(turn + 1) & 1];
+    if (threadIdx.x == 0) line[(turn + 1) & 1] = tile_of<true, false>(a, sc, later);
+    const int gs = rows.shift(a.gate + m.at, stride), ds = rows.shift(a.dh + m.at, stride);
+    rows.template arrived<1>();
+    float g[kSteps][VEC], v[kSteps][VEC], A[VEC], B[VEC];  // gate and dh
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) A[i] = 1.0f, B[i] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      load_shared<VEC>(g[s], rows.at(0, s, gs, turn_by));
+      load_shared<VEC>(v[s], rows.at(1, s, ds, turn_by));
+      const bool live = mine + s >= m.from && mine + s < m.to;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        float s1 = g[s][i], rest;
+        if (SIGMOID) sigmoid_pair(s1, s1, rest);
+        if (!live) s1 = 1.0f;
+        A[i] *= s1;
+        B[i] = s1 * (B[i] + v[s][i]);
+      }
+    }
+    float eA[VEC], eB[VEC];
+    join_groups<VEC>(A, B, eA, eB, group, column, parts[warp]);
+    __syncthreads();
+    if (warp != 0) fetch(next);
+    if (warp == 0) {  // a lane to a channel
+      Record* const record = sc.records + static_cast<int64_t>(m.row) * kWide + lane;
+      const float start = a.dstate && lane < m.channels ? __ldg(a.dstate + m.edge + lane) : 0.0f;
+      float wA = 1.0f, wB = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        wB = fmaf(parts[w][0][lane], wB, parts[w][1][lane]);
+        wA *= parts[w][0][lane];
+      }
+      float state = start;
+      if (m.chunk > 0) {
+        if (!m.last) put(record, wA, wB, 0.0f, 1u);
+        fetch(next);
+        state = enter(record, static_cast<int>(m.chunk), start, lane, err);
+      } else {
+        fetch(next);
+      }
+      if (!m.last) put(record, wA, wB, advance(state, wA, wB), 2u);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        entries[w][lane] = state;
+        state = advance(state, parts[w][0][lane], parts[w][1][lane]);
+      }
+    }
+    if (threadIdx.x == 0) later = atomicAdd(sc.ticket, 1u);
+    __syncthreads();
+    float c[VEC];
+    enter_group<VEC>(c, entries[warp], eA, eB, group, column);
+    rows.template arrived<1>();
+    const int hs = rows.shift(a.hs + m.at - a.channels, stride), xs = SIGMOID ? rows.shift(a.x + m.at, stride) : 0;
+    float *p = a.dgate + m.at + mine * stride + column, *q = a.dx + m.at + mine * stride + column;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
+      if (column >= m.channels || mine + s >= m.steps) continue;
+      float before[VEC], x[VEC] = {}, dgate[VEC], dx[VEC];
+      load_shared<VEC>(before, rows.at(2, s, hs, turn_by));
+      if (m.last && mine + s + 1 == m.steps) start_of<VEC>(before, a.initial, m.edge + column);
+      if (SIGMOID) load_shared<VEC>(x, rows.at(3, s, xs, turn_by));
+      backward_step<VEC, SIGMOID>(g[s], v[s], before, x, mine + s >= m.from, c, dgate, dx);
+      store<VEC>(p, dgate);
+      store<VEC>(q, dx);
+    }
+    if (a.dinitial && column < m.channels && m.last && mine < m.steps && mine + kSteps >= m.steps)
+      store<VEC>(a.dinitial + m.edge + column, c);
+    rows.done();
+    fetch_rest(next);
   }
-  return 1;
+}
+
+// ------------------------------------------------------------------------- launches
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Rows of whole 16-byte words in every buffer.
+bool wide(const Args& a) {
+  const void* all[] = {a.gate, a.x, a.initial, a.h, a.state, a.dh, a.hs, a.dstate, a.dgate, a.dx, a.dinitial};
+  bool fits = a.channels % 4 == 0;
+  for (const void* p : all) fits = fits && aligned(p);
+  return fits;
+}
+
+// Threads walk through time alone where there are few steps, and up to a chunk of them where
+// the channels fill the machine: a chunk that is mostly empty costs its block as much as a
+// full one.
+constexpr int64_t kWalkSteps = 16;
+template <int VEC>
+bool walks(const Args& a) {
+  return a.time <= kWalkSteps || (a.time <= kChunk && a.batch * a.channels >= 256 * VEC * sm_count());
 }
 
 // Whole chains to a block, where the last of their rounds leaves few blocks idle.
-bool walks(int64_t chains, int64_t blocks) { return chains * 10 >= ceil_div(chains, blocks) * blocks * 8; }
+bool takes_whole(int64_t chains, int64_t blocks) { return chains * 10 >= ceil_div(chains, blocks) * blocks * 8; }
 
-// `whole`: a block takes whole chains, and there are no records.
-template <typename Sh>
-int launch_scan(cudaStream_t s, const Args& a, void (*kernel)(Args, Scan, int*), bool whole, void* workspace) {
-  const int64_t blocks = ceil_div(a.channels, kWide), chunks = ceil_div(a.time, Sh::kChunk);
+template <auto kKernel>
+int launch_scan(cudaStream_t s, const Args& a, int threads, int bytes, int per_sm, bool whole, void* workspace) {
+  const int64_t blocks = ceil_div(a.channels, kWide), chunks = ceil_div(a.time, kChunk);
   const int64_t tiles = a.batch * blocks * chunks;
   if (tiles > INT32_MAX) return invalid("recurrence is too large for one call");
   Scan sc;
@@ -854,41 +825,48 @@ int launch_scan(cudaStream_t s, const Args& a, void (*kernel)(Args, Scan, int*),
   sc.tiles = static_cast<unsigned>(tiles);
   sc.records = whole ? nullptr : static_cast<Record*>(workspace);
   sc.ticket = whole ? nullptr : reinterpret_cast<unsigned*>(sc.records + tiles * kWide);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kBytes) != cudaSuccess)
-    return launch_status("recurrence shared memory attribute");
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return launch_status("recurrence shared memory attribute");
+    if (dev >= 0 && dev < 64) attr_done[dev] = true;
+  }
   if (!whole) cudaMemsetAsync(workspace, 0, tiles * kWide * sizeof(Record) + sizeof(unsigned), s);
-  const int64_t grid = std::min<int64_t>(whole ? sc.chains : tiles, Sh::kPerSm * sm_count());
-  TimedLaunch timer("recurrence_scan", s);
-  kernel<<<static_cast<unsigned>(grid), Sh::kThreads, Sh::kBytes, s>>>(a, sc, device_error_word());
+  const int64_t grid = std::min<int64_t>(whole ? sc.chains : tiles, per_sm * sm_count());
+  kKernel<<<static_cast<unsigned>(grid), threads, bytes, s>>>(a, sc, device_error_word());
   return launch_status("recurrence");
 }
 
-template <int VEC, bool SIGMOID, bool BACK>
-int launch(cudaStream_t s, const Args& a, void* workspace) {
-  if (a.time <= kWalkSteps) {
-    const unsigned grid = static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC));
-    TimedLaunch timer(BACK ? "recurrence_walk_backward" : "recurrence_walk", s);
-    if (BACK) walk_backward_kernel<VEC, SIGMOID><<<grid, 256, 0, s>>>(a);
-    else walk_forward_kernel<VEC, SIGMOID><<<grid, 256, 0, s>>>(a);
+template <int VEC, bool SIGMOID>
+int launch_forward(cudaStream_t s, const Args& a, void* workspace) {
+  if (walks<VEC>(a)) {
+    TimedLaunch timer("recurrence_walk", s);
+    walk_forward_kernel<VEC, SIGMOID>
+        <<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
     return launch_status("recurrence");
   }
-  const int64_t chains = a.batch * ceil_div(a.channels, kWide);
-  if constexpr (BACK) {
-    return launch_scan<Shape<VEC, SIGMOID, true>>(s, a, scan_kernel<VEC, SIGMOID, true>, false, workspace);
-  } else {
-    if (walks(chains, Forward<VEC>::kPerSm * sm_count()))
-      return launch_scan<Forward<VEC>>(s, a, scan_forward_kernel<VEC, SIGMOID, true>, true, workspace);
-    return launch_scan<Forward<VEC>>(s, a, scan_forward_kernel<VEC, SIGMOID, false>, false, workspace);
-  }
+  using F = Forward<VEC>;
+  TimedLaunch timer("recurrence_scan", s);
+  const bool whole = takes_whole(a.batch * ceil_div(a.channels, kWide), F::kPerSm * sm_count());
+  if (whole)
+    return launch_scan<scan_forward_kernel<VEC, SIGMOID, true>>(s, a, F::kThreads, F::kBytes, F::kPerSm, true, nullptr);
+  return launch_scan<scan_forward_kernel<VEC, SIGMOID, false>>(s, a, F::kThreads, F::kBytes, F::kPerSm, false,
+                                                               workspace);
 }
 
-template <bool SIGMOID, bool BACK>
-int launch_width(cudaStream_t s, const Args& a, void* workspace) {
-  switch (width_of(a)) {
-    case 4: return launch<4, SIGMOID, BACK>(s, a, workspace);
-    case 2: return launch<2, SIGMOID, BACK>(s, a, workspace);
-    default: return launch<1, SIGMOID, BACK>(s, a, workspace);
+template <int VEC, bool SIGMOID>
+int launch_backward(cudaStream_t s, const Args& a, void* workspace) {
+  if (walks<VEC>(a)) {
+    TimedLaunch timer("recurrence_walk_backward", s);
+    walk_backward_kernel<VEC, SIGMOID>
+        <<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
+    return launch_status("recurrence");
   }
+  using K = Backward<VEC, SIGMOID>;
+  TimedLaunch timer("recurrence_scan_backward", s);
+  return launch_scan<scan_backward_kernel<VEC, SIGMOID>>(s, a, K::kThreads, K::kBytes, K::kPerSm, false, workspace);
 }
 
 // A call of no steps: the state goes through.
@@ -915,7 +893,7 @@ using namespace tcx;
 extern "C" size_t tcx_sm100_recurrence_workspace_bytes(int64_t batch, int64_t time, int64_t channels) {
   if (check_recurrence(TCX_RECURRENCE_DECAY, batch, time, channels) || time <= kWalkSteps) return 0;
   // a record per channel for each chunk, and the ticket
-  const int64_t tiles = batch * ceil_div(channels, kWide) * ceil_div(time, kLeastChunk);
+  const int64_t tiles = batch * ceil_div(channels, kWide) * ceil_div(time, kChunk);
   return static_cast<size_t>(tiles) * kWide * sizeof(Record) + sizeof(unsigned);
 }
 
@@ -933,8 +911,9 @@ extern "C" int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const
          channels};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (time == 0) return pass_through(s, initial, state, batch * channels);
-  return form == TCX_RECURRENCE_SIGMOID ? launch_width<true, false>(s, a, workspace)
-                                        : launch_width<false, false>(s, a, workspace);
+  const bool sigmoid = form == TCX_RECURRENCE_SIGMOID;
+  if (wide(a)) return sigmoid ? launch_forward<4, true>(s, a, workspace) : launch_forward<4, false>(s, a, workspace);
+  return sigmoid ? launch_forward<1, true>(s, a, workspace) : launch_forward<1, false>(s, a, workspace);
 }
 
 extern "C" int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, const float* dh, const float* gate,
@@ -952,6 +931,7 @@ extern "C" int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, cons
   Args a{gate, x, initial, lengths, nullptr, nullptr, dh, h, dstate, dgate, dx, dinitial, batch, time, channels};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (time == 0) return pass_through(s, dstate, dinitial, batch * channels);
-  return form == TCX_RECURRENCE_SIGMOID ? launch_width<true, true>(s, a, workspace)
-                                        : launch_width<false, true>(s, a, workspace);
+  const bool sigmoid = form == TCX_RECURRENCE_SIGMOID;
+  if (wide(a)) return sigmoid ? launch_backward<4, true>(s, a, workspace) : launch_backward<4, false>(s, a, workspace);
+  return sigmoid ? launch_backward<1, true>(s, a, workspace) : launch_backward<1, false>(s, a, workspace);
 }
