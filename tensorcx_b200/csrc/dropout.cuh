@@ -48,10 +48,26 @@ __device__ __forceinline__ uint32_t word_of(uint4 w, uint32_t i) {
   return i & 2u ? hi : lo;
 }
 
+// The words of places e .. e + 3: one block when e starts one, else two.
+__device__ __forceinline__ uint4 words_at(uint64_t e, const philox::RoundKeys& rk) {
+  const uint4 a = philox::block_words(e >> 2, rk);
+  const uint32_t r = static_cast<uint32_t>(e & 3);
+  if (r == 0) return a;
+  const uint4 b = philox::block_words((e >> 2) + 1, rk);
+  return r == 1 ? make_uint4(a.y, a.z, a.w, b.x) : r == 2 ? make_uint4(a.z, a.w, b.x, b.y) : make_uint4(a.w, b.x, b.y, b.z);
+}
+
 __device__ __forceinline__ bool kept(uint32_t word, uint32_t threshold) { return (word >> 8) >= threshold; }
 
 __device__ __forceinline__ float dropped(float x, bool keep, float scale) {
   return keep ? __fmul_rn(x, scale) : 0.0f;
+}
+
+__device__ __forceinline__ float4 dropped4(float4 x, uint64_t e, const philox::RoundKeys& rk, uint32_t threshold,
+                                           float scale) {
+  const uint4 w = words_at(e, rk);
+  return make_float4(dropped(x.x, kept(w.x, threshold), scale), dropped(x.y, kept(w.y, threshold), scale),
+                     dropped(x.z, kept(w.z, threshold), scale), dropped(x.w, kept(w.w, threshold), scale));
 }
 
 }  // namespace tcx
