@@ -63,6 +63,13 @@ __device__ __forceinline__ float dropped(float x, bool keep, float scale) {
   return keep ? __fmul_rn(x, scale) : 0.0f;
 }
 
+// Bit j: place e + j is kept.
+__device__ __forceinline__ uint32_t kept4(uint64_t e, const philox::RoundKeys& rk, uint32_t threshold) {
+  const uint4 w = words_at(e, rk);
+  return (kept(w.x, threshold) ? 1u : 0u) | (kept(w.y, threshold) ? 2u : 0u) | (kept(w.z, threshold) ? 4u : 0u) |
+         (kept(w.w, threshold) ? 8u : 0u);
+}
+
 __device__ __forceinline__ float4 dropped4(float4 x, uint64_t e, const philox::RoundKeys& rk, uint32_t threshold,
                                            float scale) {
   const uint4 w = words_at(e, rk);

@@ -203,10 +203,16 @@ struct Words {
       if (valid(word, 3)) q[3] = v.w;
     }
   }
+  // The word with `other` outside the row.
+  __device__ __forceinline__ float4 within(int word, float4 v, float other) const {
+    return make_float4(valid(word, 0) ? v.x : other, valid(word, 1) ? v.y : other, valid(word, 2) ? v.z : other,
+                       valid(word, 3) ? v.w : other);
+  }
   // A word of a vector over the columns (nothing outside the row).
   __device__ __forceinline__ float4 column(const float* p, int word) const {
     if (!ODD) return __ldg(reinterpret_cast<const float4*>(p) + word);
     const float* const q = p + 4 * word - phase;
+    if (whole(word)) return make_float4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (valid(word, 0)) v.x = __ldg(q);
     if (valid(word, 1)) v.y = __ldg(q + 1);
@@ -224,6 +230,7 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
   using B = Block<THREADS>;
   const int tid = threadIdx.x;
   const float n = static_cast<float>(a.cols);
+  const philox::RoundKeys rk = philox::round_keys(a.drop.key);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const Words<ODD> words(row, a.cols, a.rows);
     float v[VPT][4];
@@ -235,6 +242,7 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
     } else {
       level = __ldg(a.x + first);
     }
+    float4 res[FUSED ? VPT : 1];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int word = tid + k * THREADS;
@@ -242,43 +250,68 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
       if (words.holds(word)) t = words.load(a.x, word);
       v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
     }
+    if (FUSED && a.residual) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k)
+        if (words.holds(tid + k * THREADS)) res[FUSED ? k : 0] = words.load(a.residual, tid + k * THREADS);
+    }
     if (FUSED) {
-      const philox::RoundKeys rk = philox::round_keys(a.drop.key);
-      const uint64_t start = dropout_start(a.drop) + static_cast<uint64_t>(words.at);
+      if (a.drop.threshold) {
+        // the mask while the loads are on their way: 4 bits to a word
+        static_assert(!FUSED || VPT <= 16, "the mask's bits");
+        const uint64_t start = dropout_start(a.drop) + static_cast<uint64_t>(words.at);
+        uint32_t mask[(VPT + 7) / 8] = {};
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+          mask[k / 8] |= kept4(start + 4 * static_cast<uint64_t>(tid + k * THREADS), rk, a.drop.threshold) << (4 * (k % 8));
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[k][j] = dropped(v[k][j], mask[k / 8] >> (4 * (k % 8) + j) & 1, a.drop.scale);
+      }
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int word = tid + k * THREADS;
         if (words.holds(word)) {
-          float4 t = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
-          if (a.drop.threshold) t = dropped4(t, start + 4 * static_cast<uint64_t>(word), rk, a.drop.threshold, a.drop.scale);
           if (a.residual) {
-            const float4 r = words.load(a.residual, word);
-            t = make_float4(__fadd_rn(r.x, t.x), __fadd_rn(r.y, t.y), __fadd_rn(r.z, t.z), __fadd_rn(r.w, t.w));
+            const float4 r = res[FUSED ? k : 0];
+            v[k][0] = __fadd_rn(r.x, v[k][0]), v[k][1] = __fadd_rn(r.y, v[k][1]);
+            v[k][2] = __fadd_rn(r.z, v[k][2]), v[k][3] = __fadd_rn(r.w, v[k][3]);
           }
-          words.store(a.total, word, t);
-          v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
+          words.store(a.total, word, make_float4(v[k][0], v[k][1], v[k][2], v[k][3]));
+        } else {
+          v[k][0] = v[k][1] = v[k][2] = v[k][3] = level;
         }
       }
     }
     float s = 0.0f;
 #pragma unroll
-    for (int k = 0; k < VPT; ++k)
+    for (int k = 0; k < VPT; ++k) {
+      const int word = tid + k * THREADS;
+      if (!words.whole(word)) {  // nothing for what is outside the row
+        const float4 t = words.within(word, make_float4(v[k][0], v[k][1], v[k][2], v[k][3]), level);
+        v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (words.valid(tid + k * THREADS, j)) s += v[k][j] - level;  // 0 past the row's words
+      for (int j = 0; j < 4; ++j) s += v[k][j] - level;
+    }
     const float m1 = level + __fdiv_rn(B::sum(s, smem), n);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int word = tid + k * THREADS;
       if (words.holds(word)) {
+        float d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = v[k][j] -= m1;
+        if (!words.whole(word)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[j] = words.valid(word, j) ? d[j] : 0.0f;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[k][j] -= m1;
-          if (words.valid(word, j)) {
-            s1 += v[k][j];
-            s2 = fmaf(v[k][j], v[k][j], s2);
-          }
+          s1 += d[j];
+          s2 = fmaf(d[j], d[j], s2);
         }
       }
     }
@@ -315,22 +348,35 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
 // time. A group's rows are a multiple of 4 apart, so that they all start in the same phase
 // and a thread's columns are the same in each: the weight's and the bias's gradients add up in
 // its registers over the group's rows, the groups' in shared memory, and the blocks' in a
-// second kernel, each in a fixed order. The next row's words are loaded before this row's sums
-// are taken.
+// second kernel, each in a fixed order.
+//
+// dy and total come through a ring of places in shared memory (cp.async; a thread copies and
+// reads its own words only, so that needs no barrier): a place is copied into again as soon as
+// its row is in registers, while that row's sums cross the block.
+template <int TPR, int GROUPS, int VPT>
+struct BackwardShape {
+  static constexpr int kThreads = TPR * GROUPS;
+  static constexpr int kPerSm = 512 / kThreads, kRing = 3;
+  static constexpr int kPlaces = kRing * 2 * VPT * kThreads * 16, kColumns = GROUPS > 1 ? 2 * 4 * TPR * VPT * 4 : 0;
+  static constexpr int kBytes = kPlaces > kColumns ? kPlaces : kColumns;
+};
+
 template <int TPR, int GROUPS, int VPT, int CLUSTER, bool ODD, bool FUSED>
-__global__ void __launch_bounds__(TPR* GROUPS, 512 / (TPR * GROUPS)) norm_backward_kernel(BackwardArgs a, float* partial,
-                                                                                        int* err) {
-  constexpr int kWarps = TPR / 32, kSpan = TPR * VPT;  // words of a block's part of a row
+__global__ void __launch_bounds__(TPR* GROUPS, BackwardShape<TPR, GROUPS, VPT>::kPerSm)
+norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
+  constexpr int kThreadsAll = TPR * GROUPS, kWarps = TPR / 32, kSpan = TPR * VPT;  // words of a block's part of a row
+  constexpr int kRing = BackwardShape<TPR, GROUPS, VPT>::kRing;
   static_assert(CLUSTER == 1 || GROUPS == 1, "");
-  __shared__ float2 sums[2][GROUPS][kWarps];
+  extern __shared__ __align__(16) float4 stage[];
+  __shared__ float sums[2][GROUPS][2][kWarps];
   __shared__ float2 peers[2][CLUSTER];
   __shared__ __align__(8) uint64_t arrived[2];
-  __shared__ float columns[GROUPS > 1 ? 2 * 4 * kSpan : 1];
   const int tid = threadIdx.x % TPR, group = threadIdx.x / TPR, lane = tid & 31, warp = tid >> 5;
   const int rank = CLUSTER > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
+  const int first_word = rank * kSpan + tid;
   const int64_t step = static_cast<int64_t>(gridDim.x / CLUSTER) * GROUPS;
   const int64_t opening = static_cast<int64_t>(blockIdx.x / CLUSTER) * GROUPS + group;
-  const float n = static_cast<float>(a.cols);
+  const float share = 1.0f / static_cast<float>(a.cols);
   if (CLUSTER > 1) {
     if (threadIdx.x == 0) {
       ptx::mbar_init(ptx::smem_u32(&arrived[0]), 1);
@@ -341,95 +387,132 @@ __global__ void __launch_bounds__(TPR* GROUPS, 512 / (TPR * GROUPS)) norm_backwa
   }
   bool live = true;  // false once a wait gave up: later ones are skipped
 
+  const Words<ODD> columns_of(opening, a.cols, a.rows);  // its phase, cols and words: those of all its rows
   float dw[VPT][4], db[VPT][4];
+  float4 weight[ODD ? VPT : 1];
 #pragma unroll
-  for (int k = 0; k < VPT; ++k)
+  for (int k = 0; k < VPT; ++k) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[k][j] = db[k][j] = 0.0f;
-  float4 dy[VPT], t[VPT];
-  float mean = 0.0f, rstd = 0.0f;
-  auto fetch = [&](int64_t row) {
-    if (row >= a.rows) return;
-    const Words<ODD> words(row, a.cols, a.rows);
+    if (ODD) weight[ODD ? k : 0] = a.weight ? columns_of.column(a.weight, first_word + k * TPR) : make_float4(1, 1, 1, 1);
+  }
+
+  // Copies a row into a place: word k of dy and of total.
+  auto copy = [&](int place, int64_t row) {
+    if (row < a.rows) {
+      const Words<ODD> words(row, a.cols, a.rows);
+      float4* const to = stage + place * (2 * VPT * kThreadsAll) + threadIdx.x;
+      const int64_t at = words.at + 4 * static_cast<int64_t>(first_word);
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int word = rank * kSpan + tid + k * TPR;
-      if (words.holds(word)) {
-        dy[k] = words.load(a.dy, word);
-        t[k] = words.load(a.total, word);
+      for (int k = 0; k < VPT; ++k) {
+        if (words.holds(first_word + k * TPR)) {
+          const int64_t i = at + 4 * k * TPR;
+          const int bytes = !ODD || i + 4 <= words.count ? 16 : 4 * static_cast<int>(words.count - i);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + k * kThreadsAll)),
+                       "l"(a.dy + i), "r"(bytes)
+                       : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + (VPT + k) * kThreadsAll)),
+                       "l"(a.total + i), "r"(bytes)
+                       : "memory");
+        }
       }
     }
-    mean = __ldg(a.mean + row);
-    rstd = __ldg(a.rstd + row);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  fetch(opening);
+  auto statistics = [&](int64_t row, float& m, float& r) {
+    m = row < a.rows ? __ldg(a.mean + row) : 0.0f;
+    r = row < a.rows ? __ldg(a.rstd + row) : 0.0f;
+  };
+
   const philox::RoundKeys rk = philox::round_keys(a.drop.key);
-  const uint64_t place = FUSED ? dropout_start(a.drop) : 0;
+  const uint64_t from = FUSED ? dropout_start(a.drop) : 0;
+#pragma unroll
+  for (int k = 0; k < kRing; ++k) copy(k, opening + k * step);
+  float mean, rstd, next_mean, next_rstd;
+  statistics(opening, mean, rstd);
   unsigned turn = 0;
+  int place = 0;
   for (int64_t row = opening; row < a.rows; row += step, ++turn) {
     const Words<ODD> words(row, a.cols, a.rows);
-    float g[VPT][4], hat[VPT][4];
-    const float r = rstd;
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int word = rank * kSpan + tid + k * TPR;
-      const bool in = words.holds(word);
-      float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-      if (a.weight && in) w = words.column(a.weight, word);
-      const float y4[4] = {dy[k].x, dy[k].y, dy[k].z, dy[k].w}, t4[4] = {t[k].x, t[k].y, t[k].z, t[k].w};
-      const float w4[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool ok = in && words.valid(word, j);
-        const float d = ok ? y4[j] : 0.0f;
-        hat[k][j] = ok ? (t4[j] - mean) * r : 0.0f;
-        g[k][j] = d * w4[j];
-        s1 += g[k][j];
-        s2 = fmaf(g[k][j], hat[k][j], s2);
-        dw[k][j] = fmaf(d, hat[k][j], dw[k][j]);
-        db[k][j] += d;
-      }
-    }
-    fetch(row + step);
+    statistics(row + step, next_mean, next_rstd);
     float4 extra[FUSED ? VPT : 1];
     if (FUSED && a.dtotal) {
 #pragma unroll
-      for (int k = 0; k < VPT; ++k) {
-        const int word = rank * kSpan + tid + k * TPR;
-        if (words.holds(word)) extra[FUSED ? k : 0] = words.load(a.dtotal, word);
+      for (int k = 0; k < VPT; ++k)
+        if (words.holds(first_word + k * TPR)) extra[FUSED ? k : 0] = words.load(a.dtotal, first_word + k * TPR);
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+    const float4* const here = stage + place * (2 * VPT * kThreadsAll) + threadIdx.x;
+    float g[VPT][4], hat[VPT][4];
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int word = first_word + k * TPR;
+      const bool in = words.holds(word);
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), t = make_float4(mean, mean, mean, mean);
+      float4 w = ODD ? weight[ODD ? k : 0] : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      if (in) {
+        y = here[k * kThreadsAll];
+        t = here[(VPT + k) * kThreadsAll];
+        if (!ODD && a.weight) w = words.column(a.weight, word);
+        if (!words.whole(word)) {
+          y = words.within(word, y, 0.0f);
+          t = words.within(word, t, mean);
+        }
+      }
+      const float y4[4] = {y.x, y.y, y.z, y.w}, t4[4] = {t.x, t.y, t.z, t.w}, w4[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        hat[k][j] = (t4[j] - mean) * rstd;
+        g[k][j] = y4[j] * w4[j];
+        s1 += g[k][j];
+        s2 = fmaf(g[k][j], hat[k][j], s2);
+        dw[k][j] = fmaf(y4[j], hat[k][j], dw[k][j]);
+        db[k][j] += y4[j];
       }
     }
+    copy(place, row + kRing * step);
+    place = place + 1 == kRing ? 0 : place + 1;
+    uint32_t mask = 0;
+    if (FUSED && a.dx) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      s1 += __shfl_xor_sync(0xffffffffu, s1, off);
-      s2 += __shfl_xor_sync(0xffffffffu, s2, off);
+      for (int k = 0; k < VPT; ++k)
+        mask |= kept4(from + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(first_word + k * TPR), rk,
+                      a.drop.threshold)
+                << (4 * k);
     }
+    // both sums in one butterfly: the lower lanes take s1, the upper ones s2
+    const bool upper = lane & 16;
+    float s = (upper ? s2 : s1) + __shfl_xor_sync(0xffffffffu, upper ? s1 : s2, 16);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
     if (kWarps > 1) {
-      if (lane == 0) sums[turn & 1][group][warp] = make_float2(s1, s2);
+      if ((lane & 15) == 0) sums[turn & 1][group][lane >> 4][warp] = s;
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(TPR) : "memory");
       s1 = s2 = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float2 v = sums[turn & 1][group][w];
-        s1 += v.x;
-        s2 += v.y;
+        s1 += sums[turn & 1][group][0][w];
+        s2 += sums[turn & 1][group][1][w];
       }
+    } else {
+      s1 = __shfl_sync(0xffffffffu, s, 0);
+      s2 = __shfl_sync(0xffffffffu, s, 16);
     }
     if (CLUSTER > 1) {
-      // this block's sums go to every block of the cluster, its own too; the slots of a parity
-      // are read (before the block's next barrier) ahead of the row after next's sums
+      // This block's sums go to every block of the cluster, its own too. A peer that sends
+      // those of the row after next has this block's of the next row, which are sent when all
+      // of its threads have read this row's slots.
       const uint32_t bar = ptx::smem_u32(&arrived[turn & 1]);
       if (threadIdx.x == 0) ptx::mbar_expect_tx(bar, CLUSTER * 8);
       if (threadIdx.x < CLUSTER) {
-        const uint32_t peer = threadIdx.x;
-        const uint32_t slot = ptx::map_rank(ptx::smem_u32(&peers[turn & 1][rank]), peer);
-        const uint32_t its = ptx::map_rank(bar, peer);
+        const uint32_t slot = ptx::map_rank(ptx::smem_u32(&peers[turn & 1][rank]), threadIdx.x);
+        const uint32_t its = ptx::map_rank(bar, threadIdx.x);
         asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(slot),
                      "r"(__float_as_uint(s1)), "r"(__float_as_uint(s2)), "r"(its)
                      : "memory");
       }
-      if (live) live = ptx::wait_or_give_up(bar, (turn >> 1) & 1, err, 0x601);
+      if (live) live = ptx::wait_or_give_up(bar, turn >> 1 & 1, err, 0x601);
       s1 = s2 = 0.0f;
 #pragma unroll
       for (int c = 0; c < CLUSTER; ++c) {
@@ -438,38 +521,39 @@ __global__ void __launch_bounds__(TPR* GROUPS, 512 / (TPR * GROUPS)) norm_backwa
         s2 += v.y;
       }
     }
-    const float c1 = __fdiv_rn(s1, n), c2 = __fdiv_rn(s2, n);
+    const float c1 = -rstd * (s1 * share), c2 = -rstd * (s2 * share);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = rank * kSpan + tid + k * TPR;
+      const int word = first_word + k * TPR;
       if (!words.holds(word)) continue;
-      float4 d = make_float4(r * (g[k][0] - c1 - hat[k][0] * c2), r * (g[k][1] - c1 - hat[k][1] * c2),
-                             r * (g[k][2] - c1 - hat[k][2] * c2), r * (g[k][3] - c1 - hat[k][3] * c2));
+      float d[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = fmaf(hat[k][j], c2, fmaf(g[k][j], rstd, c1));
       if (FUSED && a.dtotal) {
         const float4 e = extra[FUSED ? k : 0];
-        d = make_float4(d.x + e.x, d.y + e.y, d.z + e.z, d.w + e.w);
+        d[0] += e.x, d[1] += e.y, d[2] += e.z, d[3] += e.w;
       }
-      words.store(a.dresidual, word, d);
-      if (FUSED && a.dx)
-        words.store(a.dx, word,
-                    dropped4(d, place + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(word), rk,
-                             a.drop.threshold, a.drop.scale));
+      words.store(a.dresidual, word, make_float4(d[0], d[1], d[2], d[3]));
+      if (FUSED && a.dx) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = dropped(d[j], mask >> (4 * k + j) & 1, a.drop.scale);
+        words.store(a.dx, word, make_float4(d[0], d[1], d[2], d[3]));
+      }
     }
+    mean = next_mean, rstd = next_rstd;
   }
   dependents_may_launch();
   if (CLUSTER > 1) ptx::cluster_sync_all();  // no block leaves while a peer may still send to it
   if (!partial) return;
 
   const int64_t at = static_cast<int64_t>(blockIdx.x / CLUSTER) * 2 * a.cols;
+  const Words<ODD>& words = columns_of;  // a group without rows adds zeros
   if (GROUPS == 1) {
-    // a group without rows has the phase that its rows would have
-    const Words<ODD> words(opening, a.cols, a.rows);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = rank * kSpan + tid + k * TPR;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int c = 4 * word + j - words.phase;
+        const int c = 4 * (first_word + k * TPR) + j - words.phase;
         if (c >= 0 && c < words.cols) {
           partial[at + c] = dw[k][j];
           partial[at + a.cols + c] = db[k][j];
@@ -477,16 +561,18 @@ __global__ void __launch_bounds__(TPR* GROUPS, 512 / (TPR * GROUPS)) norm_backwa
       }
     }
   } else {
-    for (int i = threadIdx.x; i < 2 * 4 * kSpan; i += TPR * GROUPS) columns[i] = 0.0f;
-    for (int turn_of = 0; turn_of < GROUPS; ++turn_of) {
+    float* const columns = reinterpret_cast<float*>(stage);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * 4 * kSpan; i += kThreadsAll) columns[i] = 0.0f;
+    for (int whose = 0; whose < GROUPS; ++whose) {
       __syncthreads();
-      if (group != turn_of) continue;
-      const Words<ODD> words(opening, a.cols, a.rows);
+      if (group != whose) continue;
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int c = 4 * (tid + k * TPR) + j - words.phase;
+          const int c = 4 * (first_word + k * TPR) + j - words.phase;
           if (c >= 0 && c < words.cols) {
             columns[c] += dw[k][j];
             columns[4 * kSpan + c] += db[k][j];
@@ -494,7 +580,7 @@ __global__ void __launch_bounds__(TPR* GROUPS, 512 / (TPR * GROUPS)) norm_backwa
         }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < static_cast<int>(a.cols); c += TPR * GROUPS) {
+    for (int c = threadIdx.x; c < static_cast<int>(a.cols); c += kThreadsAll) {
       partial[at + c] = columns[c];
       partial[at + a.cols + c] = columns[4 * kSpan + c];
     }
@@ -538,62 +624,122 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 // Words that a row can touch.
 int64_t words_of(int64_t cols) { return cols % 4 ? (cols + 6) / 4 : cols / 4; }
 
-template <int THREADS, int VPT>
-void launch_forward(cudaStream_t s, const ForwardArgs& a, bool odd, bool fused) {
+template <int THREADS, int VPT, bool FUSED>
+void launch_forward(cudaStream_t s, const ForwardArgs& a, bool odd) {
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 30));
-  if (odd) {
-    if (fused) norm_forward_kernel<THREADS, VPT, true, true><<<grid, THREADS, 0, s>>>(a);
-    else norm_forward_kernel<THREADS, VPT, true, false><<<grid, THREADS, 0, s>>>(a);
+  if (odd) norm_forward_kernel<THREADS, VPT, true, FUSED><<<grid, THREADS, 0, s>>>(a);
+  else norm_forward_kernel<THREADS, VPT, false, FUSED><<<grid, THREADS, 0, s>>>(a);
+}
+
+// Small blocks of many words: 64 values to a thread, or 32 of each of two inputs.
+void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
+  if (a.total) {
+    if (words <= 32) launch_forward<32, 1, true>(s, a, odd);
+    else if (words <= 64) launch_forward<32, 2, true>(s, a, odd);
+    else if (words <= 128) launch_forward<32, 4, true>(s, a, odd);
+    else if (words <= 256) launch_forward<32, 8, true>(s, a, odd);
+    else if (words <= 512) launch_forward<64, 8, true>(s, a, odd);
+    else if (words <= 1024) launch_forward<128, 8, true>(s, a, odd);
+    else if (words <= 2048) launch_forward<256, 8, true>(s, a, odd);
+    else if (words <= 4096) launch_forward<512, 8, true>(s, a, odd);
+    else launch_forward<512, 16, true>(s, a, odd);
   } else {
-    if (fused) norm_forward_kernel<THREADS, VPT, false, true><<<grid, THREADS, 0, s>>>(a);
-    else norm_forward_kernel<THREADS, VPT, false, false><<<grid, THREADS, 0, s>>>(a);
+    if (words <= 32) launch_forward<32, 1, false>(s, a, odd);
+    else if (words <= 64) launch_forward<32, 2, false>(s, a, odd);
+    else if (words <= 128) launch_forward<32, 4, false>(s, a, odd);
+    else if (words <= 256) launch_forward<32, 8, false>(s, a, odd);
+    else if (words <= 512) launch_forward<32, 16, false>(s, a, odd);
+    else if (words <= 1024) launch_forward<64, 16, false>(s, a, odd);
+    else if (words <= 2048) launch_forward<128, 16, false>(s, a, odd);
+    else if (words <= 4096) launch_forward<256, 16, false>(s, a, odd);
+    else launch_forward<512, 16, false>(s, a, odd);
   }
 }
 
 // Blocks (or clusters) that the backward kernel runs as: what the machine holds at a time, no
-// more than there are rows for, and a multiple of 4 groups (rows a group apart keep the phase).
-int64_t backward_blocks(int64_t rows, int groups, int resident) {
+// more than there are rows for; where rows start in different phases, a multiple of
+// 4 (the rows of a group are that far apart).
+int64_t backward_blocks(int64_t rows, int64_t cols, int groups, int resident) {
   const int64_t want = std::min<int64_t>(ceil_div(rows, groups), resident);
-  return ceil_div(want, 4) * 4;
+  return cols % 4 == 0 ? want : std::max<int64_t>(4, want / 4 * 4);
 }
 
 struct BackwardPlan {
-  int threads, groups, cluster;  // threads of a block, rows of a block at a time, blocks of a row; threads 0: none
-  int64_t blocks;                // or clusters: partial rows
+  int tpr, vpt, cluster;  // threads of a block to a row, their words, blocks to a row; tpr 0: none
+  int64_t blocks;         // or clusters: partial rows, at most
 };
 
 BackwardPlan backward_plan(int64_t rows, int64_t cols) {
   const int64_t words = words_of(cols);
   if (words > 8 * 2048) return {0, 0, 0, 0};
-  const int tpr = words <= 128 ? 32 : words <= 256 ? 64 : words <= 512 ? 128 : words <= 1024 ? 256 : 512;
-  const int cluster = words <= 2048 ? 1 : words <= 4096 ? 2 : words <= 8192 ? 4 : 8;
-  const int groups = tpr < 256 ? 256 / tpr : 1, threads = tpr * groups;
-  return {threads, groups, cluster, backward_blocks(rows, groups, 512 / threads * sm_count() / cluster)};
+  const int tpr = words <= 128 ? 32 : words <= 256 ? 64 : words <= 512 ? 128 : words <= 8192 ? 256 : 512;
+  const int vpt = words <= 32 ? 1 : words <= 64 ? 2 : 4;
+  const int cluster = words <= 1024 ? 1 : words <= 2048 ? 2 : words <= 4096 ? 4 : 8;
+  const int threads = tpr < 256 ? 256 : tpr, groups = threads / tpr;
+  return {tpr, vpt, cluster, backward_blocks(rows, cols, groups, 512 / threads * sm_count() / cluster)};
 }
 
 template <int TPR, int GROUPS, int VPT, int CLUSTER, bool ODD, bool FUSED>
-void launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan) {
+int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial) {
+  using Sh = BackwardShape<TPR, GROUPS, VPT>;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(plan.blocks * CLUSTER));
   cfg.blockDim = dim3(TPR * GROUPS);
+  cfg.dynamicSmemBytes = Sh::kBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {CLUSTER, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = CLUSTER > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, norm_backward_kernel<TPR, GROUPS, VPT, CLUSTER, ODD, FUSED>, a, partial, device_error_word());
+  auto* kernel = norm_backward_kernel<TPR, GROUPS, VPT, CLUSTER, ODD, FUSED>;
+  // how many blocks or clusters the device holds at a time, looked up once per device
+  static int resident[64] = {0};
+  int dev = 0, held = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64) held = resident[dev];
+  if (held == 0) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kBytes);
+    held = Sh::kPerSm * sm_count() / CLUSTER;
+    cfg.gridDim = dim3(static_cast<unsigned>(held * CLUSTER));
+    int clusters = 0;
+    if (CLUSTER > 1 && cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0)
+      held = std::min(held, clusters);
+    if (dev >= 0 && dev < 64) resident[dev] = held;
+  }
+  const int64_t blocks = backward_blocks(a.rows, a.cols, GROUPS, held);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * CLUSTER));
+  cudaLaunchKernelEx(&cfg, kernel, a, partial, device_error_word());
+  return blocks;
 }
 
 template <int TPR, int GROUPS, int VPT, int CLUSTER>
-void launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd,
-                     bool fused) {
-  if (odd) {
-    if (fused) launch_backward<TPR, GROUPS, VPT, CLUSTER, true, true>(s, a, partial, plan);
-    else launch_backward<TPR, GROUPS, VPT, CLUSTER, true, false>(s, a, partial, plan);
-  } else {
-    if (fused) launch_backward<TPR, GROUPS, VPT, CLUSTER, false, true>(s, a, partial, plan);
-    else launch_backward<TPR, GROUPS, VPT, CLUSTER, false, false>(s, a, partial, plan);
+int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, bool odd) {
+  const bool fused = a.dtotal || a.dx;
+  if (odd)
+    return fused ? launch_backward<TPR, GROUPS, VPT, CLUSTER, true, true>(s, a, partial)
+                 : launch_backward<TPR, GROUPS, VPT, CLUSTER, true, false>(s, a, partial);
+  return fused ? launch_backward<TPR, GROUPS, VPT, CLUSTER, false, true>(s, a, partial)
+               : launch_backward<TPR, GROUPS, VPT, CLUSTER, false, false>(s, a, partial);
+}
+
+// Returns the partial rows that it leaves.
+int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd) {
+  switch (plan.cluster) {
+    case 2: return launch_backward<256, 1, 4, 2>(s, a, partial, odd);
+    case 4: return launch_backward<256, 1, 4, 4>(s, a, partial, odd);
+    case 8:
+      return plan.tpr == 256 ? launch_backward<256, 1, 4, 8>(s, a, partial, odd)
+                             : launch_backward<512, 1, 4, 8>(s, a, partial, odd);
+    default: break;
+  }
+  switch (plan.tpr) {
+    case 32:
+      return plan.vpt == 1   ? launch_backward<32, 8, 1, 1>(s, a, partial, odd)
+             : plan.vpt == 2 ? launch_backward<32, 8, 2, 1>(s, a, partial, odd)
+                             : launch_backward<32, 8, 4, 1>(s, a, partial, odd);
+    case 64: return launch_backward<64, 4, 4, 1>(s, a, partial, odd);
+    case 128: return launch_backward<128, 2, 4, 1>(s, a, partial, odd);
+    default: return launch_backward<256, 1, 4, 1>(s, a, partial, odd);
   }
 }
 
@@ -632,16 +778,8 @@ extern "C" int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* inp
     norm_forward_any_kernel<<<grid, kThreads, 0, s>>>(a);
     return launch_status("layer norm forward");
   }
-  const bool odd = cols % 4 != 0 || !aligned(weight) || !aligned(bias), fused = a.total != nullptr;
-  if (words <= 32) launch_forward<32, 1>(s, a, odd, fused);
-  else if (words <= 64) launch_forward<32, 2>(s, a, odd, fused);
-  else if (words <= 128) launch_forward<32, 4>(s, a, odd, fused);
-  else if (words <= 256) launch_forward<32, 8>(s, a, odd, fused);
-  else if (words <= 512) launch_forward<32, 16>(s, a, odd, fused);
-  else if (words <= 1024) launch_forward<64, 16>(s, a, odd, fused);
-  else if (words <= 2048) launch_forward<128, 16>(s, a, odd, fused);
-  else if (words <= 4096) launch_forward<256, 16>(s, a, odd, fused);
-  else launch_forward<512, 16>(s, a, odd, fused);
+  const bool odd = cols % 4 != 0 || !aligned(weight) || !aligned(bias);
+  launch_forward(s, a, words, odd);
   return launch_status("layer norm forward");
 }
 
@@ -680,22 +818,11 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
   TimedLaunch timer("norm_backward", s);
   float* partial = dweight ? static_cast<float*>(workspace) : nullptr;
   const BackwardPlan plan = backward_plan(rows, cols);
-  if (plan.threads && aligned(dy) && aligned(total) && aligned(dtotal) && aligned(dresidual) && aligned(a.dx)) {
-    const bool odd = cols % 4 != 0 || !aligned(weight), fused = dtotal || a.dx;
-    const int64_t words = words_of(cols);
-    if (words <= 32) launch_backward<32, 8, 1, 1>(s, a, partial, plan, odd, fused);
-    else if (words <= 64) launch_backward<32, 8, 2, 1>(s, a, partial, plan, odd, fused);
-    else if (words <= 128) launch_backward<32, 8, 4, 1>(s, a, partial, plan, odd, fused);
-    else if (words <= 256) launch_backward<64, 4, 4, 1>(s, a, partial, plan, odd, fused);
-    else if (words <= 512) launch_backward<128, 2, 4, 1>(s, a, partial, plan, odd, fused);
-    else if (words <= 1024) launch_backward<256, 1, 4, 1>(s, a, partial, plan, odd, fused);
-    else if (words <= 2048) launch_backward<512, 1, 4, 1>(s, a, partial, plan, odd, fused);
-    else if (words <= 4096) launch_backward<512, 1, 4, 2>(s, a, partial, plan, odd, fused);
-    else if (words <= 8192) launch_backward<512, 1, 4, 4>(s, a, partial, plan, odd, fused);
-    else launch_backward<512, 1, 4, 8>(s, a, partial, plan, odd, fused);
+  if (plan.tpr && aligned(dy) && aligned(total) && aligned(dtotal) && aligned(dresidual) && aligned(a.dx)) {
+    const int64_t splits = launch_backward(s, a, partial, plan, cols % 4 != 0 || !aligned(weight));
     if (partial)
       launch_after(norm_join_kernel, dim3(static_cast<unsigned>(ceil_div(cols, 32))), dim3(1024), s, 0, partial,
-                   static_cast<int>(plan.blocks), cols, dweight, dbias);
+                   static_cast<int>(splits), cols, dweight, dbias);
     return launch_status("layer norm backward");
   }
   const int grid = static_cast<int>(std::min<int64_t>(rows, 8 * sm_count()));
