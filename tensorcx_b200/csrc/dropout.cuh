@@ -48,33 +48,40 @@ __device__ __forceinline__ uint32_t word_of(uint4 w, uint32_t i) {
   return i & 2u ? hi : lo;
 }
 
-// The words of places e .. e + 3: one block when e starts one, else two.
-__device__ __forceinline__ uint4 words_at(uint64_t e, const philox::RoundKeys& rk) {
-  const uint4 a = philox::block_words(e >> 2, rk);
-  const uint32_t r = static_cast<uint32_t>(e & 3);
-  if (r == 0) return a;
-  const uint4 b = philox::block_words((e >> 2) + 1, rk);
-  return r == 1 ? make_uint4(a.y, a.z, a.w, b.x) : r == 2 ? make_uint4(a.z, a.w, b.x, b.y) : make_uint4(a.w, b.x, b.y, b.z);
-}
-
 __device__ __forceinline__ bool kept(uint32_t word, uint32_t threshold) { return (word >> 8) >= threshold; }
 
 __device__ __forceinline__ float dropped(float x, bool keep, float scale) {
   return keep ? __fmul_rn(x, scale) : 0.0f;
 }
 
-// Bit j: place e + j is kept.
-__device__ __forceinline__ uint32_t kept4(uint64_t e, const philox::RoundKeys& rk, uint32_t threshold) {
-  const uint4 w = words_at(e, rk);
+// Bit j: word j of the block is kept.
+__device__ __forceinline__ uint32_t kept_block(uint64_t block, const philox::RoundKeys& rk, uint32_t threshold) {
+  const uint4 w = philox::block_words(block, rk);
   return (kept(w.x, threshold) ? 1u : 0u) | (kept(w.y, threshold) ? 2u : 0u) | (kept(w.z, threshold) ? 4u : 0u) |
          (kept(w.w, threshold) ? 8u : 0u);
 }
 
-__device__ __forceinline__ float4 dropped4(float4 x, uint64_t e, const philox::RoundKeys& rk, uint32_t threshold,
-                                           float scale) {
-  const uint4 w = words_at(e, rk);
-  return make_float4(dropped(x.x, kept(w.x, threshold), scale), dropped(x.y, kept(w.y, threshold), scale),
-                     dropped(x.z, kept(w.z, threshold), scale), dropped(x.w, kept(w.w, threshold), scale));
+// Bit 4 k + j: place e + 4 k STRIDE + j is kept, k < WORDS (at most 8). For whole warps whose
+// lanes' places lie 4 apart. Where they do not start a block, a lane's words end in the next
+// lane's blocks, and the last lane's in WORDS blocks of which each lane makes one.
+template <int WORDS, int STRIDE>
+__device__ __forceinline__ uint32_t kept_words(uint64_t e, const philox::RoundKeys& rk, uint32_t threshold) {
+  static_assert(WORDS <= 8, "the mask's bits");
+  const uint64_t block = e >> 2;
+  const int r = static_cast<int>(e & 3);  // the same for all lanes
+  uint32_t mask = 0;
+#pragma unroll
+  for (int k = 0; k < WORDS; ++k) mask |= kept_block(block + static_cast<uint64_t>(k) * STRIDE, rk, threshold) << (4 * k);
+  if (r == 0) return mask;
+  const int lane = threadIdx.x & 31;
+  uint32_t next = __shfl_down_sync(0xffffffffu, mask, 1), ends = 0;
+  const uint64_t after = __shfl_sync(0xffffffffu, block, 31) + 1;
+  if (lane < WORDS) ends = kept_block(after + static_cast<uint64_t>(lane) * STRIDE, rk, threshold) << (4 * lane);
+  ends = __reduce_or_sync(0xffffffffu, ends);
+  if (lane == 31) next = ends;
+  // bits r .. 3 of each word's own block, then bits 0 .. r - 1 of the next one
+  const uint32_t low = 0x11111111u * (0xfu >> r);
+  return ((mask >> r) & low) | ((next << (4 - r)) & ~low);
 }
 
 }  // namespace tcx

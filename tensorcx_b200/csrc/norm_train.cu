@@ -258,12 +258,12 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
     if (FUSED) {
       if (a.drop.threshold) {
         // the mask while the loads are on their way: 4 bits to a word
-        static_assert(!FUSED || VPT <= 16, "the mask's bits");
         const uint64_t start = dropout_start(a.drop) + static_cast<uint64_t>(words.at);
-        uint32_t mask[(VPT + 7) / 8] = {};
+        uint32_t mask[(VPT + 7) / 8];
 #pragma unroll
-        for (int k = 0; k < VPT; ++k)
-          mask[k / 8] |= kept4(start + 4 * static_cast<uint64_t>(tid + k * THREADS), rk, a.drop.threshold) << (4 * (k % 8));
+        for (int k = 0; k < VPT; k += 8)
+          mask[k / 8] = kept_words<(VPT < 8 ? VPT : 8), THREADS>(start + 4 * static_cast<uint64_t>(tid + k * THREADS), rk,
+                                                                a.drop.threshold);
 #pragma unroll
         for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -474,13 +474,9 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     copy(place, row + kRing * step);
     place = place + 1 == kRing ? 0 : place + 1;
     uint32_t mask = 0;
-    if (FUSED && a.dx) {
-#pragma unroll
-      for (int k = 0; k < VPT; ++k)
-        mask |= kept4(from + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(first_word + k * TPR), rk,
-                      a.drop.threshold)
-                << (4 * k);
-    }
+    if (FUSED && a.dx)
+      mask = kept_words<VPT, TPR>(from + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(first_word), rk,
+                                  a.drop.threshold);
     // both sums in one butterfly: the lower lanes take s1, the upper ones s2
     const bool upper = lane & 16;
     float s = (upper ? s2 : s1) + __shfl_xor_sync(0xffffffffu, upper ? s1 : s2, 16);

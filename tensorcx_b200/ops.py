@@ -691,25 +691,58 @@ def rand_uniform(shape, low: float = 0.0, high: float = 1.0, device="cuda", seed
 # Operators that a model learns with (no counterpart in the reference, an inference
 # runtime). Backward passes are functions of their own: the caller keeps what the forward
 # pass returned and hands it over.
-def _check_floats(shape, device, **tensors) -> None:
-    """Each tensor that is not None: a contiguous float32 CUDA tensor of `shape`."""
-    for name, t in tensors.items():
+#
+# A call of these on a small tensor takes less time on the GPU than Python's checks would, so
+# they test what has to hold in one expression per tensor and leave the words to _refuse.
+_Tensor, _float32 = torch.Tensor, torch.float32
+_new_like = torch.empty_like
+
+
+def _refuse(name: str, t, shape, index: int) -> None:
+    """Raises the reason why t is not a contiguous float32 tensor of `shape` on the current
+    device, `index`."""
+    _check_tensor(t, name)
+    if t.dtype != torch.float32:
+        raise ValueError(f"{name} must be a float32 tensor")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    raise ValueError(f"device mismatch: {name} is on {t.device}, not cuda:{index}")
+
+
+def _floats(index: int, shape, *named) -> None:
+    """named: name, tensor, name, tensor ...; None stands for an absent one."""
+    for i in range(1, len(named), 2):
+        t = named[i]
         if t is None:
             continue
-        _check_tensor(t, name)
-        if t.dtype != torch.float32:
-            raise ValueError(f"{name} must be a float32 tensor")
-        if t.shape != shape:
-            raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-        if t.device != device:
-            raise ValueError(f"device mismatch: {name} is on {t.device}, not {device}")
+        if not (isinstance(t, _Tensor) and t.dtype is _float32 and t.get_device() == index and t.is_contiguous()
+                and t.shape == shape):
+            _refuse(named[i - 1], t, shape, index)
 
 
-def _dropout_stream(p, seed, offset, device):
-    """(p, seed, offset, pointer of a device-side offset) as the C ABI takes them."""
-    if isinstance(p, (bool, np.bool_)) or not isinstance(p, (int, float, np.integer, np.floating)):
-        raise TypeError("dropout probability must be a real number")
-    p = float(p)
+def _leading(name: str, t) -> int:
+    """The current device; t, which the other arguments are held to, is a float32 tensor on it."""
+    index = torch.cuda.current_device()
+    if not (isinstance(t, _Tensor) and t.dtype is _float32 and t.get_device() == index and t.is_contiguous()):
+        _refuse(name, t, None, index)
+    return index
+
+
+def _raw(index: int) -> int:
+    """torch's current stream on device `index`, as the C ABI's integer handle."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _at(t) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _dropout_stream(p, seed, offset, index):
+    """(p, seed, offset, address of a device-side offset) as the C ABI takes them."""
+    if type(p) is not float:
+        if isinstance(p, (bool, np.bool_)) or not isinstance(p, (int, float, np.integer, np.floating)):
+            raise TypeError("dropout probability must be a real number")
+        p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError("dropout probability must be in [0, 1]")
     if p == 0.0:
@@ -718,9 +751,9 @@ def _dropout_stream(p, seed, offset, device):
         raise ValueError("dropout needs a seed: the backward pass makes the same mask from it")
     seed = _seed_of(seed)
     if isinstance(offset, torch.Tensor):
-        if offset.dtype != torch.int64 or offset.numel() != 1 or not offset.is_cuda or offset.device != device:
-            raise ValueError(f"a tensor offset must hold one int64 on {device}")
-        return p, seed, 0, _ptr(offset)
+        if offset.dtype != torch.int64 or offset.numel() != 1 or offset.get_device() != index:
+            raise ValueError(f"a tensor offset must hold one int64 on cuda:{index}")
+        return p, seed, 0, offset.data_ptr()
     if isinstance(offset, (bool, np.bool_)) or not isinstance(offset, (int, np.integer)) or not 0 <= offset < 2**64:
         raise ValueError("offset must be an integer in [0, 2**64), or an int64 tensor")
     return p, seed, int(offset), None
@@ -733,10 +766,13 @@ def dropout(x: torch.Tensor, p: float, seed: int, *, offset=0, residual: torch.T
     stored: dropout_backward makes it again from the same seed and offset. `offset` is an
     integer, or a CUDA int64 tensor of one element that is read when the kernel runs
     (advance it between the replays of a captured graph)."""
-    _check_floats(getattr(x, "shape", None), getattr(x, "device", None), x=x, residual=residual)
-    p, seed, offset, step = _dropout_stream(p, seed, offset, x.device)
-    out = torch.empty_like(x)
-    check(lib().tcx_sm100_dropout(_stream(), _ptr(x), _ptr(residual), _ptr(out), x.numel(), p, seed, offset, step))
+    index = _leading("x", x)
+    if residual is not None:
+        _floats(index, x.shape, "residual", residual)
+    p, seed, offset, step = _dropout_stream(p, seed, offset, index)
+    out = _new_like(x)
+    check(lib().tcx_sm100_dropout(_raw(index), x.data_ptr(), _at(residual), out.data_ptr(), x.numel(), p, seed, offset,
+                                  step))
     return out
 
 
@@ -752,21 +788,23 @@ def layernorm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias:
     it: total = residual + dropout(x), y = (total - mean) * rstd * weight + bias. Returns
     (y, total, mean, rstd); mean and rstd have x's shape without its last axis, and total
     is x itself without a residual and with p = 0. p, seed and offset as for dropout."""
-    _check_tensor(x, "x")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    index = _leading("x", x)
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("layernorm_forward requires a non-empty last axis")
-    _check_floats(x.shape, x.device, x=x, residual=residual)
-    cols = x.shape[-1]
-    _check_floats((cols,), x.device, weight=weight, bias=bias)
+    cols = shape[-1]
+    if residual is not None:
+        _floats(index, shape, "residual", residual)
+    _floats(index, (cols,), "weight", weight, "bias", bias)
     e = plan.epsilon(eps)
-    p, seed, offset, step = _dropout_stream(p, seed, offset, x.device)
-    y = torch.empty_like(x)
-    total = torch.empty_like(x) if residual is not None or p > 0.0 else None
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    p, seed, offset, step = _dropout_stream(p, seed, offset, index)
+    y = _new_like(x)
+    total = _new_like(x) if residual is not None or p > 0.0 else None
+    mean = x.new_empty(shape[:-1])
+    rstd = _new_like(mean)
     check(lib().tcx_sm100_layernorm_forward(
-        _stream(), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y), _ptr(total), _ptr(mean), _ptr(rstd),
-        x.numel() // cols, cols, e, p, seed, offset, step))
+        _raw(index), x.data_ptr(), _at(residual), _at(weight), _at(bias), y.data_ptr(), _at(total), mean.data_ptr(),
+        rstd.data_ptr(), x.numel() // cols, cols, e, p, seed, offset, step))
     return y, x if total is None else total, mean, rstd
 
 
@@ -777,45 +815,56 @@ def layernorm_backward(dy: torch.Tensor, total: torch.Tensor, mean: torch.Tensor
     dbias). dresidual is the gradient of total (dtotal, what reaches total by other ways,
     added), and dx the same through the dropout: with p = 0 both are one tensor. Without a
     weight dweight and dbias are None. Sums over rows have a fixed order."""
-    _check_tensor(total, "total")
-    if total.dim() == 0 or total.shape[-1] == 0:
+    index = _leading("total", total)
+    shape = total.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("layernorm_backward requires a non-empty last axis")
-    _check_floats(total.shape, total.device, total=total, dy=dy, dtotal=dtotal)
-    cols = total.shape[-1]
-    _check_floats(total.shape[:-1], total.device, mean=mean, rstd=rstd)
-    _check_floats((cols,), total.device, weight=weight)
-    p, seed, offset, step = _dropout_stream(p, seed, offset, total.device)
+    cols = shape[-1]
+    if dy is None or mean is None or rstd is None:
+        raise TypeError("layernorm_backward needs dy, mean and rstd")
+    _floats(index, shape, "dy", dy, "dtotal", dtotal)
+    _floats(index, shape[:-1], "mean", mean, "rstd", rstd)
+    p, seed, offset, step = _dropout_stream(p, seed, offset, index)
     rows = total.numel() // cols
-    dresidual = torch.empty_like(total)
-    dx = torch.empty_like(total) if p > 0.0 else None
+    dresidual = _new_like(total)
+    dx = _new_like(total) if p > 0.0 else None
     dweight = dbias = keep = ws = None
     ws_bytes = 0
     if weight is not None:
-        dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
+        _floats(index, (cols,), "weight", weight)
+        dweight, dbias = _new_like(weight), _new_like(weight)
         ws_bytes = lib().tcx_sm100_layernorm_backward_workspace_bytes(rows, cols)
         keep, ws = _workspace(ws_bytes, total.device)
     check(lib().tcx_sm100_layernorm_backward(
-        _stream(), _ptr(dy), _ptr(total), _ptr(mean), _ptr(rstd), _ptr(weight), _ptr(dtotal), _ptr(dresidual),
-        _ptr(dx), _ptr(dweight), _ptr(dbias), rows, cols, p, seed, offset, step, ws, ws_bytes))
+        _raw(index), dy.data_ptr(), total.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _at(weight), _at(dtotal),
+        dresidual.data_ptr(), _at(dx), _at(dweight), _at(dbias), rows, cols, p, seed, offset, step, ws, ws_bytes))
     del keep
     return dresidual if dx is None else dx, dresidual, dweight, dbias
 
 
-def _recurrence_args(gate, form, lengths, **tensors):
-    if form not in RECURRENCE:
+def _recurrence_args(gate, form, lengths, *named):
+    """(device, form, shape, lengths' address) of a recurrence over tensors like gate."""
+    kind = RECURRENCE.get(form) if isinstance(form, str) else None
+    if kind is None:
         raise ValueError(f"recurrence form must be one of {sorted(RECURRENCE)}")
-    _check_tensor(gate, "gate")
-    if gate.dim() != 3:
+    index = _leading("gate", gate)
+    shape = gate.shape
+    if len(shape) != 3:
         raise ValueError("a recurrence runs over [batch, time, channels]")
-    _check_floats(gate.shape, gate.device, gate=gate, **tensors)
-    batch, time, channels = gate.shape
-    if lengths is not None:
-        _check_tensor(lengths, "lengths")
-        if lengths.dtype != torch.int32 or lengths.shape != (batch,) or lengths.device != gate.device:
-            raise ValueError(f"lengths must be an int32 tensor of shape ({batch},) on {gate.device}")
-    ws_bytes = lib().tcx_sm100_recurrence_workspace_bytes(batch, time, channels)
-    keep, ws = _workspace(ws_bytes, gate.device)
-    return batch, time, channels, keep, ws, ws_bytes
+    _floats(index, shape, *named)
+    if lengths is None:
+        return index, kind, shape, None
+    _check_tensor(lengths, "lengths")
+    if lengths.dtype != torch.int32 or lengths.shape != shape[:1]:
+        raise ValueError(f"lengths must be an int32 tensor of shape ({shape[0]},)")
+    return index, kind, shape, lengths.data_ptr()
+
+
+def _recurrence_workspace(shape, device):
+    ws_bytes = 0
+    if shape[1] > 1:  # a single step needs none
+        ws_bytes = lib().tcx_sm100_recurrence_workspace_bytes(*shape)
+    return *_workspace(ws_bytes, device), ws_bytes
 
 
 def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, initial: torch.Tensor | None = None, *,
@@ -829,14 +878,16 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, initial: torch.Tensor 
     running sequence) state is a view of h."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a tensor")
-    batch, time, channels, keep, ws, ws_bytes = _recurrence_args(gate, form, lengths, x=x)
-    _check_floats((batch, channels), gate.device, initial=initial)
-    h = torch.empty_like(gate)
-    state = h.view(batch, channels) if time == 1 else torch.empty((batch, channels), dtype=torch.float32,
-                                                                  device=gate.device)
+    index, kind, shape, ends = _recurrence_args(gate, form, lengths, "x", x)
+    batch, time, channels = shape
+    if initial is not None:
+        _floats(index, (batch, channels), "initial", initial)
+    h = _new_like(gate)
+    state = h.view(batch, channels) if time == 1 else gate.new_empty((batch, channels))
+    keep, ws, ws_bytes = _recurrence_workspace(shape, gate.device)
     check(lib().tcx_sm100_recurrence_forward(
-        _stream(), RECURRENCE[form], _ptr(gate), _ptr(x), _ptr(initial), _ptr(lengths), _ptr(h),
-        None if time == 1 else _ptr(state), batch, time, channels, ws, ws_bytes))
+        _raw(index), kind, gate.data_ptr(), x.data_ptr(), _at(initial), ends, h.data_ptr(),
+        None if time == 1 else state.data_ptr(), batch, time, channels, ws, ws_bytes))
     del keep
     return h, state
 
@@ -852,12 +903,14 @@ def gated_recurrence_backward(dh: torch.Tensor, gate: torch.Tensor, x: torch.Ten
             raise TypeError(f"{name} must be a tensor")
     if form == "sigmoid" and x is None:
         raise ValueError("the sigmoid form's gradient needs x")
-    batch, time, channels, keep, ws, ws_bytes = _recurrence_args(gate, form, lengths, dh=dh, x=x, h=h)
-    _check_floats((batch, channels), gate.device, initial=initial, dstate=dstate)
-    dgate, dx = torch.empty_like(gate), torch.empty_like(gate)
-    dinitial = None if initial is None else torch.empty_like(initial)
+    index, kind, shape, ends = _recurrence_args(gate, form, lengths, "dh", dh, "x", x, "h", h)
+    batch, time, channels = shape
+    _floats(index, (batch, channels), "initial", initial, "dstate", dstate)
+    dgate, dx = _new_like(gate), _new_like(gate)
+    dinitial = None if initial is None else _new_like(initial)
+    keep, ws, ws_bytes = _recurrence_workspace(shape, gate.device)
     check(lib().tcx_sm100_recurrence_backward(
-        _stream(), RECURRENCE[form], _ptr(dh), _ptr(gate), _ptr(x), _ptr(h), _ptr(initial), _ptr(lengths),
-        _ptr(dstate), _ptr(dgate), _ptr(dx), _ptr(dinitial), batch, time, channels, ws, ws_bytes))
+        _raw(index), kind, dh.data_ptr(), gate.data_ptr(), _at(x), h.data_ptr(), _at(initial), ends, _at(dstate),
+        dgate.data_ptr(), dx.data_ptr(), _at(dinitial), batch, time, channels, ws, ws_bytes))
     del keep
     return dgate, dx, dinitial
