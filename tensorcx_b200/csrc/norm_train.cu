@@ -212,7 +212,15 @@ struct Words {
   __device__ __forceinline__ float4 column(const float* p, int word) const {
     if (!ODD) return __ldg(reinterpret_cast<const float4*>(p) + word);
     const float* const q = p + 4 * word - phase;
-    if (whole(word)) return make_float4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+    if (whole(word) && 4 * word + 4 <= cols && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      // the columns lie in the vector's own words `word - 1` and `word`
+      const float4 b = __ldg(reinterpret_cast<const float4*>(p) + word);
+      if (phase == 0) return b;
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p) + word - 1);
+      return phase == 1   ? make_float4(a.w, b.x, b.y, b.z)
+             : phase == 2 ? make_float4(a.z, a.w, b.x, b.y)
+                          : make_float4(a.y, a.z, a.w, b.x);
+    }
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (valid(word, 0)) v.x = __ldg(q);
     if (valid(word, 1)) v.y = __ldg(q + 1);
@@ -222,13 +230,44 @@ struct Words {
   }
 };
 
-// One block to a row, VPT words to a thread. Each element is read once and written once; the
-// statistics take two block reductions.
-template <int THREADS, int VPT, bool ODD, bool FUSED>
-__global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
-  __shared__ float smem[64];
-  using B = Block<THREADS>;
-  const int tid = threadIdx.x;
+// Two sums over a warp in one butterfly: the lower lanes end with a's, the upper ones with b's.
+__device__ __forceinline__ float warp_sums(float a, float b) {
+  const bool upper = threadIdx.x & 16;
+  float s = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  return s;
+}
+
+// Two sums over `warps` warps that share `smem` and the barrier; every thread receives them.
+__device__ __forceinline__ float2 row_sums(float a, float b, float2* smem, int warps, int warp, int barrier) {
+  const float s = warp_sums(a, b);
+  const int lane = threadIdx.x & 31;
+  if (warps == 1) return make_float2(__shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, s, 16));
+  if ((lane & 15) == 0) (lane ? smem[warp].y : smem[warp].x) = s;
+  asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory");
+  float2 sums = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+  for (int w = 0; w < warps; ++w) {
+    const float2 v = smem[w];
+    sums.x += v.x;
+    sums.y += v.y;
+  }
+  return sums;
+}
+
+// Kernels for a known number of warps to a row (WARPS), or any up to kMostWarps (0).
+constexpr int kMostWarps = 16;
+constexpr int most_threads(int warps) { return 32 * (warps ? warps : kMostWarps); }
+
+// One block to a row, VPT words to a thread, as many warps as the row needs. Each element is
+// read once and written once; the statistics take two block reductions.
+template <int VPT, int WARPS, bool ODD, bool FUSED>
+__global__ void __launch_bounds__(most_threads(WARPS), (FUSED ? 512 : 768) / most_threads(WARPS))
+norm_forward_kernel(ForwardArgs a) {
+  __shared__ float2 smem[2][kMostWarps];
+  const int warps = WARPS ? WARPS : blockDim.x >> 5, warp = threadIdx.x >> 5;
+  const int mine = warp * 32 * VPT + (threadIdx.x & 31);  // its first word, of a warp's 32 VPT
   const float n = static_cast<float>(a.cols);
   const philox::RoundKeys rk = philox::round_keys(a.drop.key);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -245,7 +284,7 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
     float4 res[FUSED ? VPT : 1];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = tid + k * THREADS;
+      const int word = mine + 32 * k;
       float4 t = make_float4(level, level, level, level);
       if (words.holds(word)) t = words.load(a.x, word);
       v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
@@ -253,7 +292,7 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
     if (FUSED && a.residual) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (words.holds(tid + k * THREADS)) res[FUSED ? k : 0] = words.load(a.residual, tid + k * THREADS);
+        if (words.holds(mine + 32 * k)) res[FUSED ? k : 0] = words.load(a.residual, mine + 32 * k);
     }
     if (FUSED) {
       if (a.drop.threshold) {
@@ -262,8 +301,8 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
         uint32_t mask[(VPT + 7) / 8];
 #pragma unroll
         for (int k = 0; k < VPT; k += 8)
-          mask[k / 8] = kept_words<(VPT < 8 ? VPT : 8), THREADS>(start + 4 * static_cast<uint64_t>(tid + k * THREADS), rk,
-                                                                a.drop.threshold);
+          mask[k / 8] = kept_words<(VPT < 8 ? VPT : 8)>(start + 4 * static_cast<uint64_t>(mine + 32 * k), 32,
+                                                        rk, a.drop.threshold);
 #pragma unroll
         for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -271,7 +310,7 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
       }
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
-        const int word = tid + k * THREADS;
+        const int word = mine + 32 * k;
         if (words.holds(word)) {
           if (a.residual) {
             const float4 r = res[FUSED ? k : 0];
@@ -287,7 +326,7 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
     float s = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = tid + k * THREADS;
+      const int word = mine + 32 * k;
       if (!words.whole(word)) {  // nothing for what is outside the row
         const float4 t = words.within(word, make_float4(v[k][0], v[k][1], v[k][2], v[k][3]), level);
         v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
@@ -295,11 +334,11 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) s += v[k][j] - level;
     }
-    const float m1 = level + __fdiv_rn(B::sum(s, smem), n);
+    const float m1 = level + __fdiv_rn(row_sums(s, 0.0f, smem[0], warps, warp, 0).x, n);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = tid + k * THREADS;
+      const int word = mine + 32 * k;
       if (words.holds(word)) {
         float d[4];
 #pragma unroll
@@ -315,14 +354,14 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
         }
       }
     }
-    const float2 r = B::sum2(s1, s2, smem);
+    const float2 r = row_sums(s1, s2, smem[1], warps, warp, 0);
     const float shift = __fdiv_rn(r.x, n);
     float var = __fdiv_rn(r.y, n) - shift * shift;
     if (var < 0.0f) var = 0.0f;  // rounding; a NaN stays one
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(var + a.eps));
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = tid + k * THREADS;
+      const int word = mine + 32 * k;
       if (words.holds(word)) {
         float4 y = make_float4((v[k][0] - shift) * rstd, (v[k][1] - shift) * rstd, (v[k][2] - shift) * rstd,
                                (v[k][3] - shift) * rstd);
@@ -337,45 +376,49 @@ __global__ void __launch_bounds__(THREADS) norm_forward_kernel(ForwardArgs a) {
         words.store(a.y, word, y);
       }
     }
-    if (tid == 0) {
+    if (threadIdx.x == 0) {
       a.mean[row] = m1 + shift;
       a.rstd[row] = rstd;
     }
   }
 }
 
-// TPR threads (of CLUSTER blocks) to a row, VPT words to each, GROUPS rows to a block at a
-// time. A group's rows are a multiple of 4 apart, so that they all start in the same phase
-// and a thread's columns are the same in each: the weight's and the bias's gradients add up in
-// its registers over the group's rows, the groups' in shared memory, and the blocks' in a
-// second kernel, each in a fixed order.
+// Some warps of a block (of each of CLUSTER blocks) to a row, VPT words to a thread, and several
+// rows to a block at a time where they are short, a group of warps to each. A group's rows are a multiple of 4 apart, so that they
+// all start in the same phase and a thread's columns are the same in each: the weight's and the
+// bias's gradients add up in its registers over the group's rows, the groups' in shared memory,
+// and the blocks' in a second kernel, each in a fixed order.
 //
 // dy and total come through a ring of places in shared memory (cp.async; a thread copies and
 // reads its own words only, so that needs no barrier): a place is copied into again as soon as
 // its row is in registers, while that row's sums cross the block.
-template <int TPR, int GROUPS, int VPT>
-struct BackwardShape {
-  static constexpr int kThreads = TPR * GROUPS;
-  static constexpr int kPerSm = 512 / kThreads, kRing = 3;
-  static constexpr int kPlaces = kRing * 2 * VPT * kThreads * 16, kColumns = GROUPS > 1 ? 2 * 4 * TPR * VPT * 4 : 0;
-  static constexpr int kBytes = kPlaces > kColumns ? kPlaces : kColumns;
-};
+constexpr int kRing = 3, kWarpsPerSm = 16;  // 128 registers a thread
 
-template <int TPR, int GROUPS, int VPT, int CLUSTER, bool ODD, bool FUSED>
-__global__ void __launch_bounds__(TPR* GROUPS, BackwardShape<TPR, GROUPS, VPT>::kPerSm)
+template <int VPT>
+constexpr int backward_bytes(int threads, bool multi) {
+  const int ring = kRing * 2 * VPT * threads * 16, columns = multi ? 2 * 4 * 128 * VPT * 4 : 0;
+  return ring > columns ? ring : columns;
+}
+
+// WARPS: warps of a row, with 8 / WARPS rows to a block (GROUPS); 0: any number, one row to a block.
+template <int VPT, int WARPS, int CLUSTER, bool ODD, bool FUSED>
+__global__ void __launch_bounds__(WARPS ? 256 : 512, WARPS ? 2 : 1)
 norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
-  constexpr int kThreadsAll = TPR * GROUPS, kWarps = TPR / 32, kSpan = TPR * VPT;  // words of a block's part of a row
-  constexpr int kRing = BackwardShape<TPR, GROUPS, VPT>::kRing;
-  static_assert(CLUSTER == 1 || GROUPS == 1, "");
+  static_assert(CLUSTER == 1 || WARPS == 0, "");
+  constexpr bool MULTI = WARPS != 0;
+  const int warps = MULTI ? WARPS : blockDim.x >> 5;
   extern __shared__ __align__(16) float4 stage[];
-  __shared__ float sums[2][GROUPS][2][kWarps];
+  __shared__ float2 sums[2][kMostWarps];
   __shared__ float2 peers[2][CLUSTER];
   __shared__ __align__(8) uint64_t arrived[2];
-  const int tid = threadIdx.x % TPR, group = threadIdx.x / TPR, lane = tid & 31, warp = tid >> 5;
+  const int tpr = warps * 32, kSpan = tpr * VPT;  // words of a block's part of a row
+  constexpr int groups = MULTI ? 8 / (MULTI ? WARPS : 1) : 1;
+  const int group = MULTI ? threadIdx.x / (32 * (MULTI ? WARPS : 1)) : 0;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - group * warps;
   const int rank = CLUSTER > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
-  const int first_word = rank * kSpan + tid;
-  const int64_t step = static_cast<int64_t>(gridDim.x / CLUSTER) * GROUPS;
-  const int64_t opening = static_cast<int64_t>(blockIdx.x / CLUSTER) * GROUPS + group;
+  const int first_word = rank * kSpan + warp * 32 * VPT + lane;  // a warp's words are side by side
+  const int64_t step = static_cast<int64_t>(gridDim.x / CLUSTER) * groups;
+  const int64_t opening = static_cast<int64_t>(blockIdx.x / CLUSTER) * groups + group;
   const float share = 1.0f / static_cast<float>(a.cols);
   if (CLUSTER > 1) {
     if (threadIdx.x == 0) {
@@ -394,24 +437,25 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   for (int k = 0; k < VPT; ++k) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[k][j] = db[k][j] = 0.0f;
-    if (ODD) weight[ODD ? k : 0] = a.weight ? columns_of.column(a.weight, first_word + k * TPR) : make_float4(1, 1, 1, 1);
+    if (ODD) weight[ODD ? k : 0] = a.weight ? columns_of.column(a.weight, first_word + 32 * k) : make_float4(1, 1, 1, 1);
   }
 
+  float4* const mine = stage + (threadIdx.x >> 5) * (kRing * 2 * VPT * 32) + lane;  // this thread's first place
   // Copies a row into a place: word k of dy and of total.
   auto copy = [&](int place, int64_t row) {
     if (row < a.rows) {
       const Words<ODD> words(row, a.cols, a.rows);
-      float4* const to = stage + place * (2 * VPT * kThreadsAll) + threadIdx.x;
+        float4* const to = mine + place * (2 * VPT * 32);
       const int64_t at = words.at + 4 * static_cast<int64_t>(first_word);
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
-        if (words.holds(first_word + k * TPR)) {
-          const int64_t i = at + 4 * k * TPR;
+        if (words.holds(first_word + 32 * k)) {
+          const int64_t i = at + 128 * k;
           const int bytes = !ODD || i + 4 <= words.count ? 16 : 4 * static_cast<int>(words.count - i);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + k * kThreadsAll)),
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + 32 * k)),
                        "l"(a.dy + i), "r"(bytes)
                        : "memory");
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + (VPT + k) * kThreadsAll)),
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + 32 * (VPT + k))),
                        "l"(a.total + i), "r"(bytes)
                        : "memory");
         }
@@ -439,21 +483,21 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     if (FUSED && a.dtotal) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (words.holds(first_word + k * TPR)) extra[FUSED ? k : 0] = words.load(a.dtotal, first_word + k * TPR);
+        if (words.holds(first_word + 32 * k)) extra[FUSED ? k : 0] = words.load(a.dtotal, first_word + 32 * k);
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-    const float4* const here = stage + place * (2 * VPT * kThreadsAll) + threadIdx.x;
+    const float4* const here = mine + place * (2 * VPT * 32);
     float g[VPT][4], hat[VPT][4];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = first_word + k * TPR;
+      const int word = first_word + 32 * k;
       const bool in = words.holds(word);
       float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), t = make_float4(mean, mean, mean, mean);
       float4 w = ODD ? weight[ODD ? k : 0] : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
       if (in) {
-        y = here[k * kThreadsAll];
-        t = here[(VPT + k) * kThreadsAll];
+        y = here[32 * k];
+        t = here[32 * (VPT + k)];
         if (!ODD && a.weight) w = words.column(a.weight, word);
         if (!words.whole(word)) {
           y = words.within(word, y, 0.0f);
@@ -475,26 +519,10 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     place = place + 1 == kRing ? 0 : place + 1;
     uint32_t mask = 0;
     if (FUSED && a.dx)
-      mask = kept_words<VPT, TPR>(from + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(first_word), rk,
-                                  a.drop.threshold);
-    // both sums in one butterfly: the lower lanes take s1, the upper ones s2
-    const bool upper = lane & 16;
-    float s = (upper ? s2 : s1) + __shfl_xor_sync(0xffffffffu, upper ? s1 : s2, 16);
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (kWarps > 1) {
-      if ((lane & 15) == 0) sums[turn & 1][group][lane >> 4][warp] = s;
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(TPR) : "memory");
-      s1 = s2 = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        s1 += sums[turn & 1][group][0][w];
-        s2 += sums[turn & 1][group][1][w];
-      }
-    } else {
-      s1 = __shfl_sync(0xffffffffu, s, 0);
-      s2 = __shfl_sync(0xffffffffu, s, 16);
-    }
+      mask = kept_words<VPT>(from + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(first_word), 32, rk,
+                             a.drop.threshold);
+    const float2 sums_all = row_sums(s1, s2, sums[turn & 1] + group * warps, warps, warp, 1 + group);
+    s1 = sums_all.x, s2 = sums_all.y;
     if (CLUSTER > 1) {
       // This block's sums go to every block of the cluster, its own too. A peer that sends
       // those of the row after next has this block's of the next row, which are sent when all
@@ -520,7 +548,7 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     const float c1 = -rstd * (s1 * share), c2 = -rstd * (s2 * share);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = first_word + k * TPR;
+      const int word = first_word + 32 * k;
       if (!words.holds(word)) continue;
       float d[4];
 #pragma unroll
@@ -544,12 +572,12 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
 
   const int64_t at = static_cast<int64_t>(blockIdx.x / CLUSTER) * 2 * a.cols;
   const Words<ODD>& words = columns_of;  // a group without rows adds zeros
-  if (GROUPS == 1) {
+  if (!MULTI) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int c = 4 * (first_word + k * TPR) + j - words.phase;
+        const int c = 4 * (first_word + 32 * k) + j - words.phase;
         if (c >= 0 && c < words.cols) {
           partial[at + c] = dw[k][j];
           partial[at + a.cols + c] = db[k][j];
@@ -560,15 +588,15 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     float* const columns = reinterpret_cast<float*>(stage);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * 4 * kSpan; i += kThreadsAll) columns[i] = 0.0f;
-    for (int whose = 0; whose < GROUPS; ++whose) {
+    for (int i = threadIdx.x; i < 2 * 4 * kSpan; i += blockDim.x) columns[i] = 0.0f;
+    for (int whose = 0; whose < groups; ++whose) {
       __syncthreads();
       if (group != whose) continue;
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int c = 4 * (first_word + k * TPR) + j - words.phase;
+          const int c = 4 * (first_word + 32 * k) + j - words.phase;
           if (c >= 0 && c < words.cols) {
             columns[c] += dw[k][j];
             columns[4 * kSpan + c] += db[k][j];
@@ -576,7 +604,7 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
         }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < static_cast<int>(a.cols); c += kThreadsAll) {
+    for (int c = threadIdx.x; c < static_cast<int>(a.cols); c += blockDim.x) {
       partial[at + c] = columns[c];
       partial[at + a.cols + c] = columns[4 * kSpan + c];
     }
@@ -620,36 +648,38 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 // Words that a row can touch.
 int64_t words_of(int64_t cols) { return cols % 4 ? (cols + 6) / 4 : cols / 4; }
 
-template <int THREADS, int VPT, bool FUSED>
-void launch_forward(cudaStream_t s, const ForwardArgs& a, bool odd) {
+template <int VPT, int WARPS, bool FUSED>
+void launch_forward(cudaStream_t s, const ForwardArgs& a, int warps, bool odd) {
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 30));
-  if (odd) norm_forward_kernel<THREADS, VPT, true, FUSED><<<grid, THREADS, 0, s>>>(a);
-  else norm_forward_kernel<THREADS, VPT, false, FUSED><<<grid, THREADS, 0, s>>>(a);
+  if (odd) norm_forward_kernel<VPT, WARPS, true, FUSED><<<grid, 32 * warps, 0, s>>>(a);
+  else norm_forward_kernel<VPT, WARPS, false, FUSED><<<grid, 32 * warps, 0, s>>>(a);
 }
 
-// Small blocks of many words: 64 values to a thread, or 32 of each of two inputs.
+template <int VPT, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
-  if (a.total) {
-    if (words <= 32) launch_forward<32, 1, true>(s, a, odd);
-    else if (words <= 64) launch_forward<32, 2, true>(s, a, odd);
-    else if (words <= 128) launch_forward<32, 4, true>(s, a, odd);
-    else if (words <= 256) launch_forward<32, 8, true>(s, a, odd);
-    else if (words <= 512) launch_forward<64, 8, true>(s, a, odd);
-    else if (words <= 1024) launch_forward<128, 8, true>(s, a, odd);
-    else if (words <= 2048) launch_forward<256, 8, true>(s, a, odd);
-    else if (words <= 4096) launch_forward<512, 8, true>(s, a, odd);
-    else launch_forward<512, 16, true>(s, a, odd);
+  const int warps = static_cast<int>(ceil_div(words, 32 * VPT));
+  if constexpr (VPT < 8) {
+    launch_forward<VPT, 1, FUSED>(s, a, 1, odd);
+  } else if constexpr (VPT == 16 && FUSED) {  // rows of 9 warps and more
+    launch_forward<VPT, 0, FUSED>(s, a, warps, odd);
   } else {
-    if (words <= 32) launch_forward<32, 1, false>(s, a, odd);
-    else if (words <= 64) launch_forward<32, 2, false>(s, a, odd);
-    else if (words <= 128) launch_forward<32, 4, false>(s, a, odd);
-    else if (words <= 256) launch_forward<32, 8, false>(s, a, odd);
-    else if (words <= 512) launch_forward<32, 16, false>(s, a, odd);
-    else if (words <= 1024) launch_forward<64, 16, false>(s, a, odd);
-    else if (words <= 2048) launch_forward<128, 16, false>(s, a, odd);
-    else if (words <= 4096) launch_forward<256, 16, false>(s, a, odd);
-    else launch_forward<512, 16, false>(s, a, odd);
+    if (warps == 1) launch_forward<VPT, 1, FUSED>(s, a, warps, odd);
+    else if (warps == 2) launch_forward<VPT, 2, FUSED>(s, a, warps, odd);
+    else if (warps == 4) launch_forward<VPT, 4, FUSED>(s, a, warps, odd);
+    else launch_forward<VPT, 0, FUSED>(s, a, warps, odd);
   }
+}
+
+// Small blocks of many words: up to 64 values to a thread, or 32 of each of two inputs. Rows
+// that leave more than an eighth of the places of 16 words to a thread empty take 8.
+template <bool FUSED>
+void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
+  const bool many = !FUSED && words * 8 >= ceil_div(words, 512) * 512 * 7;
+  if (words <= 32) launch_forward<1, FUSED>(s, a, words, odd);
+  else if (words <= 64) launch_forward<2, FUSED>(s, a, words, odd);
+  else if (words <= 128) launch_forward<4, FUSED>(s, a, words, odd);
+  else if (words <= 4096 && !many) launch_forward<8, FUSED>(s, a, words, odd);
+  else launch_forward<16, FUSED>(s, a, words, odd);
 }
 
 // Blocks (or clusters) that the backward kernel runs as: what the machine holds at a time, no
@@ -661,81 +691,82 @@ int64_t backward_blocks(int64_t rows, int64_t cols, int groups, int resident) {
 }
 
 struct BackwardPlan {
-  int tpr, vpt, cluster;  // threads of a block to a row, their words, blocks to a row; tpr 0: none
-  int64_t blocks;         // or clusters: partial rows, at most
+  int vpt, warps, cluster, groups;  // words of a thread; warps of a block to a row; vpt 0: no such kernel
+  int per_sm;                       // blocks that an SM's registers and shared memory hold
 };
 
-BackwardPlan backward_plan(int64_t rows, int64_t cols) {
+BackwardPlan backward_plan(int64_t cols) {
   const int64_t words = words_of(cols);
-  if (words > 8 * 2048) return {0, 0, 0, 0};
-  const int tpr = words <= 128 ? 32 : words <= 256 ? 64 : words <= 512 ? 128 : words <= 8192 ? 256 : 512;
-  const int vpt = words <= 32 ? 1 : words <= 64 ? 2 : 4;
-  const int cluster = words <= 1024 ? 1 : words <= 2048 ? 2 : words <= 4096 ? 4 : 8;
-  const int threads = tpr < 256 ? 256 : tpr, groups = threads / tpr;
-  return {tpr, vpt, cluster, backward_blocks(rows, cols, groups, 512 / threads * sm_count() / cluster)};
+  if (words > 8 * 128 * kMostWarps) return {0, 0, 0, 0, 0};
+  BackwardPlan plan;
+  plan.vpt = words <= 32 ? 1 : words <= 64 ? 2 : 4;
+  const int warps = static_cast<int>(ceil_div(words, 32 * plan.vpt));
+  plan.cluster = warps <= 8 ? 1 : warps <= 16 ? 2 : warps <= 32 ? 4 : 8;
+  plan.warps = static_cast<int>(ceil_div(warps, plan.cluster));
+  plan.groups = plan.warps == 1 || plan.warps == 2 || plan.warps == 4 ? 8 / plan.warps : 1;
+  plan.per_sm = std::max(1, kWarpsPerSm / (plan.warps * plan.groups));
+  return plan;
 }
 
-template <int TPR, int GROUPS, int VPT, int CLUSTER, bool ODD, bool FUSED>
-int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial) {
-  using Sh = BackwardShape<TPR, GROUPS, VPT>;
+template <int VPT, int WARPS, int CLUSTER, bool ODD, bool FUSED>
+int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan) {
+  auto* kernel = norm_backward_kernel<VPT, WARPS, CLUSTER, ODD, FUSED>;
+  const int threads = plan.warps * plan.groups * 32;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(TPR * GROUPS);
-  cfg.dynamicSmemBytes = Sh::kBytes;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = backward_bytes<VPT>(threads, WARPS != 0);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {CLUSTER, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = CLUSTER > 1 ? 1 : 0;
-  auto* kernel = norm_backward_kernel<TPR, GROUPS, VPT, CLUSTER, ODD, FUSED>;
-  // how many blocks or clusters the device holds at a time, looked up once per device
-  static int resident[64] = {0};
+  // how many blocks or clusters the device holds at a time, looked up once for each size
+  static int resident[64][kMostWarps + 1] = {};
   int dev = 0, held = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64) held = resident[dev];
+  if (dev >= 0 && dev < 64) held = resident[dev][plan.warps];
   if (held == 0) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kBytes);
-    held = Sh::kPerSm * sm_count() / CLUSTER;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         backward_bytes<VPT>(kMostWarps * 32, WARPS != 0));
+    held = plan.per_sm * sm_count() / CLUSTER;
     cfg.gridDim = dim3(static_cast<unsigned>(held * CLUSTER));
     int clusters = 0;
     if (CLUSTER > 1 && cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0)
       held = std::min(held, clusters);
-    if (dev >= 0 && dev < 64) resident[dev] = held;
+    if (dev >= 0 && dev < 64) resident[dev][plan.warps] = held;
   }
-  const int64_t blocks = backward_blocks(a.rows, a.cols, GROUPS, held);
+  const int64_t blocks = backward_blocks(a.rows, a.cols, plan.groups, held);
   cfg.gridDim = dim3(static_cast<unsigned>(blocks * CLUSTER));
   cudaLaunchKernelEx(&cfg, kernel, a, partial, device_error_word());
   return blocks;
 }
 
-template <int TPR, int GROUPS, int VPT, int CLUSTER>
-int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, bool odd) {
+template <int VPT, int WARPS, int CLUSTER>
+int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd) {
   const bool fused = a.dtotal || a.dx;
   if (odd)
-    return fused ? launch_backward<TPR, GROUPS, VPT, CLUSTER, true, true>(s, a, partial)
-                 : launch_backward<TPR, GROUPS, VPT, CLUSTER, true, false>(s, a, partial);
-  return fused ? launch_backward<TPR, GROUPS, VPT, CLUSTER, false, true>(s, a, partial)
-               : launch_backward<TPR, GROUPS, VPT, CLUSTER, false, false>(s, a, partial);
+    return fused ? launch_backward<VPT, WARPS, CLUSTER, true, true>(s, a, partial, plan)
+                 : launch_backward<VPT, WARPS, CLUSTER, true, false>(s, a, partial, plan);
+  return fused ? launch_backward<VPT, WARPS, CLUSTER, false, true>(s, a, partial, plan)
+               : launch_backward<VPT, WARPS, CLUSTER, false, false>(s, a, partial, plan);
 }
 
 // Returns the partial rows that it leaves.
 int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd) {
   switch (plan.cluster) {
-    case 2: return launch_backward<256, 1, 4, 2>(s, a, partial, odd);
-    case 4: return launch_backward<256, 1, 4, 4>(s, a, partial, odd);
-    case 8:
-      return plan.tpr == 256 ? launch_backward<256, 1, 4, 8>(s, a, partial, odd)
-                             : launch_backward<512, 1, 4, 8>(s, a, partial, odd);
+    case 2: return launch_backward<4, 0, 2>(s, a, partial, plan, odd);
+    case 4: return launch_backward<4, 0, 4>(s, a, partial, plan, odd);
+    case 8: return launch_backward<4, 0, 8>(s, a, partial, plan, odd);
     default: break;
   }
-  switch (plan.tpr) {
-    case 32:
-      return plan.vpt == 1   ? launch_backward<32, 8, 1, 1>(s, a, partial, odd)
-             : plan.vpt == 2 ? launch_backward<32, 8, 2, 1>(s, a, partial, odd)
-                             : launch_backward<32, 8, 4, 1>(s, a, partial, odd);
-    case 64: return launch_backward<64, 4, 4, 1>(s, a, partial, odd);
-    case 128: return launch_backward<128, 2, 4, 1>(s, a, partial, odd);
-    default: return launch_backward<256, 1, 4, 1>(s, a, partial, odd);
+  if (plan.vpt == 1) return launch_backward<1, 1, 1>(s, a, partial, plan, odd);
+  if (plan.vpt == 2) return launch_backward<2, 1, 1>(s, a, partial, plan, odd);
+  switch (plan.warps) {
+    case 1: return launch_backward<4, 1, 1>(s, a, partial, plan, odd);
+    case 2: return launch_backward<4, 2, 1>(s, a, partial, plan, odd);
+    case 4: return launch_backward<4, 4, 1>(s, a, partial, plan, odd);
+    default: return launch_backward<4, 0, 1>(s, a, partial, plan, odd);
   }
 }
 
@@ -775,14 +806,18 @@ extern "C" int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* inp
     return launch_status("layer norm forward");
   }
   const bool odd = cols % 4 != 0 || !aligned(weight) || !aligned(bias);
-  launch_forward(s, a, words, odd);
+  if (a.total) launch_forward<true>(s, a, words, odd);
+  else launch_forward<false>(s, a, words, odd);
   return launch_status("layer norm forward");
 }
 
 extern "C" size_t tcx_sm100_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
   // either path's partial column sums
-  const int64_t splits = std::max(splits_of(rows), backward_plan(rows, cols).blocks);
+  const BackwardPlan plan = backward_plan(cols);
+  int64_t splits = splits_of(rows);
+  if (plan.vpt)
+    splits = std::max(splits, backward_blocks(rows, cols, plan.groups, plan.per_sm * sm_count() / plan.cluster));
   return static_cast<size_t>(splits) * 2 * cols * sizeof(float);
 }
 
@@ -813,8 +848,8 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
     return invalid("workspace too small for the layer norm gradient");
   TimedLaunch timer("norm_backward", s);
   float* partial = dweight ? static_cast<float*>(workspace) : nullptr;
-  const BackwardPlan plan = backward_plan(rows, cols);
-  if (plan.tpr && aligned(dy) && aligned(total) && aligned(dtotal) && aligned(dresidual) && aligned(a.dx)) {
+  const BackwardPlan plan = backward_plan(cols);
+  if (plan.vpt && aligned(dy) && aligned(total) && aligned(dtotal) && aligned(dresidual) && aligned(a.dx)) {
     const int64_t splits = launch_backward(s, a, partial, plan, cols % 4 != 0 || !aligned(weight));
     if (partial)
       launch_after(norm_join_kernel, dim3(static_cast<unsigned>(ceil_div(cols, 32))), dim3(1024), s, 0, partial,
