@@ -161,74 +161,44 @@ norm_columns_join_kernel(const float* partial, int64_t splits, int64_t cols, flo
 }
 
 // ------------------------------------------------------------------ rows in registers
-// The tensor is read in 16-byte words at places that are multiples of 4 of the whole tensor,
-// whatever the row length: a row of an odd length starts `phase` elements into its first word,
-// and the words it shares with its neighbours are stored element by element. So every access
-// is 128 bits wide, and a word of the tensor is a block of the random stream.
+// A row as its whole 16-byte words, at places that are multiples of 4 of the whole tensor
+// whatever the row length, and where rows start elsewhere (ODD) up to 3 loose elements before
+// and after them: a lane of the row's first warp to each. So all but a few accesses are 128 bits
+// wide, and a word of the tensor is a block of the random stream.
 template <bool ODD>
 struct Words {
-  int64_t at;       // of the row's first word in the tensor
-  int phase, cols;  // elements of that word before the row; elements of the row
-  int64_t count;    // of the tensor
+  int64_t at;             // of the first whole word in the tensor
+  int head, words, tail;  // loose elements before the whole words, those, and loose elements after
 
-  __device__ Words(int64_t row, int64_t n, int64_t rows) {
+  __device__ Words(int64_t row, int64_t n) {
     const int64_t first = row * n;
-    phase = ODD ? static_cast<int>(first & 3) : 0;
-    at = first - phase;
-    cols = static_cast<int>(n);
-    count = rows * n;
+    const int cols = static_cast<int>(n);
+    head = ODD ? min(static_cast<int>(-first & 3), cols) : 0;
+    at = first + head;
+    words = (cols - head) >> 2;
+    tail = ODD ? cols - head - 4 * words : 0;
   }
-  __device__ bool holds(int word) const { return 4 * word - phase < cols; }
-  __device__ bool whole(int word) const { return !ODD || (4 * word >= phase && 4 * word + 4 - phase <= cols); }
-  __device__ bool valid(int word, int j) const {
-    const int c = 4 * word + j - phase;
-    return !ODD || (c >= 0 && c < cols);
-  }
+  __device__ bool holds(int word) const { return word < words; }
   __device__ __forceinline__ float4 load(const float* p, int word) const {
-    const int64_t i = at + 4 * static_cast<int64_t>(word);
-    if (!ODD || i + 4 <= count) return __ldcs(reinterpret_cast<const float4*>(p + i));
-    float4 v = make_float4(p[i], 0.0f, 0.0f, 0.0f);
-    if (i + 1 < count) v.y = p[i + 1];
-    if (i + 2 < count) v.z = p[i + 2];
-    return v;
+    return __ldcs(reinterpret_cast<const float4*>(p + at) + word);
   }
   __device__ __forceinline__ void store(float* p, int word, float4 v) const {
-    float* const q = p + at + 4 * static_cast<int64_t>(word);
-    if (whole(word)) {
-      __stcs(reinterpret_cast<float4*>(q), v);
-    } else {
-      if (valid(word, 0)) q[0] = v.x;
-      if (valid(word, 1)) q[1] = v.y;
-      if (valid(word, 2)) q[2] = v.z;
-      if (valid(word, 3)) q[3] = v.w;
-    }
+    __stcs(reinterpret_cast<float4*>(p + at) + word, v);
   }
-  // The word with `other` outside the row.
-  __device__ __forceinline__ float4 within(int word, float4 v, float other) const {
-    return make_float4(valid(word, 0) ? v.x : other, valid(word, 1) ? v.y : other, valid(word, 2) ? v.z : other,
-                       valid(word, 3) ? v.w : other);
-  }
-  // A word of a vector over the columns (nothing outside the row).
+  // A word's columns of a vector over the row.
   __device__ __forceinline__ float4 column(const float* p, int word) const {
     if (!ODD) return __ldg(reinterpret_cast<const float4*>(p) + word);
-    const float* const q = p + 4 * word - phase;
-    if (whole(word) && 4 * word + 4 <= cols && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-      // the columns lie in the vector's own words `word - 1` and `word`
-      const float4 b = __ldg(reinterpret_cast<const float4*>(p) + word);
-      if (phase == 0) return b;
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p) + word - 1);
-      return phase == 1   ? make_float4(a.w, b.x, b.y, b.z)
-             : phase == 2 ? make_float4(a.z, a.w, b.x, b.y)
-                          : make_float4(a.y, a.z, a.w, b.x);
-    }
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (valid(word, 0)) v.x = __ldg(q);
-    if (valid(word, 1)) v.y = __ldg(q + 1);
-    if (valid(word, 2)) v.z = __ldg(q + 2);
-    if (valid(word, 3)) v.w = __ldg(q + 3);
-    return v;
+    const float* const q = p + head + 4 * word;
+    return make_float4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
   }
+  __device__ bool loose(int lane) const { return ODD && lane < head + tail; }
+  __device__ int loose_column(int lane) const { return lane < head ? lane : 4 * words + lane; }
 };
+
+// Place e of the stream is kept.
+__device__ __forceinline__ bool kept_place(uint64_t e, const philox::RoundKeys& rk, uint32_t threshold) {
+  return kept(word_of(philox::block_words(e >> 2, rk), static_cast<uint32_t>(e & 3)), threshold);
+}
 
 // Two sums over a warp in one butterfly: the lower lanes end with a's, the upper ones with b's.
 __device__ __forceinline__ float warp_sums(float a, float b) {
@@ -267,11 +237,11 @@ __global__ void __launch_bounds__(most_threads(WARPS), (FUSED ? 512 : 768) / mos
 norm_forward_kernel(ForwardArgs a) {
   __shared__ float2 smem[2][kMostWarps];
   const int warps = WARPS ? WARPS : blockDim.x >> 5, warp = threadIdx.x >> 5;
-  const int mine = warp * 32 * VPT + (threadIdx.x & 31);  // its first word, of a warp's 32 VPT
+  const int lane = threadIdx.x & 31, mine = warp * 32 * VPT + lane;  // its first word, of a warp's 32 VPT
   const float n = static_cast<float>(a.cols);
   const philox::RoundKeys rk = philox::round_keys(a.drop.key);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const Words<ODD> words(row, a.cols, a.rows);
+    const Words<ODD> words(row, a.cols);
     float v[VPT][4];
     const int64_t first = row * a.cols;
     float level;  // what the sums are taken about: the row's first element, or near it
@@ -294,15 +264,20 @@ norm_forward_kernel(ForwardArgs a) {
       for (int k = 0; k < VPT; ++k)
         if (words.holds(mine + 32 * k)) res[FUSED ? k : 0] = words.load(a.residual, mine + 32 * k);
     }
+    // a loose element, with `level` for none
+    const bool loose = ODD && warp == 0 && words.loose(lane);
+    const int column = ODD ? words.loose_column(lane) : 0;
+    float one = level;
+    if (ODD && loose) one = __ldcs(a.x + first + column);
     if (FUSED) {
+      const uint64_t start = a.drop.threshold ? dropout_start(a.drop) : 0;
       if (a.drop.threshold) {
         // the mask while the loads are on their way: 4 bits to a word
-        const uint64_t start = dropout_start(a.drop) + static_cast<uint64_t>(words.at);
         uint32_t mask[(VPT + 7) / 8];
 #pragma unroll
         for (int k = 0; k < VPT; k += 8)
-          mask[k / 8] = kept_words<(VPT < 8 ? VPT : 8)>(start + 4 * static_cast<uint64_t>(mine + 32 * k), 32,
-                                                        rk, a.drop.threshold);
+          mask[k / 8] = kept_words<(VPT < 8 ? VPT : 8)>(
+              start + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(mine + 32 * k), 32, rk, a.drop.threshold);
 #pragma unroll
         for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -322,35 +297,29 @@ norm_forward_kernel(ForwardArgs a) {
           v[k][0] = v[k][1] = v[k][2] = v[k][3] = level;
         }
       }
-    }
-    float s = 0.0f;
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-      const int word = mine + 32 * k;
-      if (!words.whole(word)) {  // nothing for what is outside the row
-        const float4 t = words.within(word, make_float4(v[k][0], v[k][1], v[k][2], v[k][3]), level);
-        v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
+      if (ODD && loose) {
+        if (a.drop.threshold)
+          one = dropped(one, kept_place(start + static_cast<uint64_t>(first + column), rk, a.drop.threshold), a.drop.scale);
+        if (a.residual) one = __fadd_rn(__ldcs(a.residual + first + column), one);
+        a.total[first + column] = one;
       }
+    }
+    float s = ODD ? one - level : 0.0f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s += v[k][j] - level;
-    }
     const float m1 = level + __fdiv_rn(row_sums(s, 0.0f, smem[0], warps, warp, 0).x, n);
-    float s1 = 0.0f, s2 = 0.0f;
+    one = ODD && loose ? one - m1 : 0.0f;
+    float s1 = one, s2 = one * one;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = mine + 32 * k;
-      if (words.holds(word)) {
-        float d[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] = v[k][j] -= m1;
-        if (!words.whole(word)) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) d[j] = words.valid(word, j) ? d[j] : 0.0f;
-        }
+      if (words.holds(mine + 32 * k)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s1 += d[j];
-          s2 = fmaf(d[j], d[j], s2);
+          v[k][j] -= m1;
+          s1 += v[k][j];
+          s2 = fmaf(v[k][j], v[k][j], s2);
         }
       }
     }
@@ -376,6 +345,12 @@ norm_forward_kernel(ForwardArgs a) {
         words.store(a.y, word, y);
       }
     }
+    if (ODD && loose) {
+      float y = (one - shift) * rstd;
+      if (a.weight) y *= __ldg(a.weight + column);
+      if (a.bias) y += __ldg(a.bias + column);
+      a.y[first + column] = y;
+    }
     if (threadIdx.x == 0) {
       a.mean[row] = m1 + shift;
       a.rstd[row] = rstd;
@@ -385,7 +360,7 @@ norm_forward_kernel(ForwardArgs a) {
 
 // Some warps of a block (of each of CLUSTER blocks) to a row, VPT words to a thread, and several
 // rows to a block at a time where they are short, a group of warps to each. A group's rows are a multiple of 4 apart, so that they
-// all start in the same phase and a thread's columns are the same in each: the weight's and the
+// all start at the same place of a word and a thread's columns are the same in each: the weight's and the
 // bias's gradients add up in its registers over the group's rows, the groups' in shared memory,
 // and the blocks' in a second kernel, each in a fixed order.
 //
@@ -396,7 +371,7 @@ constexpr int kRing = 3, kWarpsPerSm = 16;  // 128 registers a thread
 
 template <int VPT>
 constexpr int backward_bytes(int threads, bool multi) {
-  const int ring = kRing * 2 * VPT * threads * 16, columns = multi ? 2 * 4 * 128 * VPT * 4 : 0;
+  const int ring = kRing * 2 * VPT * threads * 16, columns = multi ? 2 * (128 * 4 * VPT + 4) * 4 : 0;
   return ring > columns ? ring : columns;
 }
 
@@ -430,33 +405,36 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   }
   bool live = true;  // false once a wait gave up: later ones are skipped
 
-  const Words<ODD> columns_of(opening, a.cols, a.rows);  // its phase, cols and words: those of all its rows
+  const Words<ODD> words(opening, a.cols);  // but for their places, those of all its rows
+  const bool loose = rank == 0 && warp == 0 && words.loose(lane);
+  const int column = ODD ? words.loose_column(lane) : 0;
+  float loose_dw = 0.0f, loose_db = 0.0f, loose_w = 1.0f;
+  if (ODD && loose && a.weight) loose_w = __ldg(a.weight + column);
   float dw[VPT][4], db[VPT][4];
   float4 weight[ODD ? VPT : 1];
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[k][j] = db[k][j] = 0.0f;
-    if (ODD) weight[ODD ? k : 0] = a.weight ? columns_of.column(a.weight, first_word + 32 * k) : make_float4(1, 1, 1, 1);
+    if (ODD)
+      weight[ODD ? k : 0] = a.weight && words.holds(first_word + 32 * k) ? words.column(a.weight, first_word + 32 * k)
+                                                                        : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
   }
 
   float4* const mine = stage + (threadIdx.x >> 5) * (kRing * 2 * VPT * 32) + lane;  // this thread's first place
   // Copies a row into a place: word k of dy and of total.
   auto copy = [&](int place, int64_t row) {
     if (row < a.rows) {
-      const Words<ODD> words(row, a.cols, a.rows);
-        float4* const to = mine + place * (2 * VPT * 32);
-      const int64_t at = words.at + 4 * static_cast<int64_t>(first_word);
+      float4* const to = mine + place * (2 * VPT * 32);
+      const int64_t at = row * a.cols + words.head + 4 * static_cast<int64_t>(first_word);
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         if (words.holds(first_word + 32 * k)) {
           const int64_t i = at + 128 * k;
-          const int bytes = !ODD || i + 4 <= words.count ? 16 : 4 * static_cast<int>(words.count - i);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + 32 * k)),
-                       "l"(a.dy + i), "r"(bytes)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + 32 * k)), "l"(a.dy + i)
                        : "memory");
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(to + 32 * (VPT + k))),
-                       "l"(a.total + i), "r"(bytes)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + 32 * (VPT + k))),
+                       "l"(a.total + i)
                        : "memory");
         }
       }
@@ -467,23 +445,31 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     m = row < a.rows ? __ldg(a.mean + row) : 0.0f;
     r = row < a.rows ? __ldg(a.rstd + row) : 0.0f;
   };
+  auto loose_of = [&](int64_t row, float& d, float& t) {
+    if (ODD && loose && row < a.rows) {
+      d = __ldcs(a.dy + row * a.cols + column);
+      t = __ldcs(a.total + row * a.cols + column);
+    }
+  };
 
   const philox::RoundKeys rk = philox::round_keys(a.drop.key);
   const uint64_t from = FUSED ? dropout_start(a.drop) : 0;
 #pragma unroll
   for (int k = 0; k < kRing; ++k) copy(k, opening + k * step);
-  float mean, rstd, next_mean, next_rstd;
+  float mean, rstd, next_mean, next_rstd, loose_d = 0.0f, loose_t = 0.0f;
   statistics(opening, mean, rstd);
+  loose_of(opening, loose_d, loose_t);
   unsigned turn = 0;
   int place = 0;
   for (int64_t row = opening; row < a.rows; row += step, ++turn) {
-    const Words<ODD> words(row, a.cols, a.rows);
+    const int64_t at = row * a.cols;
     statistics(row + step, next_mean, next_rstd);
     float4 extra[FUSED ? VPT : 1];
     if (FUSED && a.dtotal) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (words.holds(first_word + 32 * k)) extra[FUSED ? k : 0] = words.load(a.dtotal, first_word + 32 * k);
+        if (words.holds(first_word + 32 * k))
+          extra[FUSED ? k : 0] = __ldcs(reinterpret_cast<const float4*>(a.dtotal + at + words.head) + first_word + 32 * k);
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
     const float4* const here = mine + place * (2 * VPT * 32);
@@ -499,10 +485,6 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
         y = here[32 * k];
         t = here[32 * (VPT + k)];
         if (!ODD && a.weight) w = words.column(a.weight, word);
-        if (!words.whole(word)) {
-          y = words.within(word, y, 0.0f);
-          t = words.within(word, t, mean);
-        }
       }
       const float y4[4] = {y.x, y.y, y.z, y.w}, t4[4] = {t.x, t.y, t.z, t.w}, w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -515,12 +497,22 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
         db[k][j] += y4[j];
       }
     }
+    float loose_g = 0.0f, loose_hat = 0.0f;
+    if (ODD && loose) {
+      loose_hat = (loose_t - mean) * rstd;
+      loose_g = loose_d * loose_w;
+      s1 += loose_g;
+      s2 = fmaf(loose_g, loose_hat, s2);
+      loose_dw = fmaf(loose_d, loose_hat, loose_dw);
+      loose_db += loose_d;
+      loose_of(row + step, loose_d, loose_t);
+    }
     copy(place, row + kRing * step);
     place = place + 1 == kRing ? 0 : place + 1;
     uint32_t mask = 0;
     if (FUSED && a.dx)
-      mask = kept_words<VPT>(from + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(first_word), 32, rk,
-                             a.drop.threshold);
+      mask = kept_words<VPT>(from + static_cast<uint64_t>(at + words.head) + 4 * static_cast<uint64_t>(first_word), 32,
+                             rk, a.drop.threshold);
     const float2 sums_all = row_sums(s1, s2, sums[turn & 1] + group * warps, warps, warp, 1 + group);
     s1 = sums_all.x, s2 = sums_all.y;
     if (CLUSTER > 1) {
@@ -546,6 +538,8 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       }
     }
     const float c1 = -rstd * (s1 * share), c2 = -rstd * (s2 * share);
+    float4* const out = reinterpret_cast<float4*>(a.dresidual + at + words.head) + first_word;
+    float4* const out_x = FUSED && a.dx ? reinterpret_cast<float4*>(a.dx + at + words.head) + first_word : nullptr;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int word = first_word + 32 * k;
@@ -557,12 +551,20 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
         const float4 e = extra[FUSED ? k : 0];
         d[0] += e.x, d[1] += e.y, d[2] += e.z, d[3] += e.w;
       }
-      words.store(a.dresidual, word, make_float4(d[0], d[1], d[2], d[3]));
+      __stcs(out + 32 * k, make_float4(d[0], d[1], d[2], d[3]));
       if (FUSED && a.dx) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) d[j] = dropped(d[j], mask >> (4 * k + j) & 1, a.drop.scale);
-        words.store(a.dx, word, make_float4(d[0], d[1], d[2], d[3]));
+        __stcs(out_x + 32 * k, make_float4(d[0], d[1], d[2], d[3]));
       }
+    }
+    if (ODD && loose) {
+      const int64_t i = at + column;
+      float d = fmaf(loose_hat, c2, fmaf(loose_g, rstd, c1));
+      if (FUSED && a.dtotal) d += __ldcs(a.dtotal + i);
+      a.dresidual[i] = d;
+      if (FUSED && a.dx)
+        a.dx[i] = dropped(d, kept_place(from + static_cast<uint64_t>(i), rk, a.drop.threshold), a.drop.scale);
     }
     mean = next_mean, rstd = next_rstd;
   }
@@ -571,42 +573,49 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   if (!partial) return;
 
   const int64_t at = static_cast<int64_t>(blockIdx.x / CLUSTER) * 2 * a.cols;
-  const Words<ODD>& words = columns_of;  // a group without rows adds zeros
-  if (!MULTI) {
+  if (!MULTI) {  // a block without rows leaves zeros
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
+      if (!words.holds(first_word + 32 * k)) continue;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int c = 4 * (first_word + 32 * k) + j - words.phase;
-        if (c >= 0 && c < words.cols) {
-          partial[at + c] = dw[k][j];
-          partial[at + a.cols + c] = db[k][j];
-        }
+        const int64_t c = at + words.head + 4 * (first_word + 32 * k) + j;
+        partial[c] = dw[k][j];
+        partial[c + a.cols] = db[k][j];
       }
+    }
+    if (ODD && loose) {
+      partial[at + column] = loose_dw;
+      partial[at + a.cols + column] = loose_db;
     }
   } else {
     float* const columns = reinterpret_cast<float*>(stage);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * 4 * kSpan; i += blockDim.x) columns[i] = 0.0f;
+    constexpr int kMostColumns = 128 * (MULTI ? WARPS : 1) * VPT + 4;  // whole words, and fewer loose ones than a word
+    for (int i = threadIdx.x; i < 2 * kMostColumns; i += blockDim.x) columns[i] = 0.0f;
     for (int whose = 0; whose < groups; ++whose) {
       __syncthreads();
       if (group != whose) continue;
 #pragma unroll
-      for (int k = 0; k < VPT; ++k)
+      for (int k = 0; k < VPT; ++k) {
+        if (!words.holds(first_word + 32 * k)) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int c = 4 * (first_word + 32 * k) + j - words.phase;
-          if (c >= 0 && c < words.cols) {
-            columns[c] += dw[k][j];
-            columns[4 * kSpan + c] += db[k][j];
-          }
+          const int c = words.head + 4 * (first_word + 32 * k) + j;
+          columns[c] += dw[k][j];
+          columns[kMostColumns + c] += db[k][j];
         }
+      }
+      if (ODD && loose) {
+        columns[column] += loose_dw;
+        columns[kMostColumns + column] += loose_db;
+      }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < static_cast<int>(a.cols); c += blockDim.x) {
       partial[at + c] = columns[c];
-      partial[at + a.cols + c] = columns[4 * kSpan + c];
+      partial[at + a.cols + c] = columns[kMostColumns + c];
     }
   }
 }
@@ -645,8 +654,8 @@ norm_join_kernel(const float* __restrict__ partial, int splits, int64_t cols, fl
 // ------------------------------------------------------------------------- launches
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Words that a row can touch.
-int64_t words_of(int64_t cols) { return cols % 4 ? (cols + 6) / 4 : cols / 4; }
+// Whole words of a row, at most.
+int64_t words_of(int64_t cols) { return std::max<int64_t>(1, cols / 4); }
 
 template <int VPT, int WARPS, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int warps, bool odd) {
@@ -683,7 +692,7 @@ void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool od
 }
 
 // Blocks (or clusters) that the backward kernel runs as: what the machine holds at a time, no
-// more than there are rows for; where rows start in different phases, a multiple of
+// more than there are rows for; where rows start anywhere in a word, a multiple of
 // 4 (the rows of a group are that far apart).
 int64_t backward_blocks(int64_t rows, int64_t cols, int groups, int resident) {
   const int64_t want = std::min<int64_t>(ceil_div(rows, groups), resident);
