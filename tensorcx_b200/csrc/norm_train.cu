@@ -366,14 +366,24 @@ norm_forward_kernel(ForwardArgs a) {
 //
 // dy and total come through a ring of places in shared memory (cp.async; a thread copies and
 // reads its own words only, so that needs no barrier): a place is copied into again as soon as
-// its row is in registers, while that row's sums cross the block.
-constexpr int kRing = 3, kWarpsPerSm = 16;  // 128 registers a thread
+// its row is in registers, while that row's sums cross the block. Where a block has several
+// rows, dtotal has two places of its own, in use until the row's gradient is stored, and the
+// ring one less ([8191, 1001]: 60 -> 50 us); a longer row's is loaded when its turn comes
+// ([16384, 4096]: 216 us against 250). The weight lies beside the places where its words are
+// not aligned or the block's rows share them; else it is read through the first-level cache.
+constexpr int kWarpsPerSm = 16;  // 128 registers a thread
 
-template <int VPT>
-constexpr int backward_bytes(int threads, bool multi) {
-  const int ring = kRing * 2 * VPT * threads * 16, columns = multi ? 2 * (128 * 4 * VPT + 4) * 4 : 0;
-  return ring > columns ? ring : columns;
-}
+template <int VPT, int WARPS, bool ODD, bool FUSED>
+struct Places {
+  static constexpr bool kExtra = FUSED && WARPS, kWeight = ODD || WARPS;
+  static constexpr int kRing = kExtra ? 2 : 3;
+  static constexpr int kWarp = 32 * VPT * (kRing * 2 + (kExtra ? 2 : 0) + (kWeight ? 1 : 0));  // words of a warp
+  // with several rows to a block its column sums take their place in the end
+  static constexpr int bytes(int threads) {
+    const int words = kWarp * (threads / 32) * 16, columns = WARPS ? 2 * (128 * 4 * VPT + 4) * 4 : 0;
+    return words > columns ? words : columns;
+  }
+};
 
 // WARPS: warps of a row, with 8 / WARPS rows to a block (GROUPS); 0: any number, one row to a block.
 template <int VPT, int WARPS, int CLUSTER, bool ODD, bool FUSED>
@@ -405,23 +415,26 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   }
   bool live = true;  // false once a wait gave up: later ones are skipped
 
+  using P = Places<VPT, WARPS, ODD, FUSED>;
+  constexpr int kRing = P::kRing;
+  float4* const mine = stage + (threadIdx.x >> 5) * P::kWarp + lane;  // this thread's first place
+  float4* const mine_extra = mine + kRing * 2 * VPT * 32;             // of dtotal
+  float4* const weight = mine + (kRing * 2 + (P::kExtra ? 2 : 0)) * VPT * 32;
   const Words<ODD> words(opening, a.cols);  // but for their places, those of all its rows
   const bool loose = rank == 0 && warp == 0 && words.loose(lane);
   const int column = ODD ? words.loose_column(lane) : 0;
   float loose_dw = 0.0f, loose_db = 0.0f, loose_w = 1.0f;
   if (ODD && loose && a.weight) loose_w = __ldg(a.weight + column);
   float dw[VPT][4], db[VPT][4];
-  float4 weight[ODD ? VPT : 1];
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[k][j] = db[k][j] = 0.0f;
-    if (ODD)
-      weight[ODD ? k : 0] = a.weight && words.holds(first_word + 32 * k) ? words.column(a.weight, first_word + 32 * k)
-                                                                        : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    if (P::kWeight)
+      weight[32 * k] = a.weight && words.holds(first_word + 32 * k) ? words.column(a.weight, first_word + 32 * k)
+                                                                    : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
   }
 
-  float4* const mine = stage + (threadIdx.x >> 5) * (kRing * 2 * VPT * 32) + lane;  // this thread's first place
   // Copies a row into a place: word k of dy and of total.
   auto copy = [&](int place, int64_t row) {
     if (row < a.rows) {
@@ -441,6 +454,19 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  auto copy_extra = [&](int place, int64_t row) {
+    if (a.dtotal && row < a.rows) {
+      const int64_t at = row * a.cols + words.head + 4 * static_cast<int64_t>(first_word);
+#pragma unroll
+      for (int k = 0; k < VPT; ++k)
+        if (words.holds(first_word + 32 * k))
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           ptx::smem_u32(mine_extra + (place * VPT + k) * 32)),
+                       "l"(a.dtotal + at + 128 * k)
+                       : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   auto statistics = [&](int64_t row, float& m, float& r) {
     m = row < a.rows ? __ldg(a.mean + row) : 0.0f;
     r = row < a.rows ? __ldg(a.rstd + row) : 0.0f;
@@ -455,7 +481,10 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   const philox::RoundKeys rk = philox::round_keys(a.drop.key);
   const uint64_t from = FUSED ? dropout_start(a.drop) : 0;
 #pragma unroll
-  for (int k = 0; k < kRing; ++k) copy(k, opening + k * step);
+  for (int k = 0; k < kRing; ++k) {
+    copy(k, opening + k * step);
+    if (P::kExtra) copy_extra(k, opening + k * step);
+  }
   float mean, rstd, next_mean, next_rstd, loose_d = 0.0f, loose_t = 0.0f;
   statistics(opening, mean, rstd);
   loose_of(opening, loose_d, loose_t);
@@ -464,14 +493,15 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   for (int64_t row = opening; row < a.rows; row += step, ++turn) {
     const int64_t at = row * a.cols;
     statistics(row + step, next_mean, next_rstd);
-    float4 extra[FUSED ? VPT : 1];
-    if (FUSED && a.dtotal) {
+    float4 extra[FUSED && !P::kExtra ? VPT : 1];
+    if (FUSED && !P::kExtra && a.dtotal) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
         if (words.holds(first_word + 32 * k))
-          extra[FUSED ? k : 0] = __ldcs(reinterpret_cast<const float4*>(a.dtotal + at + words.head) + first_word + 32 * k);
+          extra[P::kExtra ? 0 : k] =
+              __ldcs(reinterpret_cast<const float4*>(a.dtotal + at + words.head) + first_word + 32 * k);
     }
-    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(P::kExtra ? 3 : kRing - 1) : "memory");
     const float4* const here = mine + place * (2 * VPT * 32);
     float g[VPT][4], hat[VPT][4];
     float s1 = 0.0f, s2 = 0.0f;
@@ -480,11 +510,11 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       const int word = first_word + 32 * k;
       const bool in = words.holds(word);
       float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), t = make_float4(mean, mean, mean, mean);
-      float4 w = ODD ? weight[ODD ? k : 0] : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      float4 w = P::kWeight ? weight[32 * k] : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
       if (in) {
         y = here[32 * k];
         t = here[32 * (VPT + k)];
-        if (!ODD && a.weight) w = words.column(a.weight, word);
+        if (!P::kWeight && a.weight) w = words.column(a.weight, word);
       }
       const float y4[4] = {y.x, y.y, y.z, y.w}, t4[4] = {t.x, t.y, t.z, t.w}, w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -508,7 +538,6 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       loose_of(row + step, loose_d, loose_t);
     }
     copy(place, row + kRing * step);
-    place = place + 1 == kRing ? 0 : place + 1;
     uint32_t mask = 0;
     if (FUSED && a.dx)
       mask = kept_words<VPT>(from + static_cast<uint64_t>(at + words.head) + 4 * static_cast<uint64_t>(first_word), 32,
@@ -538,6 +567,7 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       }
     }
     const float c1 = -rstd * (s1 * share), c2 = -rstd * (s2 * share);
+    if (P::kExtra) asm volatile("cp.async.wait_group 3;" ::: "memory");
     float4* const out = reinterpret_cast<float4*>(a.dresidual + at + words.head) + first_word;
     float4* const out_x = FUSED && a.dx ? reinterpret_cast<float4*>(a.dx + at + words.head) + first_word : nullptr;
 #pragma unroll
@@ -548,7 +578,7 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = fmaf(hat[k][j], c2, fmaf(g[k][j], rstd, c1));
       if (FUSED && a.dtotal) {
-        const float4 e = extra[FUSED ? k : 0];
+        const float4 e = P::kExtra ? mine_extra[(place * VPT + k) * 32] : extra[P::kExtra ? 0 : k];
         d[0] += e.x, d[1] += e.y, d[2] += e.z, d[3] += e.w;
       }
       __stcs(out + 32 * k, make_float4(d[0], d[1], d[2], d[3]));
@@ -566,6 +596,8 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       if (FUSED && a.dx)
         a.dx[i] = dropped(d, kept_place(from + static_cast<uint64_t>(i), rk, a.drop.threshold), a.drop.scale);
     }
+    if (P::kExtra) copy_extra(place, row + kRing * step);
+    place = place + 1 == kRing ? 0 : place + 1;
     mean = next_mean, rstd = next_rstd;
   }
   dependents_may_launch();
@@ -723,7 +755,7 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
   const int threads = plan.warps * plan.groups * 32;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = backward_bytes<VPT>(threads, WARPS != 0);
+  cfg.dynamicSmemBytes = Places<VPT, WARPS, ODD, FUSED>::bytes(threads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -737,7 +769,7 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
   if (dev >= 0 && dev < 64) held = resident[dev][plan.warps];
   if (held == 0) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         backward_bytes<VPT>(kMostWarps * 32, WARPS != 0));
+                         Places<VPT, WARPS, ODD, FUSED>::bytes(kMostWarps * 32));
     held = plan.per_sm * sm_count() / CLUSTER;
     cfg.gridDim = dim3(static_cast<unsigned>(held * CLUSTER));
     int clusters = 0;
