@@ -326,16 +326,17 @@ __device__ Tile tile_of(const Args& a, const Scan& sc, unsigned i) {
 }
 
 // A thread's rows of an array of a chunk in shared memory. VEC = 4: each thread copies and
-// reads places of its own (16 bytes of a row). VEC = 1: rows start at any element, so a warp
-// copies the 16-byte words that hold its rows, 9 to a row, and a lane reads its channel at the
-// row's own distance from the word's start; rows that begin before the array itself does are
-// copied element by element.
-template <int VEC>
+// reads places of its own (16 bytes of a row). VEC = 1 and SHIFTED: rows start at any element
+// of an aligned array, so a warp copies the 16-byte words that hold its rows, 9 to a row, and a
+// lane reads its channel at the row's own distance (shift) from the first word's start, which is
+// the same in every array. VEC = 1 alone: arrays at any address, copied element by element (an
+// instruction that copies 4 bytes a lane takes the load unit some 30 cycles: only where needed).
+template <int VEC, bool SHIFTED>
 struct Rows {
   static constexpr int kWarps = VEC == 4 ? 4 : 8;           // that work on a chunk
   static constexpr int kSteps = kChunk / (kWarps * VEC);    // of one group
   static constexpr int kGroup = 32 / VEC;                   // lanes of a group
-  static constexpr int kNext = VEC == 4 ? 128 : 36;         // floats from one step's place to the next one's
+  static constexpr int kNext = SHIFTED ? 36 : 32 * VEC;     // floats from one step's place to the next one's
   static constexpr int kArray = kWarps * kSteps * kNext;    // floats of an array
   static_assert(kWarps * VEC * kSteps == kChunk, "");
   int lane, warp, column, mine;  // its first channel within the chain, its first step of the chunk
@@ -345,74 +346,83 @@ struct Rows {
     lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     column = (lane % kGroup) * VEC;
     mine = (warp * VEC + lane / kGroup) * kSteps;
-    place = stage + warp * kSteps * kNext + (VEC == 4 ? lane * VEC : 0);
+    place = stage + warp * kSteps * kNext + (SHIFTED ? 0 : lane * VEC);
   }
   __device__ int group() const { return lane / kGroup; }
 
   // Copies steps [from, to) of `channels` channels; `row` points at the chunk's first channel
-  // and step, `all` at the array of `count` elements, and a step is `stride` elements.
+  // and step, `all` at the array of `count` elements, and a step is `stride` elements. Places
+  // of steps outside become 0.
   __device__ __forceinline__ void copy(int array, const float* all, int64_t count, const float* row, int64_t stride,
                                        int channels, int from, int to) const {
-    const uint32_t dst = ptx::smem_u32(place + array * kArray);
-    if constexpr (VEC == 4) {
+    uint32_t dst = ptx::smem_u32(place + array * kArray);
+    if constexpr (!SHIFTED) {
       const float* p = row + mine * stride + column;
       if (column < channels && mine >= from && mine + kSteps <= to) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s, p += stride)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * s * kNext), "l"(p) : "memory");
+        for (int s = 0; s < kSteps; ++s, p += stride) {
+          if constexpr (VEC == 4)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * s * kNext), "l"(p) : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * s * kNext), "l"(p) : "memory");
+        }
       } else {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s, p += stride) {
           const bool in = column < channels && mine + s >= from && mine + s < to;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 4 * s * kNext), "l"(in ? p : all),
-                       "r"(in ? 16 : 0)
-                       : "memory");
+          if constexpr (VEC == 4)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 4 * s * kNext), "l"(in ? p : all),
+                         "r"(in ? 16 : 0)
+                         : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * s * kNext), "l"(in ? p : all),
+                         "r"(in ? 4 : 0)
+                         : "memory");
         }
       }
     } else {
-      const float* const end = all + count;
-      const float* const word = reinterpret_cast<const float*>(reinterpret_cast<uintptr_t>(all) & ~uintptr_t(15));
       if (lane >= 27) return;  // 9 lanes to a row, 3 rows at a time
-      int r = lane / 9;
-      const int q4 = 4 * (lane - 9 * r);
-      const float* start = row + (mine + r) * stride;
-      uint32_t to_at = dst + 4 * (r * kNext + q4);
+      const int third = lane / 9, q4 = 4 * (lane - 9 * third);
+      const float* start = row + (mine + third) * stride;
+      dst += 4 * (third * kNext + q4);
+      if (channels == kWide && mine >= from && mine + kSteps <= to && all + count - row > (kChunk + 1) * max(stride, int64_t(0)) + 64) {
+        // every row is there, and the array goes on after the last one's words
 #pragma unroll
-      for (int k = 0; k < kSteps; k += 3, r += 3, start += 3 * stride, to_at += 12 * kNext) {
-        if (r >= kSteps) break;
-        const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(start) >> 2) & 3;
-        const bool in = mine + r >= from && mine + r < to && q4 - shift < channels;
-        const float* const p = start + (q4 - shift);
-        if (in && p < all) {
-          for (int j = 0; j < 4; ++j)
-            if (p + j >= all && p + j < end)
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to_at + 4 * j), "l"(p + j) : "memory");
-        } else {
-          const int bytes = in ? static_cast<int>(min(end - p, static_cast<int64_t>(4))) * 4 : 0;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to_at), "l"(in ? p : word), "r"(bytes)
+        for (int k = 0; k < kSteps; k += 3, start += 3 * stride) {
+          const int reach = q4 - (static_cast<int>(reinterpret_cast<uintptr_t>(start) >> 2) & 3);
+          if (reach < kWide && k + third < kSteps)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 4 * k * kNext), "l"(start + reach)
+                         : "memory");
+        }
+      } else {
+#pragma unroll 1
+        for (int k = 0; k + third < kSteps; k += 3, start += 3 * stride) {
+          const int step = mine + k + third, reach = q4 - (static_cast<int>(reinterpret_cast<uintptr_t>(start) >> 2) & 3);
+          const bool in = step >= from && step < to && reach < channels;
+          const float* const word = in ? start + reach : all;
+          const int bytes = in ? 4 * static_cast<int>(min(all + count - word, static_cast<int64_t>(4))) : 0;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 4 * k * kNext), "l"(word), "r"(bytes)
                        : "memory");
         }
       }
     }
   }
-  // Where this thread's step 0 lies; a step on, at(s) of a later one.
-  __device__ __forceinline__ int shift(const float* row, int64_t stride) const {
-    if (VEC == 4) return 0;
-    return static_cast<int>(reinterpret_cast<uintptr_t>(row + mine * stride) >> 2) & 3;
+  // The shift of this thread's first step, and of the next one; rows of all arrays have it.
+  __device__ __forceinline__ int shift(int64_t at, int64_t stride) const {
+    return SHIFTED ? static_cast<int>(at + mine * stride) & 3 : 0;
   }
-  __device__ __forceinline__ float* at(int array, int s, int shift, int stride) const {
-    float* const p = place + array * kArray + s * kNext;
-    return VEC == 4 ? p : p + ((shift + s * stride) & 3) + lane;
+  __device__ __forceinline__ float* at(int array, int s, int shift) const {
+    return place + array * kArray + s * kNext + (SHIFTED ? shift + lane : 0);
   }
   // The copies of this thread's warp, all but the last N groups, are there.
   template <int N>
   __device__ __forceinline__ void arrived() const {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-    if (VEC == 1) __syncwarp();
+    if (SHIFTED) __syncwarp();
   }
   // Its places may be copied into again.
   __device__ __forceinline__ void done() const {
-    if (VEC == 1) __syncwarp();
+    if (SHIFTED) __syncwarp();
   }
 };
 
@@ -459,10 +469,10 @@ __device__ __forceinline__ void enter_group(float (&h)[VEC], const float* entry,
 // carrier): the walk back does not stand between a chunk's loads and its stores. The values
 // wait in shared memory between their two uses. A block that takes whole chains (WHOLE) has
 // the entering state from its own last chunk, and there are no records.
-template <int VEC>
+template <int VEC, bool SHIFTED>
 struct Forward {
-  static constexpr int kRing = 3, kPerSm = 2, kThreads = (Rows<VEC>::kWarps + 2) * 32;
-  static constexpr int kBytes = kRing * 2 * Rows<VEC>::kArray * 4;  // gate, x
+  static constexpr int kRing = 3, kPerSm = 2, kThreads = (Rows<VEC, SHIFTED>::kWarps + 2) * 32;
+  static constexpr int kBytes = kRing * 2 * Rows<VEC, SHIFTED>::kArray * 4;  // gate, x
 };
 
 // Barriers of the working warps with the teller and with the carrier, and of those two; two
@@ -475,11 +485,11 @@ __device__ __forceinline__ void signal(int barrier, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 }
 
-template <int VEC, bool SIGMOID, bool WHOLE>
-__global__ void __launch_bounds__(Forward<VEC>::kThreads, Forward<VEC>::kPerSm)
+template <int VEC, bool SHIFTED, bool SIGMOID, bool WHOLE>
+__global__ void __launch_bounds__(Forward<VEC, SHIFTED>::kThreads, Forward<VEC, SHIFTED>::kPerSm)
 scan_forward_kernel(Args a, Scan sc, int* err) {
-  using R = Rows<VEC>;
-  constexpr int kRing = Forward<VEC>::kRing, kSteps = R::kSteps, kWarps = R::kWarps;
+  using R = Rows<VEC, SHIFTED>;
+  constexpr int kRing = Forward<VEC, SHIFTED>::kRing, kSteps = R::kSteps, kWarps = R::kWarps;
   constexpr int kAll = (kWarps + 1) * 32;  // the warps that work, and one of the two others
   extern __shared__ __align__(16) float stage[];
   // The warps' parts. The teller puts the whole chunk's in the place of the last warp's, which
@@ -572,14 +582,14 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
   auto make = [&](unsigned i, float (&eA)[VEC], float (&eB)[VEC]) {
     const Tile& m = line[i & 7];
     const int first = 2 * (i % kRing), live = m.to - mine;
-    const int gs = rows.shift(a.gate + m.at, a.channels), xs = rows.shift(a.x + m.at, a.channels);
+    int shift = rows.shift(m.at, a.channels);
     float A[VEC], B[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) A[j] = 1.0f, B[j] = 0.0f;
 #pragma unroll 8
-    for (int s = 0; s < kSteps; ++s) {
-      float* const gp = rows.at(first, s, gs, turn_by);
-      float* const xp = rows.at(first + 1, s, xs, turn_by);
+    for (int s = 0; s < kSteps; ++s, shift = (shift + turn_by) & 3) {
+      float* const gp = rows.at(first, s, shift);
+      float* const xp = rows.at(first + 1, s, shift);
       float g[VEC], v[VEC];
       load_shared<VEC>(g, gp);
       load_shared<VEC>(v, xp);
@@ -621,15 +631,15 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
     float h[VEC];
     enter_group<VEC>(h, parts[i & 1][warp][0], eA, eB, group, column);
     const int first = 2 * (i % kRing);
-    const int gs = rows.shift(a.gate + m.at, a.channels), xs = rows.shift(a.x + m.at, a.channels);
     const bool inside = column < m.channels;
     auto write = [&](bool whole) {
       float* p = a.h + m.at + mine * a.channels + column;
+      int shift = rows.shift(m.at, a.channels);
 #pragma unroll 8
-      for (int s = 0; s < kSteps; ++s, p += a.channels) {
+      for (int s = 0; s < kSteps; ++s, p += a.channels, shift = (shift + turn_by) & 3) {
         float g[VEC], v[VEC];
-        load_shared<VEC>(g, rows.at(first, s, gs, turn_by));
-        load_shared<VEC>(v, rows.at(first + 1, s, xs, turn_by));
+        load_shared<VEC>(g, rows.at(first, s, shift));
+        load_shared<VEC>(v, rows.at(first + 1, s, shift));
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           if (!SIGMOID && !whole && mine + s >= m.to) g[j] = 1.0f;
@@ -673,16 +683,16 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
 // A chunk is twice the forward one's bytes, so three blocks to an SM hide each other's walk
 // back: gate and dh go into registers for the parts, their places take the next chunk's, and
 // the state before each step and x are read when the entering gradient is known.
-template <int VEC, bool SIGMOID>
+template <int VEC, bool SHIFTED, bool SIGMOID>
 struct Backward {
-  static constexpr int kPerSm = VEC == 4 ? 3 : 2, kThreads = Rows<VEC>::kWarps * 32;
-  static constexpr int kBytes = (SIGMOID ? 4 : 3) * Rows<VEC>::kArray * 4;  // gate, dh, the state before, x
+  static constexpr int kPerSm = VEC == 4 ? 3 : 2, kThreads = Rows<VEC, SHIFTED>::kWarps * 32;
+  static constexpr int kBytes = (SIGMOID ? 4 : 3) * Rows<VEC, SHIFTED>::kArray * 4;  // gate, dh, the state before, x
 };
 
-template <int VEC, bool SIGMOID>
-__global__ void __launch_bounds__(Backward<VEC, SIGMOID>::kThreads, Backward<VEC, SIGMOID>::kPerSm)
+template <int VEC, bool SHIFTED, bool SIGMOID>
+__global__ void __launch_bounds__(Backward<VEC, SHIFTED, SIGMOID>::kThreads, Backward<VEC, SHIFTED, SIGMOID>::kPerSm)
 scan_backward_kernel(Args a, Scan sc, int* err) {
-  using R = Rows<VEC>;
+  using R = Rows<VEC, SHIFTED>;
   constexpr int kSteps = R::kSteps, kWarps = R::kWarps;
   extern __shared__ __align__(16) float stage[];
   __shared__ float parts[kWarps][2][kWide];
@@ -718,15 +728,16 @@ scan_backward_kernel(Args a, Scan sc, int* err) {
     const Tile m = line[turn & 1];
     const Tile& next = line[(turn + 1) & 1];
     if (threadIdx.x == 0) line[(turn + 1) & 1] = tile_of<true, false>(a, sc, later);
-    const int gs = rows.shift(a.gate + m.at, stride), ds = rows.shift(a.dh + m.at, stride);
+    const int opening = rows.shift(m.at, stride);
     rows.template arrived<1>();
     float g[kSteps][VEC], v[kSteps][VEC], A[VEC], B[VEC];  // gate and dh
 #pragma unroll
     for (int i = 0; i < VEC; ++i) A[i] = 1.0f, B[i] = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      load_shared<VEC>(g[s], rows.at(0, s, gs, turn_by));
-      load_shared<VEC>(v[s], rows.at(1, s, ds, turn_by));
+      const int shift = (opening + s * turn_by) & 3;
+      load_shared<VEC>(g[s], rows.at(0, s, shift));
+      load_shared<VEC>(v[s], rows.at(1, s, shift));
       const bool live = mine + s >= m.from && mine + s < m.to;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -770,15 +781,14 @@ scan_backward_kernel(Args a, Scan sc, int* err) {
     float c[VEC];
     enter_group<VEC>(c, entries[warp], eA, eB, group, column);
     rows.template arrived<1>();
-    const int hs = rows.shift(a.hs + m.at - a.channels, stride), xs = SIGMOID ? rows.shift(a.x + m.at, stride) : 0;
     float *p = a.dgate + m.at + mine * stride + column, *q = a.dx + m.at + mine * stride + column;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s, p += stride, q += stride) {
       if (column >= m.channels || mine + s >= m.steps) continue;
       float before[VEC], x[VEC] = {}, dgate[VEC], dx[VEC];
-      load_shared<VEC>(before, rows.at(2, s, hs, turn_by));
+      load_shared<VEC>(before, rows.at(2, s, (opening + (s + 1) * turn_by) & 3));  // the row before
       if (m.last && mine + s + 1 == m.steps) start_of<VEC>(before, a.initial, m.edge + column);
-      if (SIGMOID) load_shared<VEC>(x, rows.at(3, s, xs, turn_by));
+      if (SIGMOID) load_shared<VEC>(x, rows.at(3, s, (opening + s * turn_by) & 3));
       backward_step<VEC, SIGMOID>(g[s], v[s], before, x, mine + s >= m.from, c, dgate, dx);
       store<VEC>(p, dgate);
       store<VEC>(q, dx);
@@ -793,10 +803,10 @@ scan_backward_kernel(Args a, Scan sc, int* err) {
 // ------------------------------------------------------------------------- launches
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Rows of whole 16-byte words in every buffer.
-bool wide(const Args& a) {
+// Every buffer starts on a 16-byte word; rows of whole words besides: all their rows do.
+bool all_aligned(const Args& a) {
   const void* all[] = {a.gate, a.x, a.initial, a.h, a.state, a.dh, a.hs, a.dstate, a.dgate, a.dx, a.dinitial};
-  bool fits = a.channels % 4 == 0;
+  bool fits = true;
   for (const void* p : all) fits = fits && aligned(p);
   return fits;
 }
@@ -839,7 +849,7 @@ int launch_scan(cudaStream_t s, const Args& a, int threads, int bytes, int per_s
   return launch_status("recurrence");
 }
 
-template <int VEC, bool SIGMOID>
+template <int VEC, bool SHIFTED, bool SIGMOID>
 int launch_forward(cudaStream_t s, const Args& a, void* workspace) {
   if (walks<VEC>(a)) {
     TimedLaunch timer("recurrence_walk", s);
@@ -847,16 +857,16 @@ int launch_forward(cudaStream_t s, const Args& a, void* workspace) {
         <<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
     return launch_status("recurrence");
   }
-  using F = Forward<VEC>;
+  using F = Forward<VEC, SHIFTED>;
   TimedLaunch timer("recurrence_scan", s);
   const bool whole = takes_whole(a.batch * ceil_div(a.channels, kWide), F::kPerSm * sm_count());
   if (whole)
-    return launch_scan<scan_forward_kernel<VEC, SIGMOID, true>>(s, a, F::kThreads, F::kBytes, F::kPerSm, true, nullptr);
-  return launch_scan<scan_forward_kernel<VEC, SIGMOID, false>>(s, a, F::kThreads, F::kBytes, F::kPerSm, false,
+    return launch_scan<scan_forward_kernel<VEC, SHIFTED, SIGMOID, true>>(s, a, F::kThreads, F::kBytes, F::kPerSm, true, nullptr);
+  return launch_scan<scan_forward_kernel<VEC, SHIFTED, SIGMOID, false>>(s, a, F::kThreads, F::kBytes, F::kPerSm, false,
                                                                workspace);
 }
 
-template <int VEC, bool SIGMOID>
+template <int VEC, bool SHIFTED, bool SIGMOID>
 int launch_backward(cudaStream_t s, const Args& a, void* workspace) {
   if (walks<VEC>(a)) {
     TimedLaunch timer("recurrence_walk_backward", s);
@@ -864,9 +874,23 @@ int launch_backward(cudaStream_t s, const Args& a, void* workspace) {
         <<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
     return launch_status("recurrence");
   }
-  using K = Backward<VEC, SIGMOID>;
+  using K = Backward<VEC, SHIFTED, SIGMOID>;
   TimedLaunch timer("recurrence_scan_backward", s);
-  return launch_scan<scan_backward_kernel<VEC, SIGMOID>>(s, a, K::kThreads, K::kBytes, K::kPerSm, false, workspace);
+  return launch_scan<scan_backward_kernel<VEC, SHIFTED, SIGMOID>>(s, a, K::kThreads, K::kBytes, K::kPerSm, false, workspace);
+}
+
+template <bool SIGMOID>
+int launch_forward(cudaStream_t s, const Args& a, void* workspace) {
+  if (!all_aligned(a)) return launch_forward<1, false, SIGMOID>(s, a, workspace);
+  if (a.channels % 4) return launch_forward<1, true, SIGMOID>(s, a, workspace);
+  return launch_forward<4, false, SIGMOID>(s, a, workspace);
+}
+
+template <bool SIGMOID>
+int launch_backward(cudaStream_t s, const Args& a, void* workspace) {
+  if (!all_aligned(a)) return launch_backward<1, false, SIGMOID>(s, a, workspace);
+  if (a.channels % 4) return launch_backward<1, true, SIGMOID>(s, a, workspace);
+  return launch_backward<4, false, SIGMOID>(s, a, workspace);
 }
 
 // A call of no steps: the state goes through.
@@ -911,9 +935,8 @@ extern "C" int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const
          channels};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (time == 0) return pass_through(s, initial, state, batch * channels);
-  const bool sigmoid = form == TCX_RECURRENCE_SIGMOID;
-  if (wide(a)) return sigmoid ? launch_forward<4, true>(s, a, workspace) : launch_forward<4, false>(s, a, workspace);
-  return sigmoid ? launch_forward<1, true>(s, a, workspace) : launch_forward<1, false>(s, a, workspace);
+  return form == TCX_RECURRENCE_SIGMOID ? launch_forward<true>(s, a, workspace)
+                                        : launch_forward<false>(s, a, workspace);
 }
 
 extern "C" int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, const float* dh, const float* gate,
@@ -931,7 +954,6 @@ extern "C" int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, cons
   Args a{gate, x, initial, lengths, nullptr, nullptr, dh, h, dstate, dgate, dx, dinitial, batch, time, channels};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (time == 0) return pass_through(s, dstate, dinitial, batch * channels);
-  const bool sigmoid = form == TCX_RECURRENCE_SIGMOID;
-  if (wide(a)) return sigmoid ? launch_backward<4, true>(s, a, workspace) : launch_backward<4, false>(s, a, workspace);
-  return sigmoid ? launch_backward<1, true>(s, a, workspace) : launch_backward<1, false>(s, a, workspace);
+  return form == TCX_RECURRENCE_SIGMOID ? launch_backward<true>(s, a, workspace)
+                                        : launch_backward<false>(s, a, workspace);
 }
