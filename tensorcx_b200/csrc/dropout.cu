@@ -34,7 +34,8 @@ dropout_kernel(const float* x, const float* residual, float* out, int64_t count,
         if (RESIDUAL) r[k] = __ldcs(reinterpret_cast<const float4*>(residual) + w);
       }
     }
-    const uint32_t mask = kept_words<kWords>(start + 4 * static_cast<uint64_t>(first), kThreads, rk, d.threshold);
+    uint32_t mask = ~0u;
+    if (d.threshold) mask = kept_words<kWords>(start + 4 * static_cast<uint64_t>(first), kThreads, rk, d.threshold);
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
       const int64_t w = first + k * kThreads;

@@ -371,7 +371,9 @@ norm_forward_kernel(ForwardArgs a) {
 // ring one less ([8191, 1001]: 60 -> 50 us); a longer row's is loaded when its turn comes
 // ([16384, 4096]: 216 us against 250). The weight lies beside the places where its words are
 // not aligned or the block's rows share them; else it is read through the first-level cache.
-constexpr int kWarpsPerSm = 16;  // 128 registers a thread
+
+// Warps to an SM: 128 registers a thread, or 64 where it holds one word of each array.
+constexpr int warps_per_sm(int vpt) { return vpt == 1 ? 32 : 16; }
 
 template <int VPT, int WARPS, bool ODD, bool FUSED>
 struct Places {
@@ -387,7 +389,7 @@ struct Places {
 
 // WARPS: warps of a row, with 8 / WARPS rows to a block (GROUPS); 0: any number, one row to a block.
 template <int VPT, int WARPS, int CLUSTER, bool ODD, bool FUSED>
-__global__ void __launch_bounds__(WARPS ? 256 : 512, WARPS ? 2 : 1)
+__global__ void __launch_bounds__(WARPS ? 256 : 512, WARPS ? warps_per_sm(VPT) / 8 : 1)
 norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   static_assert(CLUSTER == 1 || WARPS == 0, "");
   constexpr bool MULTI = WARPS != 0;
@@ -745,7 +747,7 @@ BackwardPlan backward_plan(int64_t cols) {
   plan.cluster = warps <= 8 ? 1 : warps <= 16 ? 2 : warps <= 32 ? 4 : 8;
   plan.warps = static_cast<int>(ceil_div(warps, plan.cluster));
   plan.groups = plan.warps == 1 || plan.warps == 2 || plan.warps == 4 ? 8 / plan.warps : 1;
-  plan.per_sm = std::max(1, kWarpsPerSm / (plan.warps * plan.groups));
+  plan.per_sm = std::max(1, warps_per_sm(plan.vpt) / (plan.warps * plan.groups));
   return plan;
 }
 
