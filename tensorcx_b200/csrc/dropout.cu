@@ -77,6 +77,21 @@ dropout_elements_kernel(const float* x, const float* residual, float* out, int64
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
+
+void launch_dropout(cudaStream_t s, const float* input, const float* residual, float* output, int64_t count,
+                    const Dropout& d) {
+  if (aligned(input) && aligned(residual) && aligned(output)) {
+    const int64_t want = count < 4 ? 1 : ceil_div(count >> 2, kThreads * kWords);
+    const unsigned grid = static_cast<unsigned>(want < (1 << 30) ? want : 1 << 30);
+    if (residual) dropout_kernel<true><<<grid, kThreads, 0, s>>>(input, residual, output, count, d);
+    else dropout_kernel<false><<<grid, kThreads, 0, s>>>(input, residual, output, count, d);
+  } else {
+    const int64_t want = ceil_div(count, kThreads);
+    const unsigned grid = static_cast<unsigned>(want < 16 * sm_count() ? want : 16 * sm_count());
+    dropout_elements_kernel<<<grid, kThreads, 0, s>>>(input, residual, output, count, d);
+  }
+}
+
 }  // namespace tcx
 
 using namespace tcx;
@@ -92,15 +107,6 @@ extern "C" int tcx_sm100_dropout(tcx_stream_t stream, const float* input, const 
   if (!input || !output) return invalid("missing buffer");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   TimedLaunch timer("dropout", s);
-  if (aligned(input) && aligned(residual) && aligned(output)) {
-    const int64_t want = count < 4 ? 1 : ceil_div(count >> 2, kThreads * kWords);
-    const unsigned grid = static_cast<unsigned>(want < (1 << 30) ? want : 1 << 30);
-    if (residual) dropout_kernel<true><<<grid, kThreads, 0, s>>>(input, residual, output, count, d);
-    else dropout_kernel<false><<<grid, kThreads, 0, s>>>(input, residual, output, count, d);
-  } else {
-    const int64_t want = ceil_div(count, kThreads);
-    const unsigned grid = static_cast<unsigned>(want < 16 * sm_count() ? want : 16 * sm_count());
-    dropout_elements_kernel<<<grid, kThreads, 0, s>>>(input, residual, output, count, d);
-  }
+  launch_dropout(s, input, residual, output, count, d);
   return launch_status("dropout");
 }

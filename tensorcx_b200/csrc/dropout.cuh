@@ -39,6 +39,10 @@ inline bool make_dropout(Dropout& d, double p, uint64_t seed, uint64_t offset, c
   return true;
 }
 
+// output = residual + dropout(input), or dropout(input) without a residual (dropout.cu).
+void launch_dropout(cudaStream_t s, const float* input, const float* residual, float* output, int64_t count,
+                    const Dropout& d);
+
 __device__ __forceinline__ uint64_t dropout_start(const Dropout& d) {
   return d.offset + (d.step_offset ? static_cast<uint64_t>(__ldg(d.step_offset)) : 0);
 }

@@ -231,18 +231,42 @@ constexpr int kMostWarps = 16;
 constexpr int most_threads(int warps) { return 32 * (warps ? warps : kMostWarps); }
 
 // One block to a row, VPT words to a thread, as many warps as the row needs. Each element is
-// read once and written once; the statistics take two block reductions.
-template <int VPT, int WARPS, bool ODD, bool FUSED>
-__global__ void __launch_bounds__(most_threads(WARPS), (FUSED ? 512 : 768) / most_threads(WARPS))
+// read once and written once; the statistics take two block reductions. STAGED: few blocks fit
+// an SM, so that each takes rows in turn, and the next row's words come into shared memory
+// (cp.async; a thread copies and reads its own only) while this one is worked on.
+template <int VPT, int WARPS, bool ODD, bool FUSED, bool STAGED>
+__global__ void __launch_bounds__(most_threads(WARPS), STAGED ? 1 : (FUSED ? 512 : 768) / most_threads(WARPS))
 norm_forward_kernel(ForwardArgs a) {
+  extern __shared__ __align__(16) float4 stage[];
   __shared__ float2 smem[2][kMostWarps];
   const int warps = WARPS ? WARPS : blockDim.x >> 5, warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31, mine = warp * 32 * VPT + lane;  // its first word, of a warp's 32 VPT
   const float n = static_cast<float>(a.cols);
   const philox::RoundKeys rk = philox::round_keys(a.drop.key);
+  float4* const place = stage + warp * (FUSED ? 2 : 1) * 32 * VPT + lane;
+  auto copy = [&](int64_t row) {
+    if (row < a.rows) {
+      const Words<ODD> words(row, a.cols);
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        if (words.holds(mine + 32 * k)) {
+          const int64_t i = words.at + 4 * static_cast<int64_t>(mine) + 128 * k;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(place + 32 * k)), "l"(a.x + i)
+                       : "memory");
+          if (FUSED && a.residual)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(place + 32 * (VPT + k))),
+                         "l"(a.residual + i)
+                         : "memory");
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (STAGED) copy(blockIdx.x);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const Words<ODD> words(row, a.cols);
     float v[VPT][4];
+    if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
     const int64_t first = row * a.cols;
     float level;  // what the sums are taken about: the row's first element, or near it
     if (FUSED) {
@@ -256,14 +280,16 @@ norm_forward_kernel(ForwardArgs a) {
     for (int k = 0; k < VPT; ++k) {
       const int word = mine + 32 * k;
       float4 t = make_float4(level, level, level, level);
-      if (words.holds(word)) t = words.load(a.x, word);
+      if (words.holds(word)) t = STAGED ? place[32 * k] : words.load(a.x, word);
       v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
     }
     if (FUSED && a.residual) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (words.holds(mine + 32 * k)) res[FUSED ? k : 0] = words.load(a.residual, mine + 32 * k);
+        if (words.holds(mine + 32 * k))
+          res[FUSED ? k : 0] = STAGED ? place[32 * (VPT + k)] : words.load(a.residual, mine + 32 * k);
     }
+    if (STAGED) copy(row + gridDim.x);
     // a loose element, with `level` for none
     const bool loose = ODD && warp == 0 && words.loose(lane);
     const int column = ODD ? words.loose_column(lane) : 0;
@@ -694,19 +720,35 @@ int64_t words_of(int64_t cols) { return std::max<int64_t>(1, cols / 4); }
 template <int VPT, int WARPS, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int warps, bool odd) {
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 30));
-  if (odd) norm_forward_kernel<VPT, WARPS, true, FUSED><<<grid, 32 * warps, 0, s>>>(a);
-  else norm_forward_kernel<VPT, WARPS, false, FUSED><<<grid, 32 * warps, 0, s>>>(a);
+  if (odd) norm_forward_kernel<VPT, WARPS, true, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
+  else norm_forward_kernel<VPT, WARPS, false, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
 }
+
+template <int VPT, bool ODD, bool FUSED>
+void launch_staged(cudaStream_t s, const ForwardArgs& a, int warps) {
+  auto* kernel = norm_forward_kernel<VPT, 0, ODD, FUSED, true>;
+  constexpr int kWarpBytes = (FUSED ? 2 : 1) * 32 * VPT * 16;
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostWarps * kWarpBytes);
+    if (dev >= 0 && dev < 64) attr_done[dev] = true;
+  }
+  const int64_t grid = std::min<int64_t>(a.rows, std::max(1, 16 / warps) * sm_count());
+  kernel<<<static_cast<unsigned>(grid), 32 * warps, warps * kWarpBytes, s>>>(a);
+}
+
+constexpr int kStagedWarps = 9;  // rows whose blocks an SM holds one of
 
 template <int VPT, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
   const int warps = static_cast<int>(ceil_div(words, 32 * VPT));
   if constexpr (VPT < 8) {
     launch_forward<VPT, 1, FUSED>(s, a, 1, odd);
-  } else if constexpr (VPT == 16 && FUSED) {  // rows of 9 warps and more
-    launch_forward<VPT, 0, FUSED>(s, a, warps, odd);
   } else {
-    if (warps == 1) launch_forward<VPT, 1, FUSED>(s, a, warps, odd);
+    if (warps >= kStagedWarps) odd ? launch_staged<VPT, true, FUSED>(s, a, warps) : launch_staged<VPT, false, FUSED>(s, a, warps);
+    else if (warps == 1) launch_forward<VPT, 1, FUSED>(s, a, warps, odd);
     else if (warps == 2) launch_forward<VPT, 2, FUSED>(s, a, warps, odd);
     else if (warps == 4) launch_forward<VPT, 4, FUSED>(s, a, warps, odd);
     else launch_forward<VPT, 0, FUSED>(s, a, warps, odd);
@@ -722,7 +764,7 @@ void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool od
   else if (words <= 64) launch_forward<2, FUSED>(s, a, words, odd);
   else if (words <= 128) launch_forward<4, FUSED>(s, a, words, odd);
   else if (words <= 4096 && !many) launch_forward<8, FUSED>(s, a, words, odd);
-  else launch_forward<16, FUSED>(s, a, words, odd);
+  else if constexpr (!FUSED) launch_forward<16, FUSED>(s, a, words, odd);
 }
 
 // Blocks (or clusters) that the backward kernel runs as: what the machine holds at a time, no
@@ -849,6 +891,12 @@ extern "C" int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* inp
     return launch_status("layer norm forward");
   }
   const bool odd = cols % 4 != 0 || !aligned(weight) || !aligned(bias);
+  if (a.total && words > 4096) {
+    // a row of two inputs would fill an SM's shared memory: the total by itself, then its norm
+    launch_dropout(s, input, residual, total, rows * cols, a.drop);
+    a.x = total, a.residual = nullptr, a.total = nullptr;
+    a.drop.threshold = 0;
+  }
   if (a.total) launch_forward<true>(s, a, words, odd);
   else launch_forward<false>(s, a, words, odd);
   return launch_status("layer norm forward");
