@@ -233,6 +233,14 @@ __device__ __forceinline__ Record get(const Record* p) {
   return r;
 }
 
+// Nothing is known at the start, and the ticket after the last record is 0.
+__global__ void __launch_bounds__(256) clear_records_kernel(uint4* records, int64_t count) {
+  dependents_may_launch();
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += stride)
+    records[i] = make_uint4(0, 0, 0, 0);
+}
+
 // The state that enters chunk `chunk` > 0 of a chain, a lane to a channel; `start` is the
 // sequence's, `mine` the lane's record of the chunk. Looks at kLook chunks at a time.
 constexpr int kLook = 8;
@@ -503,6 +511,8 @@ scan_forward_kernel(Args a, Scan sc, int* err) {
   static_assert(kRing >= 3 && kRing + 3 <= 8, "a chunk's line is set before it is read, and kept until it is done");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
+  if (!WHOLE) wait_for_prior_grid();  // the records are clear
+
   if (warp == kWarps + 1) {  // the teller
     for (int k = 0; k < kRing; ++k) __syncthreads();
     for (unsigned i = 0;; ++i) {
@@ -719,6 +729,7 @@ scan_backward_kernel(Args a, Scan sc, int* err) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
+  wait_for_prior_grid();  // the records are clear
   if (threadIdx.x == 0) line[0] = tile_of<true, false>(a, sc, atomicAdd(sc.ticket, 1u));
   __syncthreads();
   fetch(line[0]);
@@ -843,9 +854,15 @@ int launch_scan(cudaStream_t s, const Args& a, int threads, int bytes, int per_s
       return launch_status("recurrence shared memory attribute");
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
-  if (!whole) cudaMemsetAsync(workspace, 0, tiles * kWide * sizeof(Record) + sizeof(unsigned), s);
-  const int64_t grid = std::min<int64_t>(whole ? sc.chains : tiles, per_sm * sm_count());
-  kKernel<<<static_cast<unsigned>(grid), threads, bytes, s>>>(a, sc, device_error_word());
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(whole ? sc.chains : tiles, per_sm * sm_count())));
+  if (whole) {
+    kKernel<<<grid, threads, bytes, s>>>(a, sc, device_error_word());
+  } else {
+    const int64_t records = tiles * kWide + 1;
+    clear_records_kernel<<<static_cast<unsigned>(std::min<int64_t>(ceil_div(records, 256), 8 * sm_count())), 256, 0, s>>>(
+        reinterpret_cast<uint4*>(workspace), records);
+    launch_after(kKernel, grid, dim3(threads), s, bytes, a, sc, device_error_word());
+  }
   return launch_status("recurrence");
 }
 
@@ -916,9 +933,9 @@ using namespace tcx;
 
 extern "C" size_t tcx_sm100_recurrence_workspace_bytes(int64_t batch, int64_t time, int64_t channels) {
   if (check_recurrence(TCX_RECURRENCE_DECAY, batch, time, channels) || time <= kWalkSteps) return 0;
-  // a record per channel for each chunk, and the ticket
+  // a record per channel for each chunk, and the ticket in one more's place
   const int64_t tiles = batch * ceil_div(channels, kWide) * ceil_div(time, kChunk);
-  return static_cast<size_t>(tiles) * kWide * sizeof(Record) + sizeof(unsigned);
+  return (static_cast<size_t>(tiles) * kWide + 1) * sizeof(Record);
 }
 
 extern "C" int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const float* gate, const float* x,
