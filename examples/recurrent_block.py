@@ -57,7 +57,8 @@ class RecurrentBlock:
         the dropout mask in the seed's stream; None (serving) drops nothing."""
         w, k = self.params, {}
         k["u"], k["state"], k["lengths"] = u, state, lengths
-        k["p"], k["offset"] = (0.0, 0) if step is None else (self.p, step * u.shape[0] * u.shape[1] * w["w_in"].shape[0])
+        width = w["w_in"].shape[0]
+        k["p"], k["offset"] = (0.0, 0) if step is None else (self.p, step * u.shape[0] * u.shape[1] * width)
         x = ops.linear(u, w["w_in"])
         k["n"], _, k["m1"], k["r1"] = ops.layernorm_forward(x, w["n1_w"], w["n1_b"])
         k["gate"] = ops.linear(k["n"], w["w_gate"], w["b_gate"])

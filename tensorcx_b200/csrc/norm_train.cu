@@ -12,7 +12,15 @@
 // The mean is taken about the row's first element f and corrected about its own first value:
 // m1 = f + sum(x - f) / n, mean = m1 + sum(x - m1) / n, and the variance is
 // sum((x - m1)^2) / n - (sum(x - m1) / n)^2. A constant row then has mean f and variance 0
-// exactly, and a row whose level is far above its spread loses nothing in the sum.
+// exactly, and a row whose level is far above its spread loses nothing in the sum. (With a
+// dropout in front f is the residual's first element.) All sums are float32.
+//
+// Bound by memory: 8 bytes an element forward and 12 backward, 16 and 20 with the dropout and
+// the residual. Measured on one B200 (those bytes over the call's time, against a copy's 6.55
+// TB/s): [16384, 4096] forward 92 us (0.89), with dropout and residual 170 us (0.96), backward
+// 131 us (0.94; its first kernel 120 us), with dropout and residual 216 us (0.95); [16383, 4095]
+// with both forward 202 us (0.81), backward plain 162 us (0.76); [2048, 32768] backward 158 us
+// (0.78), forward 119 us (0.69); [65536, 256] backward 42 us (0.73).
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -29,6 +37,10 @@ namespace {
 
 using rowmath::Block;
 
+// ------------------------------------------------------------------------ any row
+// For buffers that are not 16-byte aligned and rows longer than the kernels below hold (32768
+// forward, 65536 backward): an element to a thread, a row's block reading it again for each
+// of its sums and once more for its outputs, and the columns' sums in a pass of their own.
 constexpr int kThreads = 256;
 
 struct ForwardArgs {
@@ -145,19 +157,6 @@ __global__ void __launch_bounds__(kThreads) norm_columns_kernel(BackwardArgs a, 
   }
   partial[(2 * blockIdx.y) * a.cols + c] = dw;
   partial[(2 * blockIdx.y + 1) * a.cols + c] = db;
-}
-
-__global__ void __launch_bounds__(kThreads)
-norm_columns_join_kernel(const float* partial, int64_t splits, int64_t cols, float* dweight, float* dbias) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (c >= cols) return;
-  float dw = 0.0f, db = 0.0f;
-  for (int64_t i = 0; i < splits; ++i) {
-    dw += partial[2 * i * cols + c];
-    db += partial[(2 * i + 1) * cols + c];
-  }
-  dweight[c] = dw;
-  dbias[c] = db;
 }
 
 // ------------------------------------------------------------------ rows in registers
@@ -299,11 +298,12 @@ norm_forward_kernel(ForwardArgs a) {
       const uint64_t start = a.drop.threshold ? dropout_start(a.drop) : 0;
       if (a.drop.threshold) {
         // the mask while the loads are on their way: 4 bits to a word
+        const uint64_t place_0 = start + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(mine);
         uint32_t mask[(VPT + 7) / 8];
 #pragma unroll
         for (int k = 0; k < VPT; k += 8)
-          mask[k / 8] = kept_words<(VPT < 8 ? VPT : 8)>(
-              start + static_cast<uint64_t>(words.at) + 4 * static_cast<uint64_t>(mine + 32 * k), 32, rk, a.drop.threshold);
+          mask[k / 8] =
+              kept_words<(VPT < 8 ? VPT : 8)>(place_0 + 128 * static_cast<uint64_t>(k), 32, rk, a.drop.threshold);
 #pragma unroll
         for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -325,7 +325,8 @@ norm_forward_kernel(ForwardArgs a) {
       }
       if (ODD && loose) {
         if (a.drop.threshold)
-          one = dropped(one, kept_place(start + static_cast<uint64_t>(first + column), rk, a.drop.threshold), a.drop.scale);
+          one = dropped(one, kept_place(start + static_cast<uint64_t>(first + column), rk, a.drop.threshold),
+                        a.drop.scale);
         if (a.residual) one = __fadd_rn(__ldcs(a.residual + first + column), one);
         a.total[first + column] = one;
       }
@@ -384,11 +385,16 @@ norm_forward_kernel(ForwardArgs a) {
   }
 }
 
+// The gradient. Its floor is one pass over dy and total, so a row stays with its block between
+// its sums and its gradient, and the columns' sums are taken on the way: [16384, 4096] took
+// 484 us with passes of their own for those.
+//
 // Some warps of a block (of each of CLUSTER blocks) to a row, VPT words to a thread, and several
-// rows to a block at a time where they are short, a group of warps to each. A group's rows are a multiple of 4 apart, so that they
-// all start at the same place of a word and a thread's columns are the same in each: the weight's and the
-// bias's gradients add up in its registers over the group's rows, the groups' in shared memory,
-// and the blocks' in a second kernel, each in a fixed order.
+// rows to a block at a time where they are short, a group of warps to each. A group's rows are
+// a multiple of 4 apart, so that they all start at the same place of a word and a thread's
+// columns are the same in each: the weight's and the bias's gradients add up in its registers
+// over the group's rows, the groups' in shared memory, and the blocks' in a second kernel, each
+// in a fixed order.
 //
 // dy and total come through a ring of places in shared memory (cp.async; a thread copies and
 // reads its own words only, so that needs no barrier): a place is copied into again as soon as
@@ -396,7 +402,13 @@ norm_forward_kernel(ForwardArgs a) {
 // rows, dtotal has two places of its own, in use until the row's gradient is stored, and the
 // ring one less ([8191, 1001]: 60 -> 50 us); a longer row's is loaded when its turn comes
 // ([16384, 4096]: 216 us against 250). The weight lies beside the places where its words are
-// not aligned or the block's rows share them; else it is read through the first-level cache.
+// not aligned or the block's rows share them; else it is read through the first-level cache
+// ([8192, 8192]: 157 us against 169). 16 warps of 128 registers and three rows' places to an SM:
+// two places, and 24 warps of 85 registers, took 140 us for [16384, 4096] against 134.
+//
+// Rows of more than 4096 go to a cluster: its blocks' sums cross by st.async, and there are as
+// many clusters as the device holds at a time (33 of 8 blocks: a few more and their rows came
+// in a second round, 245 us against 154 for [2048, 32768]).
 
 // Warps to an SM: 128 registers a thread, or 64 where it holds one word of each array.
 constexpr int warps_per_sm(int vpt) { return vpt == 1 ? 32 : 16; }
@@ -747,7 +759,8 @@ void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool od
   if constexpr (VPT < 8) {
     launch_forward<VPT, 1, FUSED>(s, a, 1, odd);
   } else {
-    if (warps >= kStagedWarps) odd ? launch_staged<VPT, true, FUSED>(s, a, warps) : launch_staged<VPT, false, FUSED>(s, a, warps);
+    if (warps >= kStagedWarps && odd) launch_staged<VPT, true, FUSED>(s, a, warps);
+    else if (warps >= kStagedWarps) launch_staged<VPT, false, FUSED>(s, a, warps);
     else if (warps == 1) launch_forward<VPT, 1, FUSED>(s, a, warps, odd);
     else if (warps == 2) launch_forward<VPT, 2, FUSED>(s, a, warps, odd);
     else if (warps == 4) launch_forward<VPT, 4, FUSED>(s, a, warps, odd);
@@ -935,7 +948,7 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
   if (!dy || !total || !mean || !rstd || !dresidual) return invalid("missing buffer");
   if (a.drop.threshold && !dx) return invalid("dropout needs a buffer for the input's gradient");
   if (!a.drop.threshold) a.dx = nullptr;  // it is the residual's gradient
-  if (dweight && workspace_bytes < tcx_sm100_layernorm_backward_workspace_bytes(rows, cols))
+  if (dweight && (!workspace || workspace_bytes < tcx_sm100_layernorm_backward_workspace_bytes(rows, cols)))
     return invalid("workspace too small for the layer norm gradient");
   TimedLaunch timer("norm_backward", s);
   float* partial = dweight ? static_cast<float*>(workspace) : nullptr;
@@ -954,7 +967,8 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
     const unsigned blocks = static_cast<unsigned>(ceil_div(cols, kThreads));
     norm_columns_kernel<<<dim3(blocks, static_cast<unsigned>(splits)), kThreads, 0, s>>>(a, partial,
                                                                                          ceil_div(rows, splits));
-    norm_columns_join_kernel<<<blocks, kThreads, 0, s>>>(partial, splits, cols, dweight, dbias);
+    norm_join_kernel<<<static_cast<unsigned>(ceil_div(cols, 32)), 1024, 0, s>>>(partial, static_cast<int>(splits), cols,
+                                                                                dweight, dbias);
   }
   return launch_status("layer norm backward");
 }

@@ -167,8 +167,8 @@ def check_forward(y, mean, rstd, total, w, b, eps):
     hat = (t - m[..., None]) * r[..., None]
     wd = np.ones(n) if w is None else np.abs(w.astype(np.float64))
     want = hat * (1 if w is None else w.astype(np.float64)) + (0 if b is None else b.astype(np.float64))
-    bound = wd * (off_mean[..., None] * r[..., None] + np.abs(hat) * (rel_r[..., None] + 4 * U)) + 2 * U * np.abs(want) \
-        + 2 * U * (0 if b is None else np.abs(b.astype(np.float64)))
+    bound = wd * (off_mean[..., None] * r[..., None] + np.abs(hat) * (rel_r[..., None] + 4 * U))
+    bound = bound + 2 * U * np.abs(want) + 2 * U * (0 if b is None else np.abs(b.astype(np.float64)))
     within(y, want, bound, "y")
 
 
@@ -269,8 +269,8 @@ def check_backward(tcx, oracle, dy, total, mean, rstd, w, dtotal, p, seed, offse
     if p:
         keep = keep_of(oracle, dy.shape, p, seed, offset)
         scale = float(scale_of(p))
-        within(host(dx), np.where(keep, want * scale, 0), np.where(keep, bound * scale + 2 * U * np.abs(want) * scale, 0),
-               "dx")
+        within(host(dx), np.where(keep, want * scale, 0),
+               np.where(keep, bound * scale + 2 * U * np.abs(want) * scale, 0), "dx")
     else:
         assert dx is dres
     if w is None:
@@ -306,6 +306,20 @@ def test_norm_backward_many_rows(tcx, oracle, rows, cols):
     assert all(a.tobytes() == b.tobytes() for a, b in zip(first, again))
 
 
+@pytest.mark.parametrize("rows,cols", [(310, 16500), (160, 20001), (200, 16384), (90, 33001)])
+def test_norm_long_rows_in_turn(tcx, oracle, rows, cols):
+    """More long rows than run at a time: a block, or a cluster of them, takes several."""
+    x, r, w, b = norm_case(rows, cols, True, seed=3)
+    y, total, mean, rstd = tcx.layernorm_forward(dev(x), dev(w), dev(b))
+    check_forward(host(y), host(mean), host(rstd), x, w, b, 1e-5)
+    y, total, mean, rstd = tcx.layernorm_forward(dev(x), dev(w), dev(b), residual=dev(r), p=0.5, seed=9, offset=1)
+    want = r + np.where(keep_of(oracle, x.shape, 0.5, 9, 1), x * 2, np.float32(0)).astype(np.float32)
+    assert host(total).tobytes() == want.tobytes()
+    check_forward(host(y), host(mean), host(rstd), want, w, b, 1e-5)
+    dy = np.random.default_rng(rows).normal(size=x.shape).astype(np.float32)
+    check_backward(tcx, oracle, dy, want, host(mean), host(rstd), w, x, 0.5, 9, 1)
+
+
 @pytest.mark.parametrize("cols", [3, 130])
 def test_norm_gradient_against_differences(tcx, oracle, cols):
     """The kernels' gradients along a direction against central differences of the 64-bit
@@ -336,8 +350,8 @@ def test_norm_gradient_against_differences(tcx, oracle, cols):
 
 
 # ----------------------------------------------------------------------- recurrence
-RSHAPES = [(1, 1, 1), (3, 1, 5), (5, 1, 1001), (300, 1, 64), (2, 2, 3), (2, 5, 3), (1, 7, 128), (4, 17, 260), (1, 64, 128), (3, 65, 130),
-           (2, 257, 33), (1, 300, 1024), (1, 1000, 256), (2, 1025, 68), (1, 5000, 4), (9, 129, 512), (1, 2049, 127),
+RSHAPES = [(1, 1, 1), (3, 1, 5), (5, 1, 1001), (300, 1, 64), (2, 2, 3), (2, 5, 3), (1, 7, 128), (4, 17, 260),
+           (1, 64, 128), (3, 65, 130), (2, 257, 33), (1, 300, 1024), (1, 1000, 256), (2, 1025, 68), (1, 5000, 4), (9, 129, 512), (1, 2049, 127),
            (70, 33, 1000)]
 
 
@@ -459,6 +473,22 @@ def test_recurrence_lengths(tcx, form, time, channels):
     for b, n in enumerate(np.clip(lengths, 0, time)):
         held = h[b, n - 1] if n else init[b]
         assert (h[b, n:] == held).all() and (host(state)[b] == (h[b, -1])).all()
+
+
+@pytest.mark.parametrize("form", ["decay", "sigmoid"])
+@pytest.mark.parametrize("batch,time,channels", [(300, 300, 20), (250, 140, 21), (300, 40, 600), (700, 100, 301)])
+def test_recurrence_many_sequences(tcx, form, batch, time, channels):
+    """Enough sequences to fill the machine, of different lengths: whole ones to a block, or a
+    thread to a channel."""
+    gate, x, init, dh, dstate = recurrence_case(batch, time, channels, form, seed=6)
+    lengths = np.random.default_rng(batch).integers(-1, time + 2, batch)
+    pad = ~live_steps(batch, time, lengths)
+    gate[pad], x[pad] = np.nan, np.inf
+    check_recurrence(tcx, gate, x, init, dh, dstate, form, lengths)
+    h, _ = tcx.gated_recurrence(dev(gate), dev(x), dev(init), form=form, lengths=dev(lengths.astype(np.int32)))
+    h = host(h)
+    for b, n in enumerate(np.clip(lengths, 0, time)):
+        assert (h[b, n:] == (h[b, n - 1] if n else init[b])).all()
 
 
 @pytest.mark.parametrize("shift", [1, 2, 3])

@@ -15,7 +15,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 @pytest.fixture(scope="module")
 def example(tcx):
-    spec = importlib.util.spec_from_file_location("recurrent_block", os.path.join(ROOT, "examples", "recurrent_block.py"))
+    path = os.path.join(ROOT, "examples", "recurrent_block.py")
+    spec = importlib.util.spec_from_file_location("recurrent_block", path)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
     return module

@@ -20,9 +20,9 @@ def norm_back(dx=B, dw=B, db=B, rows=4, cols=8, p=0.0, ws=None, ws_bytes=0, dres
                                                    None, ws, ws_bytes)
 
 
-def rec(form=0, gate=B, h=B, batch=2, time=3, channels=4):
-    return _abi.lib().tcx_sm100_recurrence_forward(None, form, gate, B, None, None, h, None, batch, time, channels, None,
-                                                   0)
+def rec(form=0, gate=B, h=B, batch=2, time=3, channels=4, ws=None, ws_bytes=0):
+    return _abi.lib().tcx_sm100_recurrence_forward(None, form, gate, B, None, None, h, None, batch, time, channels, ws,
+                                                   ws_bytes)
 
 
 def rec_back(form=0, x=B, h=B, dx=B, batch=2, time=3, channels=4):
@@ -35,8 +35,8 @@ def drop(x=B, out=B, count=4, p=0.5):
 
 
 @pytest.mark.parametrize("call,word", [
-    (lambda: drop(count=-1), b"negative"), (lambda: drop(p=-0.1), b"probability"), (lambda: drop(p=1.1), b"probability"),
-    (lambda: drop(p=NAN), b"probability"), (lambda: drop(x=None), b"buffer"), (lambda: drop(out=None), b"buffer"),
+    (lambda: drop(count=-1), b"negative"), (lambda: drop(p=-0.1), b"probability"),
+    (lambda: drop(p=1.1), b"probability"), (lambda: drop(p=NAN), b"probability"), (lambda: drop(x=None), b"buffer"), (lambda: drop(out=None), b"buffer"),
     (lambda: norm(rows=-1), b"negative"), (lambda: norm(cols=0), b"non-empty"), (lambda: norm(eps=-1.0), b"epsilon"),
     (lambda: norm(eps=NAN), b"epsilon"), (lambda: norm(eps=INF), b"epsilon"), (lambda: norm(p=2.0), b"probability"),
     (lambda: norm(x=None), b"buffer"), (lambda: norm(mean=None), b"buffer"),
@@ -45,6 +45,9 @@ def drop(x=B, out=B, count=4, p=0.5):
     (lambda: norm_back(rows=-1), b"negative"), (lambda: norm_back(db=None), b"together"),
     (lambda: norm_back(dx=None, p=0.5), b"dropout"), (lambda: norm_back(dres=None), b"buffer"),
     (lambda: norm_back(p=NAN), b"probability"), (lambda: norm_back(), b"workspace"),
+    (lambda: norm_back(ws_bytes=1 << 30), b"workspace"), (lambda: rec(time=300), b"workspace"),
+    (lambda: rec(time=300, ws_bytes=1 << 30), b"workspace"),
+    (lambda: rec(time=300, ws=ctypes.c_void_p(1028), ws_bytes=1 << 30), b"aligned"),
     (lambda: rec(form=2), b"form"), (lambda: rec(batch=-1), b"negative"), (lambda: rec(gate=None), b"buffer"),
     (lambda: rec(h=None), b"buffer"), (lambda: rec(batch=1 << 30, time=1 << 30, channels=1 << 30), b"overflows"),
     (lambda: rec_back(form=-1), b"form"), (lambda: rec_back(form=1, x=None), b"needs x"),
