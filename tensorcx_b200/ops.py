@@ -737,6 +737,13 @@ def _at(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _row_values(x, shape):
+    """An empty tensor with a value for each row of x (of its shape without the last axis)."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape[:1], (1,), dtype=_float32, device=x.device)
+    return x.new_empty(shape[:-1])
+
+
 def _dropout_stream(p, seed, offset, index):
     """(p, seed, offset, address of a device-side offset) as the C ABI takes them."""
     if type(p) is not float:
@@ -800,7 +807,7 @@ def layernorm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias:
     p, seed, offset, step = _dropout_stream(p, seed, offset, index)
     y = _new_like(x)
     total = _new_like(x) if residual is not None or p > 0.0 else None
-    mean = x.new_empty(shape[:-1])
+    mean = _row_values(x, shape)
     rstd = _new_like(mean)
     check(lib().tcx_sm100_layernorm_forward(
         _raw(index), x.data_ptr(), _at(residual), _at(weight), _at(bias), y.data_ptr(), _at(total), mean.data_ptr(),
@@ -861,9 +868,9 @@ def _recurrence_args(gate, form, lengths, *named):
 
 
 def _recurrence_workspace(shape, device):
-    ws_bytes = 0
-    if shape[1] > 1:  # a single step needs none
-        ws_bytes = lib().tcx_sm100_recurrence_workspace_bytes(*shape)
+    if shape[1] == 1:  # a single step needs none
+        return None, None, 0
+    ws_bytes = lib().tcx_sm100_recurrence_workspace_bytes(*shape)
     return *_workspace(ws_bytes, device), ws_bytes
 
 
