@@ -8,7 +8,7 @@ clip 858-876) and the primitive dispatch of CudaBackend::execute
 Every op calls the C ABI (tensorcx_b200._abi) on torch's current stream; outputs are
 fresh contiguous tensors, and workspace comes from torch's stream-ordered caching
 allocator. Ops are asynchronous like torch ops; call torch.cuda.synchronize() (or
-.cpu()) to observe results.
+.cpu()) to observe results. The training operators at the end have no counterpart there.
 """
 from __future__ import annotations
 
