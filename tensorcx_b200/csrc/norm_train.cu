@@ -692,35 +692,37 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   }
 }
 
-// Adds the blocks' column sums: a block to 32 columns, a warp to every 32nd of the partial
-// rows, then the warps in order.
-__global__ void __launch_bounds__(1024)
+// Adds the blocks' column sums: a block to 32 columns, a warp to every WARPS-th of the partial
+// rows, then the warps in order. 32 warps for many partial rows, 8 for few.
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS)
 norm_join_kernel(const float* __restrict__ partial, int splits, int64_t cols, float* dweight, float* dbias) {
-  __shared__ float2 sums[32][33];
+  __shared__ float2 sums[WARPS][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   wait_for_prior_grid();
   float2 s = make_float2(0.0f, 0.0f);
   if (c < cols) {
-#pragma unroll 8
-    for (int i = warp; i < splits; i += 32) {
+#pragma unroll 5
+    for (int i = warp; i < splits; i += WARPS) {
       s.x += __ldcg(partial + 2 * i * cols + c);
       s.y += __ldcg(partial + (2 * i + 1) * cols + c);
     }
   }
   sums[warp][lane] = s;
   __syncthreads();
-  s = sums[lane][warp];
+  if (warp < 2 && c < cols) {  // a warp to each gradient
+    float t = 0.0f;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    s.x += __shfl_xor_sync(0xffffffffu, s.x, off);
-    s.y += __shfl_xor_sync(0xffffffffu, s.y, off);
+    for (int w = 0; w < WARPS; ++w) t += warp ? sums[w][lane].y : sums[w][lane].x;
+    (warp ? dbias : dweight)[c] = t;
   }
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + warp;
-  if (lane == 0 && column < cols) {
-    dweight[column] = s.x;
-    dbias[column] = s.y;
-  }
+}
+
+void join_columns(cudaStream_t s, const float* partial, int64_t splits, int64_t cols, float* dweight, float* dbias) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(cols, 32)));
+  if (splits > 64) launch_after(norm_join_kernel<32>, grid, dim3(1024), s, 0, partial, splits, cols, dweight, dbias);
+  else launch_after(norm_join_kernel<8>, grid, dim3(256), s, 0, partial, splits, cols, dweight, dbias);
 }
 
 // ------------------------------------------------------------------------- launches
@@ -955,9 +957,7 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
   const BackwardPlan plan = backward_plan(cols);
   if (plan.vpt && aligned(dy) && aligned(total) && aligned(dtotal) && aligned(dresidual) && aligned(a.dx)) {
     const int64_t splits = launch_backward(s, a, partial, plan, cols % 4 != 0 || !aligned(weight));
-    if (partial)
-      launch_after(norm_join_kernel, dim3(static_cast<unsigned>(ceil_div(cols, 32))), dim3(1024), s, 0, partial,
-                   static_cast<int>(splits), cols, dweight, dbias);
+    if (partial) join_columns(s, partial, splits, cols, dweight, dbias);
     return launch_status("layer norm backward");
   }
   const int grid = static_cast<int>(std::min<int64_t>(rows, 8 * sm_count()));
@@ -967,8 +967,7 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
     const unsigned blocks = static_cast<unsigned>(ceil_div(cols, kThreads));
     norm_columns_kernel<<<dim3(blocks, static_cast<unsigned>(splits)), kThreads, 0, s>>>(a, partial,
                                                                                          ceil_div(rows, splits));
-    norm_join_kernel<<<static_cast<unsigned>(ceil_div(cols, 32)), 1024, 0, s>>>(partial, static_cast<int>(splits), cols,
-                                                                                dweight, dbias);
+    join_columns(s, partial, splits, cols, dweight, dbias);
   }
   return launch_status("layer norm backward");
 }
