@@ -17,9 +17,9 @@
 //
 // Bound by memory: 8 bytes an element forward and 12 backward, 16 and 20 with the dropout and
 // the residual. Measured on one B200 (those bytes over the call's time, against a copy's 6.55
-// TB/s): [16384, 4096] forward 92 us (0.89), with dropout and residual 170 us (0.96), backward
+// TB/s): [16384, 4096] forward 88 us (0.93), with dropout and residual 170 us (0.96), backward
 // 131 us (0.94; its first kernel 120 us), with dropout and residual 216 us (0.95); [16383, 4095]
-// with both forward 202 us (0.81), backward plain 162 us (0.76); [2048, 32768] backward 158 us
+// with both forward 202 us (0.81), backward plain 162 us (0.76); [2048, 32768] backward 157 us
 // (0.78), forward 119 us (0.69); [65536, 256] backward 42 us (0.73).
 #include <cuda_runtime.h>
 #include <math.h>
@@ -406,9 +406,11 @@ norm_forward_kernel(ForwardArgs a) {
 // ([8192, 8192]: 157 us against 169). 16 warps of 128 registers and three rows' places to an SM:
 // two places, and 24 warps of 85 registers, took 140 us for [16384, 4096] against 134.
 //
-// Rows of more than 4096 go to a cluster: its blocks' sums cross by st.async, and there are as
-// many clusters as the device holds at a time (33 of 8 blocks: a few more and their rows came
-// in a second round, 245 us against 154 for [2048, 32768]).
+// Rows of more than 4096 take up to 16 warps of one block, one to an SM ([8192, 8192]: 132 us
+// against 157 as two blocks of 8 warps); longer ones go to a cluster of blocks of 8: its blocks'
+// sums cross by st.async, and there are as many clusters as the device holds at a time (33 of 8
+// blocks: a few more and their rows came in a second round, 245 us against 154 for [2048,
+// 32768]; 4 blocks of 16 warps took 179).
 
 // Warps to an SM: 128 registers a thread, or 64 where it holds one word of each array.
 constexpr int warps_per_sm(int vpt) { return vpt == 1 ? 32 : 16; }
@@ -770,11 +772,16 @@ void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool od
   }
 }
 
-// Small blocks of many words: up to 64 values to a thread, or 32 of each of two inputs. Rows
-// that leave more than an eighth of the places of 16 words to a thread empty take 8.
+// 32 values to a thread, of each of two inputs where there are two. Where there are rows to
+// fill the machine a dozen times, 64 of one input in half as many warps: rows of 257 to 384
+// words, which leave one warp no block to wait for ([40000, 1100]: 66 us against 76; [50000,
+// 800] 67 against 56), and rows of 7 warps and more, of which an SM then holds twice as many
+// ([8192, 8191]: 121 us against 150; [8192, 8400] 111 against 184; [16384, 4096] 92 against 88).
+// Fewer rows finish sooner with more warps to each ([148, 8192]: 12 us against 16).
 template <bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
-  const bool many = !FUSED && words * 8 >= ceil_div(words, 512) * 512 * 7;
+  const bool many = !FUSED && (words > 1536 || (words > 256 && words <= 384)) &&
+                    a.rows >= 12 * static_cast<int64_t>(sm_count());
   if (words <= 32) launch_forward<1, FUSED>(s, a, words, odd);
   else if (words <= 64) launch_forward<2, FUSED>(s, a, words, odd);
   else if (words <= 128) launch_forward<4, FUSED>(s, a, words, odd);
@@ -801,7 +808,7 @@ BackwardPlan backward_plan(int64_t cols) {
   BackwardPlan plan;
   plan.vpt = words <= 32 ? 1 : words <= 64 ? 2 : 4;
   const int warps = static_cast<int>(ceil_div(words, 32 * plan.vpt));
-  plan.cluster = warps <= 8 ? 1 : warps <= 16 ? 2 : warps <= 32 ? 4 : 8;
+  plan.cluster = warps <= kMostWarps ? 1 : warps <= 32 ? 4 : 8;
   plan.warps = static_cast<int>(ceil_div(warps, plan.cluster));
   plan.groups = plan.warps == 1 || plan.warps == 2 || plan.warps == 4 ? 8 / plan.warps : 1;
   plan.per_sm = std::max(1, warps_per_sm(plan.vpt) / (plan.warps * plan.groups));
@@ -855,7 +862,6 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
 // Returns the partial rows that it leaves.
 int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd) {
   switch (plan.cluster) {
-    case 2: return launch_backward<4, 0, 2>(s, a, partial, plan, odd);
     case 4: return launch_backward<4, 0, 4>(s, a, partial, plan, odd);
     case 8: return launch_backward<4, 0, 8>(s, a, partial, plan, odd);
     default: break;

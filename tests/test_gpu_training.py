@@ -320,6 +320,12 @@ def test_norm_long_rows_in_turn(tcx, oracle, rows, cols):
     check_backward(tcx, oracle, dy, want, host(mean), host(rstd), w, x, 0.5, 9, 1)
 
 
+@pytest.mark.parametrize("rows,cols", [(310, 8192), (350, 6001), (1790, 6404), (1801, 1101), (1777, 8403)])
+def test_norm_many_middling_rows(tcx, oracle, rows, cols):
+    """Rows of one block, enough of them that fewer warps take more words of each."""
+    test_norm_long_rows_in_turn(tcx, oracle, rows, cols)
+
+
 @pytest.mark.parametrize("cols", [3, 130])
 def test_norm_gradient_against_differences(tcx, oracle, cols):
     """The kernels' gradients along a direction against central differences of the 64-bit
