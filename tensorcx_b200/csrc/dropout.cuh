@@ -65,25 +65,32 @@ __device__ __forceinline__ uint32_t kept_block(uint64_t block, const philox::Rou
          (kept(w.w, threshold) ? 8u : 0u);
 }
 
-// Bit 4 k + j: place e + 4 k stride + j is kept, k < WORDS (at most 8). For whole warps whose
-// lanes' places lie 4 apart. Where they do not start a block, a lane's words end in the next
-// lane's blocks, and the last lane's in WORDS blocks of which each lane makes one.
-template <int WORDS>
+// Bit 4 k + j: place e + 4 k stride + j is kept, k < WORDS (at most 8). For whole warps, the
+// places of whose LANES lanes (32, or each 16 or 8 of them) lie 4 apart. Where they do not start
+// a block, a lane's words end in the next lane's blocks, and the last lane's in WORDS blocks of
+// which each lane makes one. e must lie alike within a block for all lanes of the warp.
+template <int WORDS, int LANES = 32>
 __device__ __forceinline__ uint32_t kept_words(uint64_t e, uint32_t stride, const philox::RoundKeys& rk,
                                                uint32_t threshold) {
   static_assert(WORDS <= 8, "the mask's bits");
+  static_assert(WORDS <= LANES, "a lane to each of the last lane's blocks");
   const uint64_t block = e >> 2;
   const int r = static_cast<int>(e & 3);  // the same for all lanes
   uint32_t mask = 0;
 #pragma unroll
   for (int k = 0; k < WORDS; ++k) mask |= kept_block(block + k * stride, rk, threshold) << (4 * k);
   if (r == 0) return mask;
-  const int lane = threadIdx.x & 31;
-  uint32_t next = __shfl_down_sync(0xffffffffu, mask, 1), ends = 0;
-  const uint64_t after = __shfl_sync(0xffffffffu, block, 31) + 1;
+  const int lane = threadIdx.x & (LANES - 1);
+  uint32_t next = __shfl_down_sync(0xffffffffu, mask, 1, LANES), ends = 0;
+  const uint64_t after = __shfl_sync(0xffffffffu, block, LANES - 1, LANES) + 1;
   if (lane < WORDS) ends = kept_block(after + lane * stride, rk, threshold) << (4 * lane);
-  ends = __reduce_or_sync(0xffffffffu, ends);
-  if (lane == 31) next = ends;
+  if (LANES == 32) {
+    ends = __reduce_or_sync(0xffffffffu, ends);
+  } else {
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) ends |= __shfl_xor_sync(0xffffffffu, ends, off);
+  }
+  if (lane == LANES - 1) next = ends;
   // bits r .. 3 of each word's own block, then bits 0 .. r - 1 of the next one
   const uint32_t low = 0x11111111u * (0xfu >> r);
   return ((mask >> r) & low) | ((next << (4 - r)) & ~low);

@@ -166,14 +166,15 @@ __global__ void __launch_bounds__(kThreads) norm_columns_kernel(BackwardArgs a, 
 // wide, and a word of the tensor is a block of the random stream.
 template <bool ODD>
 struct Words {
-  int64_t at;             // of the first whole word in the tensor
+  int64_t at;             // of the first whole word in the tensor: a multiple of 4, words or none
   int head, words, tail;  // loose elements before the whole words, those, and loose elements after
 
   __device__ Words(int64_t row, int64_t n) {
     const int64_t first = row * n;
     const int cols = static_cast<int>(n);
-    head = ODD ? min(static_cast<int>(-first & 3), cols) : 0;
-    at = first + head;
+    const int ahead = ODD ? static_cast<int>(-first & 3) : 0;
+    at = first + ahead;
+    head = min(ahead, cols);
     words = (cols - head) >> 2;
     tail = ODD ? cols - head - 4 * words : 0;
   }
@@ -199,20 +200,24 @@ __device__ __forceinline__ bool kept_place(uint64_t e, const philox::RoundKeys& 
   return kept(word_of(philox::block_words(e >> 2, rk), static_cast<uint32_t>(e & 3)), threshold);
 }
 
-// Two sums over a warp in one butterfly: the lower lanes end with a's, the upper ones with b's.
-__device__ __forceinline__ float warp_sums(float a, float b) {
-  const bool upper = threadIdx.x & 16;
-  float s = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+// Two sums over LANES lanes in one butterfly: the lower half ends with a's, the upper with b's.
+template <int LANES>
+__device__ __forceinline__ float lane_sums(float a, float b) {
+  const bool upper = threadIdx.x & (LANES / 2);
+  float s = (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, LANES / 2);
 #pragma unroll
-  for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  for (int off = LANES / 4; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
   return s;
 }
 
-// Two sums over `warps` warps that share `smem` and the barrier; every thread receives them.
+// Two sums over `warps` warps that share `smem` and the barrier, or over LANES lanes of one;
+// every thread receives them.
+template <int LANES = 32>
 __device__ __forceinline__ float2 row_sums(float a, float b, float2* smem, int warps, int warp, int barrier) {
-  const float s = warp_sums(a, b);
+  const float s = lane_sums<LANES>(a, b);
   const int lane = threadIdx.x & 31;
-  if (warps == 1) return make_float2(__shfl_sync(0xffffffffu, s, 0), __shfl_sync(0xffffffffu, s, 16));
+  if (warps == 1)
+    return make_float2(__shfl_sync(0xffffffffu, s, 0, LANES), __shfl_sync(0xffffffffu, s, LANES / 2, LANES));
   if ((lane & 15) == 0) (lane ? smem[warp].y : smem[warp].x) = s;
   asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(32 * warps) : "memory");
   float2 sums = make_float2(0.0f, 0.0f);
@@ -227,19 +232,30 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* smem, int w
 
 // Kernels for a known number of warps to a row (WARPS), or any up to kMostWarps (0).
 constexpr int kMostWarps = 16;
-constexpr int most_threads(int warps) { return 32 * (warps ? warps : kMostWarps); }
+// Threads of a forward block at most, and of the blocks that an SM holds of them.
+constexpr int most_threads(int warps) { return 32 * (warps == 1 ? 2 : warps ? warps : kMostWarps); }
+constexpr int resident_threads(int vpt, bool fused) {
+  return fused ? (vpt < 4 ? 1024 : vpt < 8 ? 768 : 512) : vpt < 4 ? 1536 : vpt < 8 ? 1024 : 768;
+}
 
 // One block to a row, VPT words to a thread, as many warps as the row needs. Each element is
 // read once and written once; the statistics take two block reductions. STAGED: few blocks fit
 // an SM, so that each takes rows in turn, and the next row's words come into shared memory
 // (cp.async; a thread copies and reads its own only) while this one is worked on.
-template <int VPT, int WARPS, bool ODD, bool FUSED, bool STAGED>
-__global__ void __launch_bounds__(most_threads(WARPS), STAGED ? 1 : (FUSED ? 512 : 768) / most_threads(WARPS))
+// Rows of one warp or less (LANES lanes) share a block: with a block and a whole warp to each,
+// the starts of the blocks took [500000, 64] to 264 us against 56, [125000, 256] 72 against 47,
+// [600000, 33] with dropout and residual 459 against 117.
+template <int VPT, int WARPS, int LANES, bool ODD, bool FUSED, bool STAGED>
+__global__ void __launch_bounds__(most_threads(WARPS),
+                                  STAGED ? 1 : resident_threads(VPT, FUSED) / most_threads(WARPS))
 norm_forward_kernel(ForwardArgs a) {
+  static_assert(LANES == 32 || (WARPS == 1 && LANES >= 8), "a lane to each loose element");
+  constexpr bool SHARED = WARPS == 1;
   extern __shared__ __align__(16) float4 stage[];
   __shared__ float2 smem[2][kMostWarps];
-  const int warps = WARPS ? WARPS : blockDim.x >> 5, warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31, mine = warp * 32 * VPT + lane;  // its first word, of a warp's 32 VPT
+  const int warps = WARPS ? WARPS : blockDim.x >> 5, warp = SHARED ? 0 : threadIdx.x >> 5;
+  const int lane = threadIdx.x & (LANES - 1), mine = warp * 32 * VPT + lane;  // its first word, of a warp's 32 VPT
+  const int group = SHARED ? threadIdx.x / LANES : 0, groups = SHARED ? blockDim.x / LANES : 1;
   const float n = static_cast<float>(a.cols);
   const philox::RoundKeys rk = philox::round_keys(a.drop.key);
   float4* const place = stage + warp * (FUSED ? 2 : 1) * 32 * VPT + lane;
@@ -262,8 +278,12 @@ norm_forward_kernel(ForwardArgs a) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (STAGED) copy(blockIdx.x);
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const Words<ODD> words(row, a.cols);
+  for (int64_t first_row = static_cast<int64_t>(blockIdx.x) * groups; first_row < a.rows;
+       first_row += static_cast<int64_t>(gridDim.x) * groups) {
+    // past the last row, an empty one
+    const bool live = !SHARED || first_row + group < a.rows;
+    const int64_t row = live ? first_row + group : 0;
+    const Words<ODD> words(row, live ? a.cols : 0);
     float v[VPT][4];
     if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
     const int64_t first = row * a.cols;
@@ -277,7 +297,7 @@ norm_forward_kernel(ForwardArgs a) {
     float4 res[FUSED ? VPT : 1];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = mine + 32 * k;
+      const int word = mine + LANES * k;
       float4 t = make_float4(level, level, level, level);
       if (words.holds(word)) t = STAGED ? place[32 * k] : words.load(a.x, word);
       v[k][0] = t.x, v[k][1] = t.y, v[k][2] = t.z, v[k][3] = t.w;
@@ -285,8 +305,8 @@ norm_forward_kernel(ForwardArgs a) {
     if (FUSED && a.residual) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (words.holds(mine + 32 * k))
-          res[FUSED ? k : 0] = STAGED ? place[32 * (VPT + k)] : words.load(a.residual, mine + 32 * k);
+        if (words.holds(mine + LANES * k))
+          res[FUSED ? k : 0] = STAGED ? place[32 * (VPT + k)] : words.load(a.residual, mine + LANES * k);
     }
     if (STAGED) copy(row + gridDim.x);
     // a loose element, with `level` for none
@@ -303,7 +323,8 @@ norm_forward_kernel(ForwardArgs a) {
 #pragma unroll
         for (int k = 0; k < VPT; k += 8)
           mask[k / 8] =
-              kept_words<(VPT < 8 ? VPT : 8)>(place_0 + 128 * static_cast<uint64_t>(k), 32, rk, a.drop.threshold);
+              kept_words<(VPT < 8 ? VPT : 8), LANES>(place_0 + 4 * LANES * static_cast<uint64_t>(k), LANES, rk,
+                                                     a.drop.threshold);
 #pragma unroll
         for (int k = 0; k < VPT; ++k)
 #pragma unroll
@@ -311,7 +332,7 @@ norm_forward_kernel(ForwardArgs a) {
       }
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
-        const int word = mine + 32 * k;
+        const int word = mine + LANES * k;
         if (words.holds(word)) {
           if (a.residual) {
             const float4 r = res[FUSED ? k : 0];
@@ -336,12 +357,12 @@ norm_forward_kernel(ForwardArgs a) {
     for (int k = 0; k < VPT; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s += v[k][j] - level;
-    const float m1 = level + __fdiv_rn(row_sums(s, 0.0f, smem[0], warps, warp, 0).x, n);
+    const float m1 = level + __fdiv_rn(row_sums<LANES>(s, 0.0f, smem[0], warps, warp, 0).x, n);
     one = ODD && loose ? one - m1 : 0.0f;
     float s1 = one, s2 = one * one;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      if (words.holds(mine + 32 * k)) {
+      if (words.holds(mine + LANES * k)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           v[k][j] -= m1;
@@ -350,14 +371,14 @@ norm_forward_kernel(ForwardArgs a) {
         }
       }
     }
-    const float2 r = row_sums(s1, s2, smem[1], warps, warp, 0);
+    const float2 r = row_sums<LANES>(s1, s2, smem[1], warps, warp, 0);
     const float shift = __fdiv_rn(r.x, n);
     float var = __fdiv_rn(r.y, n) - shift * shift;
     if (var < 0.0f) var = 0.0f;  // rounding; a NaN stays one
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(var + a.eps));
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = mine + 32 * k;
+      const int word = mine + LANES * k;
       if (words.holds(word)) {
         float4 y = make_float4((v[k][0] - shift) * rstd, (v[k][1] - shift) * rstd, (v[k][2] - shift) * rstd,
                                (v[k][3] - shift) * rstd);
@@ -378,7 +399,7 @@ norm_forward_kernel(ForwardArgs a) {
       if (a.bias) y += __ldg(a.bias + column);
       a.y[first + column] = y;
     }
-    if (threadIdx.x == 0) {
+    if (SHARED ? live && lane == 0 : threadIdx.x == 0) {
       a.mean[row] = m1 + shift;
       a.rstd[row] = rstd;
     }
@@ -733,16 +754,20 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 // Whole words of a row, at most.
 int64_t words_of(int64_t cols) { return std::max<int64_t>(1, cols / 4); }
 
-template <int VPT, int WARPS, bool FUSED>
+// Rows of one warp or less: blocks of 2 warps, or 1 where that leaves an SM without one.
+template <int VPT, int WARPS, int LANES, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int warps, bool odd) {
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(a.rows, 1 << 30));
-  if (odd) norm_forward_kernel<VPT, WARPS, true, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
-  else norm_forward_kernel<VPT, WARPS, false, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
+  const int64_t all = ceil_div(a.rows * LANES, 32);
+  if (WARPS == 1) warps = static_cast<int>(std::min<int64_t>(ceil_div(all, sm_count()), 2));
+  const unsigned grid =
+      static_cast<unsigned>(std::min<int64_t>(WARPS == 1 ? ceil_div(all, warps) : a.rows, 1 << 30));
+  if (odd) norm_forward_kernel<VPT, WARPS, LANES, true, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
+  else norm_forward_kernel<VPT, WARPS, LANES, false, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
 }
 
 template <int VPT, bool ODD, bool FUSED>
 void launch_staged(cudaStream_t s, const ForwardArgs& a, int warps) {
-  auto* kernel = norm_forward_kernel<VPT, 0, ODD, FUSED, true>;
+  auto* kernel = norm_forward_kernel<VPT, 0, 32, ODD, FUSED, true>;
   constexpr int kWarpBytes = (FUSED ? 2 : 1) * 32 * VPT * 16;
   static bool attr_done[64] = {false};
   int dev = 0;
@@ -760,16 +785,12 @@ constexpr int kStagedWarps = 9;  // rows whose blocks an SM holds one of
 template <int VPT, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
   const int warps = static_cast<int>(ceil_div(words, 32 * VPT));
-  if constexpr (VPT < 8) {
-    launch_forward<VPT, 1, FUSED>(s, a, 1, odd);
-  } else {
-    if (warps >= kStagedWarps && odd) launch_staged<VPT, true, FUSED>(s, a, warps);
-    else if (warps >= kStagedWarps) launch_staged<VPT, false, FUSED>(s, a, warps);
-    else if (warps == 1) launch_forward<VPT, 1, FUSED>(s, a, warps, odd);
-    else if (warps == 2) launch_forward<VPT, 2, FUSED>(s, a, warps, odd);
-    else if (warps == 4) launch_forward<VPT, 4, FUSED>(s, a, warps, odd);
-    else launch_forward<VPT, 0, FUSED>(s, a, warps, odd);
-  }
+  if (warps >= kStagedWarps && odd) launch_staged<VPT, true, FUSED>(s, a, warps);
+  else if (warps >= kStagedWarps) launch_staged<VPT, false, FUSED>(s, a, warps);
+  else if (warps == 1) launch_forward<VPT, 1, 32, FUSED>(s, a, warps, odd);
+  else if (warps == 2) launch_forward<VPT, 2, 32, FUSED>(s, a, warps, odd);
+  else if (warps == 4) launch_forward<VPT, 4, 32, FUSED>(s, a, warps, odd);
+  else launch_forward<VPT, 0, 32, FUSED>(s, a, warps, odd);
 }
 
 // 32 values to a thread, of each of two inputs where there are two. Where there are rows to
@@ -782,9 +803,11 @@ template <bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
   const bool many = !FUSED && (words > 1536 || (words > 256 && words <= 384)) &&
                     a.rows >= 12 * static_cast<int64_t>(sm_count());
-  if (words <= 32) launch_forward<1, FUSED>(s, a, words, odd);
-  else if (words <= 64) launch_forward<2, FUSED>(s, a, words, odd);
-  else if (words <= 128) launch_forward<4, FUSED>(s, a, words, odd);
+  if (words <= 8) launch_forward<1, 1, 8, FUSED>(s, a, 1, odd);
+  else if (words <= 16) launch_forward<2, 1, 8, FUSED>(s, a, 1, odd);
+  else if (words <= 32) launch_forward<4, 1, 8, FUSED>(s, a, 1, odd);
+  else if (words <= 64) launch_forward<4, 1, 16, FUSED>(s, a, 1, odd);
+  else if (words <= 128) launch_forward<4, 1, 32, FUSED>(s, a, 1, odd);
   else if (words <= 4096 && !many) launch_forward<8, FUSED>(s, a, words, odd);
   else if constexpr (!FUSED) launch_forward<16, FUSED>(s, a, words, odd);
 }
