@@ -433,36 +433,36 @@ norm_forward_kernel(ForwardArgs a) {
 // blocks: a few more and their rows came in a second round, 245 us against 154 for [2048,
 // 32768]; 4 blocks of 16 warps took 179).
 
-// Warps to an SM: 128 registers a thread, or 64 where it holds one word of each array.
-constexpr int warps_per_sm(int vpt) { return vpt == 1 ? 32 : 16; }
+// Warps to an SM: 128 registers a thread, or 85 where it holds one word of each array.
+constexpr int warps_per_sm(int vpt) { return vpt == 1 ? 24 : 16; }
 
 template <int VPT, int WARPS, bool ODD, bool FUSED>
 struct Places {
   static constexpr bool kExtra = FUSED && WARPS, kWeight = ODD || WARPS;
   static constexpr int kRing = kExtra ? 2 : 3;
   static constexpr int kWarp = 32 * VPT * (kRing * 2 + (kExtra ? 2 : 0) + (kWeight ? 1 : 0));  // words of a warp
-  // with several rows to a block its column sums take their place in the end
-  static constexpr int bytes(int threads) {
-    const int words = kWarp * (threads / 32) * 16, columns = WARPS ? 2 * (128 * 4 * VPT + 4) * 4 : 0;
-    return words > columns ? words : columns;
-  }
+  // with several rows to a block their column sums take the rows' place in the end
+  static constexpr int bytes(int threads) { return kWarp * (threads / 32) * 16; }
 };
 
-// WARPS: warps of a row, with 8 / WARPS rows to a block (GROUPS); 0: any number, one row to a block.
-template <int VPT, int WARPS, int CLUSTER, bool ODD, bool FUSED>
+// WARPS: warps of a row, with 8 / WARPS rows to a block (groups); 0: any number, one row to a
+// block; 1 with fewer LANES than 32: several rows to a warp ([500000, 64]: 71 us
+// against 95 with a warp to each, with dropout and residual 118 against 263).
+template <int VPT, int WARPS, int LANES, int CLUSTER, bool ODD, bool FUSED>
 __global__ void __launch_bounds__(WARPS ? 256 : 512, WARPS ? warps_per_sm(VPT) / 8 : 1)
 norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   static_assert(CLUSTER == 1 || WARPS == 0, "");
-  constexpr bool MULTI = WARPS != 0;
+  static_assert(LANES == 32 || (WARPS == 1 && LANES >= 8), "a lane to each loose element");
+  constexpr bool MULTI = WARPS != 0, SHARED = LANES < 32;
   const int warps = MULTI ? WARPS : blockDim.x >> 5;
   extern __shared__ __align__(16) float4 stage[];
   __shared__ float2 sums[2][kMostWarps];
   __shared__ float2 peers[2][CLUSTER];
   __shared__ __align__(8) uint64_t arrived[2];
   const int tpr = warps * 32, kSpan = tpr * VPT;  // words of a block's part of a row
-  constexpr int groups = MULTI ? 8 / (MULTI ? WARPS : 1) : 1;
-  const int group = MULTI ? threadIdx.x / (32 * (MULTI ? WARPS : 1)) : 0;
-  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - group * warps;
+  constexpr int kGroup = LANES * (MULTI ? WARPS : 1), groups = MULTI ? 256 / kGroup : 1;
+  const int group = MULTI ? threadIdx.x / kGroup : 0;
+  const int lane = threadIdx.x & (LANES - 1), warp = SHARED ? 0 : (threadIdx.x >> 5) - group * warps;
   const int rank = CLUSTER > 1 ? static_cast<int>(ptx::cluster_rank()) : 0;
   const int first_word = rank * kSpan + warp * 32 * VPT + lane;  // a warp's words are side by side
   const int64_t step = static_cast<int64_t>(gridDim.x / CLUSTER) * groups;
@@ -480,10 +480,11 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
 
   using P = Places<VPT, WARPS, ODD, FUSED>;
   constexpr int kRing = P::kRing;
-  float4* const mine = stage + (threadIdx.x >> 5) * P::kWarp + lane;  // this thread's first place
+  float4* const mine = stage + (threadIdx.x >> 5) * P::kWarp + (threadIdx.x & 31);  // this thread's first place
   float4* const mine_extra = mine + kRing * 2 * VPT * 32;             // of dtotal
   float4* const weight = mine + (kRing * 2 + (P::kExtra ? 2 : 0)) * VPT * 32;
   const Words<ODD> words(opening, a.cols);  // but for their places, those of all its rows
+  const int ahead = static_cast<int>(words.at - opening * a.cols);
   const bool loose = rank == 0 && warp == 0 && words.loose(lane);
   const int column = ODD ? words.loose_column(lane) : 0;
   float loose_dw = 0.0f, loose_db = 0.0f, loose_w = 1.0f;
@@ -494,8 +495,9 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) dw[k][j] = db[k][j] = 0.0f;
     if (P::kWeight)
-      weight[32 * k] = a.weight && words.holds(first_word + 32 * k) ? words.column(a.weight, first_word + 32 * k)
-                                                                    : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      weight[32 * k] = a.weight && words.holds(first_word + LANES * k)
+                           ? words.column(a.weight, first_word + LANES * k)
+                           : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
   }
 
   // Copies a row into a place: word k of dy and of total.
@@ -505,8 +507,8 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       const int64_t at = row * a.cols + words.head + 4 * static_cast<int64_t>(first_word);
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
-        if (words.holds(first_word + 32 * k)) {
-          const int64_t i = at + 128 * k;
+        if (words.holds(first_word + LANES * k)) {
+          const int64_t i = at + 4 * LANES * k;
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + 32 * k)), "l"(a.dy + i)
                        : "memory");
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + 32 * (VPT + k))),
@@ -522,10 +524,10 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       const int64_t at = row * a.cols + words.head + 4 * static_cast<int64_t>(first_word);
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (words.holds(first_word + 32 * k))
+        if (words.holds(first_word + LANES * k))
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
                            ptx::smem_u32(mine_extra + (place * VPT + k) * 32)),
-                       "l"(a.dtotal + at + 128 * k)
+                       "l"(a.dtotal + at + 4 * LANES * k)
                        : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -553,14 +555,15 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
   loose_of(opening, loose_d, loose_t);
   unsigned turn = 0;
   int place = 0;
-  for (int64_t row = opening; row < a.rows; row += step, ++turn) {
+  for (int64_t row = opening; row - (SHARED ? group : 0) < a.rows; row += step, ++turn) {
+    const bool present = !SHARED || row < a.rows;  // a warp's rows run on past the last one together
     const int64_t at = row * a.cols;
     statistics(row + step, next_mean, next_rstd);
     float4 extra[FUSED && !P::kExtra ? VPT : 1];
     if (FUSED && !P::kExtra && a.dtotal) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k)
-        if (words.holds(first_word + 32 * k))
+        if (words.holds(first_word + LANES * k))
           extra[P::kExtra ? 0 : k] =
               __ldcs(reinterpret_cast<const float4*>(a.dtotal + at + words.head) + first_word + 32 * k);
     }
@@ -570,8 +573,8 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = first_word + 32 * k;
-      const bool in = words.holds(word);
+      const int word = first_word + LANES * k;
+      const bool in = present && words.holds(word);
       float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), t = make_float4(mean, mean, mean, mean);
       float4 w = P::kWeight ? weight[32 * k] : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
       if (in) {
@@ -591,7 +594,7 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
       }
     }
     float loose_g = 0.0f, loose_hat = 0.0f;
-    if (ODD && loose) {
+    if (ODD && loose && present) {
       loose_hat = (loose_t - mean) * rstd;
       loose_g = loose_d * loose_w;
       s1 += loose_g;
@@ -603,9 +606,9 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     copy(place, row + kRing * step);
     uint32_t mask = 0;
     if (FUSED && a.dx)
-      mask = kept_words<VPT>(from + static_cast<uint64_t>(at + words.head) + 4 * static_cast<uint64_t>(first_word), 32,
-                             rk, a.drop.threshold);
-    const float2 sums_all = row_sums(s1, s2, sums[turn & 1] + group * warps, warps, warp, 1 + group);
+      mask = kept_words<VPT, LANES>(from + static_cast<uint64_t>(at + ahead) + 4 * static_cast<uint64_t>(first_word),
+                                    LANES, rk, a.drop.threshold);
+    const float2 sums_all = row_sums<LANES>(s1, s2, sums[turn & 1] + group * warps, warps, warp, 1 + group);
     s1 = sums_all.x, s2 = sums_all.y;
     if (CLUSTER > 1) {
       // This block's sums go to every block of the cluster, its own too. A peer that sends
@@ -635,8 +638,8 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     float4* const out_x = FUSED && a.dx ? reinterpret_cast<float4*>(a.dx + at + words.head) + first_word : nullptr;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int word = first_word + 32 * k;
-      if (!words.holds(word)) continue;
+      const int word = first_word + LANES * k;
+      if (!present || !words.holds(word)) continue;
       float d[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j] = fmaf(hat[k][j], c2, fmaf(g[k][j], rstd, c1));
@@ -644,14 +647,14 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
         const float4 e = P::kExtra ? mine_extra[(place * VPT + k) * 32] : extra[P::kExtra ? 0 : k];
         d[0] += e.x, d[1] += e.y, d[2] += e.z, d[3] += e.w;
       }
-      __stcs(out + 32 * k, make_float4(d[0], d[1], d[2], d[3]));
+      __stcs(out + LANES * k, make_float4(d[0], d[1], d[2], d[3]));
       if (FUSED && a.dx) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) d[j] = dropped(d[j], mask >> (4 * k + j) & 1, a.drop.scale);
-        __stcs(out_x + 32 * k, make_float4(d[0], d[1], d[2], d[3]));
+        __stcs(out_x + LANES * k, make_float4(d[0], d[1], d[2], d[3]));
       }
     }
-    if (ODD && loose) {
+    if (ODD && loose && present) {
       const int64_t i = at + column;
       float d = fmaf(loose_hat, c2, fmaf(loose_g, rstd, c1));
       if (FUSED && a.dtotal) d += __ldcs(a.dtotal + i);
@@ -687,30 +690,31 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
     float* const columns = reinterpret_cast<float*>(stage);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    constexpr int kMostColumns = 128 * (MULTI ? WARPS : 1) * VPT + 4;  // whole words, and fewer loose ones than a word
-    for (int i = threadIdx.x; i < 2 * kMostColumns; i += blockDim.x) columns[i] = 0.0f;
-    for (int whose = 0; whose < groups; ++whose) {
-      __syncthreads();
-      if (group != whose) continue;
+    constexpr int kMostColumns = 4 * kGroup * VPT + 4;  // whole words, and fewer loose ones than a word
+    static_assert(groups * 2 * kMostColumns * 4 <= P::kWarp * 8 * 16, "the rows' place");
+    float* const its = columns + group * 2 * kMostColumns;
 #pragma unroll
-      for (int k = 0; k < VPT; ++k) {
-        if (!words.holds(first_word + 32 * k)) continue;
+    for (int k = 0; k < VPT; ++k) {
+      if (!words.holds(first_word + LANES * k)) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = words.head + 4 * (first_word + 32 * k) + j;
-          columns[c] += dw[k][j];
-          columns[kMostColumns + c] += db[k][j];
-        }
-      }
-      if (ODD && loose) {
-        columns[column] += loose_dw;
-        columns[kMostColumns + column] += loose_db;
+      for (int j = 0; j < 4; ++j) {
+        const int c = words.head + 4 * (first_word + LANES * k) + j;
+        its[c] = dw[k][j];
+        its[kMostColumns + c] = db[k][j];
       }
     }
+    if (ODD && loose) {
+      its[column] = loose_dw;
+      its[kMostColumns + column] = loose_db;
+    }
     __syncthreads();
-    for (int c = threadIdx.x; c < static_cast<int>(a.cols); c += blockDim.x) {
-      partial[at + c] = columns[c];
-      partial[at + a.cols + c] = columns[kMostColumns + c];
+    const int cols = static_cast<int>(a.cols);
+    for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) {
+      const float* const sum = columns + (i < cols ? i : kMostColumns + i - cols);
+      float t = 0.0f;
+#pragma unroll
+      for (int g = 0; g < groups; ++g) t += sum[g * 2 * kMostColumns];
+      partial[at + i] = t;
     }
   }
 }
@@ -821,27 +825,28 @@ int64_t backward_blocks(int64_t rows, int64_t cols, int groups, int resident) {
 }
 
 struct BackwardPlan {
-  int vpt, warps, cluster, groups;  // words of a thread; warps of a block to a row; vpt 0: no such kernel
+  int vpt, warps, lanes, cluster, groups;  // words of a thread; warps of a block to a row; vpt 0: no such kernel
   int per_sm;                       // blocks that an SM's registers and shared memory hold
 };
 
 BackwardPlan backward_plan(int64_t cols) {
   const int64_t words = words_of(cols);
-  if (words > 8 * 128 * kMostWarps) return {0, 0, 0, 0, 0};
+  if (words > 8 * 128 * kMostWarps) return {0, 0, 0, 0, 0, 0};
   BackwardPlan plan;
-  plan.vpt = words <= 32 ? 1 : words <= 64 ? 2 : 4;
-  const int warps = static_cast<int>(ceil_div(words, 32 * plan.vpt));
+  plan.vpt = words <= 8 ? 1 : words <= 64 ? 2 : 4;
+  plan.lanes = words <= 16 ? 8 : words <= 32 ? 16 : 32;
+  const int warps = static_cast<int>(ceil_div(words, plan.lanes * plan.vpt));
   plan.cluster = warps <= kMostWarps ? 1 : warps <= 32 ? 4 : 8;
   plan.warps = static_cast<int>(ceil_div(warps, plan.cluster));
-  plan.groups = plan.warps == 1 || plan.warps == 2 || plan.warps == 4 ? 8 / plan.warps : 1;
-  plan.per_sm = std::max(1, warps_per_sm(plan.vpt) / (plan.warps * plan.groups));
+  plan.groups = plan.warps == 1 || plan.warps == 2 || plan.warps == 4 ? 256 / (plan.warps * plan.lanes) : 1;
+  plan.per_sm = std::max(1, warps_per_sm(plan.vpt) * 32 / (plan.warps * plan.lanes * plan.groups));
   return plan;
 }
 
-template <int VPT, int WARPS, int CLUSTER, bool ODD, bool FUSED>
+template <int VPT, int WARPS, int LANES, int CLUSTER, bool ODD, bool FUSED>
 int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan) {
-  auto* kernel = norm_backward_kernel<VPT, WARPS, CLUSTER, ODD, FUSED>;
-  const int threads = plan.warps * plan.groups * 32;
+  auto* kernel = norm_backward_kernel<VPT, WARPS, LANES, CLUSTER, ODD, FUSED>;
+  const int threads = plan.warps * plan.groups * plan.lanes;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = Places<VPT, WARPS, ODD, FUSED>::bytes(threads);
@@ -872,30 +877,32 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
   return blocks;
 }
 
-template <int VPT, int WARPS, int CLUSTER>
+template <int VPT, int WARPS, int LANES, int CLUSTER>
 int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd) {
   const bool fused = a.dtotal || a.dx;
   if (odd)
-    return fused ? launch_backward<VPT, WARPS, CLUSTER, true, true>(s, a, partial, plan)
-                 : launch_backward<VPT, WARPS, CLUSTER, true, false>(s, a, partial, plan);
-  return fused ? launch_backward<VPT, WARPS, CLUSTER, false, true>(s, a, partial, plan)
-               : launch_backward<VPT, WARPS, CLUSTER, false, false>(s, a, partial, plan);
+    return fused ? launch_backward<VPT, WARPS, LANES, CLUSTER, true, true>(s, a, partial, plan)
+                 : launch_backward<VPT, WARPS, LANES, CLUSTER, true, false>(s, a, partial, plan);
+  return fused ? launch_backward<VPT, WARPS, LANES, CLUSTER, false, true>(s, a, partial, plan)
+               : launch_backward<VPT, WARPS, LANES, CLUSTER, false, false>(s, a, partial, plan);
 }
 
 // Returns the partial rows that it leaves.
 int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd) {
   switch (plan.cluster) {
-    case 4: return launch_backward<4, 0, 4>(s, a, partial, plan, odd);
-    case 8: return launch_backward<4, 0, 8>(s, a, partial, plan, odd);
+    case 4: return launch_backward<4, 0, 32, 4>(s, a, partial, plan, odd);
+    case 8: return launch_backward<4, 0, 32, 8>(s, a, partial, plan, odd);
     default: break;
   }
-  if (plan.vpt == 1) return launch_backward<1, 1, 1>(s, a, partial, plan, odd);
-  if (plan.vpt == 2) return launch_backward<2, 1, 1>(s, a, partial, plan, odd);
+  if (plan.vpt == 1) return launch_backward<1, 1, 8, 1>(s, a, partial, plan, odd);
+  if (plan.lanes == 8) return launch_backward<2, 1, 8, 1>(s, a, partial, plan, odd);
+  if (plan.lanes == 16) return launch_backward<2, 1, 16, 1>(s, a, partial, plan, odd);
+  if (plan.vpt == 2) return launch_backward<2, 1, 32, 1>(s, a, partial, plan, odd);
   switch (plan.warps) {
-    case 1: return launch_backward<4, 1, 1>(s, a, partial, plan, odd);
-    case 2: return launch_backward<4, 2, 1>(s, a, partial, plan, odd);
-    case 4: return launch_backward<4, 4, 1>(s, a, partial, plan, odd);
-    default: return launch_backward<4, 0, 1>(s, a, partial, plan, odd);
+    case 1: return launch_backward<4, 1, 32, 1>(s, a, partial, plan, odd);
+    case 2: return launch_backward<4, 2, 32, 1>(s, a, partial, plan, odd);
+    case 4: return launch_backward<4, 4, 32, 1>(s, a, partial, plan, odd);
+    default: return launch_backward<4, 0, 32, 1>(s, a, partial, plan, odd);
   }
 }
 

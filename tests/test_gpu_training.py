@@ -326,6 +326,13 @@ def test_norm_many_middling_rows(tcx, oracle, rows, cols):
     test_norm_long_rows_in_turn(tcx, oracle, rows, cols)
 
 
+@pytest.mark.parametrize("rows,cols", [(60001, 1), (60000, 2), (60002, 31), (31001, 64), (40003, 67), (20001, 128),
+                                       (20003, 129), (10001, 256), (10003, 259)])
+def test_norm_many_short_rows(tcx, oracle, rows, cols):
+    """Rows that share a warp, more of them than run at a time, and the last warp not full."""
+    test_norm_long_rows_in_turn(tcx, oracle, rows, cols)
+
+
 @pytest.mark.parametrize("cols", [3, 130])
 def test_norm_gradient_against_differences(tcx, oracle, cols):
     """The kernels' gradients along a direction against central differences of the 64-bit
