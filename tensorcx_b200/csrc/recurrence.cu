@@ -119,30 +119,34 @@ __device__ __forceinline__ void backward_step(const float (&gate)[VEC], const fl
 }
 
 // ------------------------------------------------------- one thread per VEC channels
-// Walks through time by itself, the loads of kAhead steps at a time. For short sequences (a
+// Walks through time by itself, the loads of AHEAD steps at a time. For short sequences (a
 // token of each running sequence is one step of this kernel) and for batches wide enough.
-// Four steps' loads in flight: [64, 32, 4096] forward 24 us, 28 with two, 26 with eight.
-constexpr int kAhead = 4;
+// Four steps' loads of 4 channels in flight: [64, 32, 4096] forward 24 us, 28 with two, 26 with
+// eight; eight of one channel: [100, 100, 1001] forward 35 us against 39. A call of one step
+// has its own kernel, of which an SM holds more threads ([4096, 1, 4096]: forward 59 us before
+// and 43 so, sigmoid backward 150 and 92).
+template <int VEC>
+constexpr int kAhead = VEC == 4 ? 4 : 8;
 
-template <int VEC, bool SIGMOID>
-__global__ void __launch_bounds__(256) walk_forward_kernel(Args a) {
+template <int VEC, int AHEAD, bool SIGMOID>
+__global__ void __launch_bounds__(256, AHEAD == 1 ? 8 : 4) walk_forward_kernel(Args a) {
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * VEC;
   if (i >= a.batch * a.channels) return;
-  const int64_t b = i / a.channels, n = length_of(a, b);
+  const int64_t b = a.batch == 1 ? 0 : i / a.channels, n = length_of(a, b);
   float h[VEC];
   start_of<VEC>(h, a.initial, i);
   int64_t at = b * (a.time - 1) * a.channels + i;
-  for (int64_t t0 = 0; t0 < a.time; t0 += kAhead) {
-    float g[kAhead][VEC], x[kAhead][VEC];
+  for (int64_t t0 = 0; t0 < a.time; t0 += AHEAD) {
+    float g[AHEAD][VEC], x[AHEAD][VEC];
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
+    for (int s = 0; s < AHEAD; ++s) {
       if (t0 + s < n) {
         load<VEC>(g[s], a.gate + at + s * a.channels);
         load<VEC>(x[s], a.x + at + s * a.channels);
       }
     }
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s, at += a.channels) {
+    for (int s = 0; s < AHEAD; ++s, at += a.channels) {
       if (t0 + s >= a.time) break;
       if (t0 + s < n) {
 #pragma unroll
@@ -161,18 +165,18 @@ __global__ void __launch_bounds__(256) walk_forward_kernel(Args a) {
   if (a.state) store<VEC>(a.state + i, h);
 }
 
-template <int VEC, bool SIGMOID>
+template <int VEC, int AHEAD, bool SIGMOID>
 __global__ void __launch_bounds__(256) walk_backward_kernel(Args a) {
   const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * VEC;
   if (i >= a.batch * a.channels) return;
-  const int64_t b = i / a.channels, n = length_of(a, b);
+  const int64_t b = a.batch == 1 ? 0 : i / a.channels, n = length_of(a, b);
   float c[VEC];
   start_of<VEC>(c, a.dstate, i);
   int64_t at = b * (a.time - 1) * a.channels + i + (a.time - 1) * a.channels;
-  for (int64_t t0 = a.time - 1; t0 >= 0; t0 -= kAhead) {
-    float gate[kAhead][VEC], dh[kAhead][VEC], before[kAhead][VEC], x[kAhead][VEC];
+  for (int64_t t0 = a.time - 1; t0 >= 0; t0 -= AHEAD) {
+    float gate[AHEAD][VEC], dh[AHEAD][VEC], before[AHEAD][VEC], x[AHEAD][VEC];
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
+    for (int s = 0; s < AHEAD; ++s) {
       const int64_t t = t0 - s, here = at - s * a.channels;
       if (t < 0) break;
       load<VEC>(dh[s], a.dh + here);
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(256) walk_backward_kernel(Args a) {
       }
     }
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s, at -= a.channels) {
+    for (int s = 0; s < AHEAD; ++s, at -= a.channels) {
       if (t0 - s < 0) break;
       float dgate[VEC], dx[VEC];
       backward_step<VEC, SIGMOID>(gate[s], dh[s], before[s], x[s], t0 - s < n, c, dgate, dx);
@@ -847,13 +851,14 @@ bool all_aligned(const Args& a) {
 }
 
 // Threads walk through time alone where there are few steps, and up to a chunk of them where
-// the channels fill the machine: a chunk that is mostly empty costs its block as much as a
-// full one. [64, 32, 4096]: walk 24 us, scan 62; [256, 100, 1024]: 56 both; [16, 64, 1024],
-// whose 4096 threads fill nothing: walk 21 us, scan 11.
+// the channels fill the machine, or as much less of it as the chunk is emptier: one that is
+// mostly empty costs its block as much as a full one. [64, 32, 4096]: walk 24 us, scan 62;
+// [64, 32, 1024] 16 and 20; [32, 64, 4096] 31 and 35; [256, 100, 1024] 56 both; [32, 100, 4096]
+// 43 and 37; [16, 64, 1024], whose 4096 threads fill nothing, 21 and 11.
 constexpr int64_t kWalkSteps = 16;
 template <int VEC>
 bool walks(const Args& a) {
-  return a.time <= kWalkSteps || (a.time <= kChunk && a.batch * a.channels >= 256 * VEC * sm_count());
+  return a.time <= kWalkSteps || (a.time <= kChunk && a.batch * a.channels * (kChunk / a.time) >= 256 * VEC * sm_count());
 }
 
 // Whole chains to a block, where the last of their rounds leaves few blocks idle: [16, 512,
@@ -897,8 +902,8 @@ template <int VEC, bool SHIFTED, bool SIGMOID>
 int launch_forward(cudaStream_t s, const Args& a, void* workspace) {
   if (walks<VEC>(a)) {
     TimedLaunch timer("recurrence_walk", s);
-    walk_forward_kernel<VEC, SIGMOID>
-        <<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
+    auto* kernel = a.time == 1 ? walk_forward_kernel<VEC, 1, SIGMOID> : walk_forward_kernel<VEC, kAhead<VEC>, SIGMOID>;
+    kernel<<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
     return launch_status("recurrence");
   }
   using F = Forward<VEC, SHIFTED>;
@@ -915,14 +920,22 @@ template <int VEC, bool SHIFTED, bool SIGMOID>
 int launch_backward(cudaStream_t s, const Args& a, void* workspace) {
   if (walks<VEC>(a)) {
     TimedLaunch timer("recurrence_walk_backward", s);
-    walk_backward_kernel<VEC, SIGMOID>
-        <<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
+    auto* kernel = a.time == 1 ? walk_backward_kernel<VEC, 1, SIGMOID> : walk_backward_kernel<VEC, kAhead<VEC>, SIGMOID>;
+    kernel<<<static_cast<unsigned>(ceil_div(a.batch * a.channels, 256 * VEC)), 256, 0, s>>>(a);
     return launch_status("recurrence");
   }
   using K = Backward<VEC, SHIFTED, SIGMOID>;
   TimedLaunch timer("recurrence_scan_backward", s);
   return launch_scan<scan_backward_kernel<VEC, SHIFTED, SIGMOID>>(s, a, K::kThreads, K::kBytes, K::kPerSm, false,
                                                                   workspace);
+}
+
+// One step of whole sequences: the batch's channels lie in a row, as one sequence's do. Then no
+// thread divides by the channels, and rows of any length are words ([1024, 1, 4097]: 31 us and
+// 18 forward, 41 and 27 backward).
+Args one_row(Args a) {
+  if (a.time == 1 && !a.lengths) a.channels *= a.batch, a.batch = 1;
+  return a;
 }
 
 template <bool SIGMOID>
@@ -987,8 +1000,8 @@ extern "C" int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const
          channels};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (time == 0) return pass_through(s, initial, state, batch * channels);
-  return form == TCX_RECURRENCE_SIGMOID ? launch_forward<true>(s, a, workspace)
-                                        : launch_forward<false>(s, a, workspace);
+  return form == TCX_RECURRENCE_SIGMOID ? launch_forward<true>(s, one_row(a), workspace)
+                                        : launch_forward<false>(s, one_row(a), workspace);
 }
 
 extern "C" int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, const float* dh, const float* gate,
@@ -1005,6 +1018,6 @@ extern "C" int tcx_sm100_recurrence_backward(tcx_stream_t stream, int form, cons
   Args a{gate, x, initial, lengths, nullptr, nullptr, dh, h, dstate, dgate, dx, dinitial, batch, time, channels};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (time == 0) return pass_through(s, dstate, dinitial, batch * channels);
-  return form == TCX_RECURRENCE_SIGMOID ? launch_backward<true>(s, a, workspace)
-                                        : launch_backward<false>(s, a, workspace);
+  return form == TCX_RECURRENCE_SIGMOID ? launch_backward<true>(s, one_row(a), workspace)
+                                        : launch_backward<false>(s, one_row(a), workspace);
 }

@@ -504,6 +504,19 @@ def test_recurrence_many_sequences(tcx, form, batch, time, channels):
         assert (h[b, n:] == (h[b, n - 1] if n else init[b])).all()
 
 
+@pytest.mark.parametrize("form", ["decay", "sigmoid"])
+@pytest.mark.parametrize("lengths", [False, True])
+@pytest.mark.parametrize("batch,channels,shift", [(1, 3, 0), (4, 1001, 0), (37, 33, 0), (300, 256, 0), (12, 1001, 1)])
+def test_recurrence_one_step(tcx, form, lengths, batch, channels, shift):
+    """The batch's channels as one row, or each entry's by its length."""
+    gate, x, init, dh, dstate = recurrence_case(batch, 1, channels, form, seed=8)
+    n = np.random.default_rng(batch).integers(-1, 3, batch) if lengths else None
+    if lengths:
+        pad = ~live_steps(batch, 1, n)
+        gate[pad], x[pad] = np.nan, np.inf
+    check_recurrence(tcx, gate, x, init, dh, dstate, form, n, shift=shift)
+
+
 @pytest.mark.parametrize("shift", [1, 2, 3])
 @pytest.mark.parametrize("channels", [128, 96, 33])
 def test_recurrence_alignment(tcx, shift, channels):
