@@ -231,7 +231,7 @@ __device__ __forceinline__ float2 row_sums(float a, float b, float2* smem, int w
 }
 
 // Kernels for a known number of warps to a row (WARPS), or any up to kMostWarps (0).
-constexpr int kMostWarps = 16;
+constexpr int kMostWarps = 16, kPairWarps = 10;
 // Threads of a forward block at most, and of the blocks that an SM holds of them.
 constexpr int most_threads(int warps) { return 32 * (warps == 1 ? 2 : warps ? warps : kMostWarps); }
 constexpr int resident_threads(int vpt, bool fused) {
@@ -239,15 +239,18 @@ constexpr int resident_threads(int vpt, bool fused) {
 }
 
 // One block to a row, VPT words to a thread, as many warps as the row needs. Each element is
-// read once and written once; the statistics take two block reductions. STAGED: few blocks fit
-// an SM, so that each takes rows in turn, and the next row's words come into shared memory
-// (cp.async; a thread copies and reads its own only) while this one is worked on.
+// read once and written once; the statistics take two block reductions. STAGED: the 1 or 2 blocks
+// that fit an SM take rows in turn, and the next row's words come into shared memory (cp.async; a
+// thread copies and reads its own only) while this one is worked on. Two blocks of up to 10 warps
+// and 96 registers ([7800, 8400] with dropout and residual: 217 us against 256 with one of 128,
+// [3000, 20000] 102 against 131), one of more ([5500, 12000] 211 against 243 with the registers
+// of two).
 // Rows of one warp or less (LANES lanes) share a block: with a block and a whole warp to each,
 // the starts of the blocks took [500000, 64] to 264 us against 56, [125000, 256] 72 against 47,
 // [600000, 33] with dropout and residual 459 against 117.
-template <int VPT, int WARPS, int LANES, bool ODD, bool FUSED, bool STAGED>
-__global__ void __launch_bounds__(most_threads(WARPS),
-                                  STAGED ? 1 : resident_threads(VPT, FUSED) / most_threads(WARPS))
+template <int VPT, int WARPS, int LANES, bool ODD, bool FUSED, int STAGED>
+__global__ void __launch_bounds__(STAGED == 2 ? 32 * kPairWarps : most_threads(WARPS),
+                                  STAGED ? STAGED : resident_threads(VPT, FUSED) / most_threads(WARPS))
 norm_forward_kernel(ForwardArgs a) {
   static_assert(LANES == 32 || (WARPS == 1 && LANES >= 8), "a lane to each loose element");
   constexpr bool SHARED = WARPS == 1;
@@ -765,26 +768,33 @@ void launch_forward(cudaStream_t s, const ForwardArgs& a, int warps, bool odd) {
   if (WARPS == 1) warps = static_cast<int>(std::min<int64_t>(ceil_div(all, sm_count()), 2));
   const unsigned grid =
       static_cast<unsigned>(std::min<int64_t>(WARPS == 1 ? ceil_div(all, warps) : a.rows, 1 << 30));
-  if (odd) norm_forward_kernel<VPT, WARPS, LANES, true, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
-  else norm_forward_kernel<VPT, WARPS, LANES, false, FUSED, false><<<grid, 32 * warps, 0, s>>>(a);
+  if (odd) norm_forward_kernel<VPT, WARPS, LANES, true, FUSED, 0><<<grid, 32 * warps, 0, s>>>(a);
+  else norm_forward_kernel<VPT, WARPS, LANES, false, FUSED, 0><<<grid, 32 * warps, 0, s>>>(a);
 }
 
-template <int VPT, bool ODD, bool FUSED>
+template <int VPT, int BLOCKS, bool ODD, bool FUSED>
 void launch_staged(cudaStream_t s, const ForwardArgs& a, int warps) {
-  auto* kernel = norm_forward_kernel<VPT, 0, 32, ODD, FUSED, true>;
+  auto* kernel = norm_forward_kernel<VPT, 0, 32, ODD, FUSED, BLOCKS>;
   constexpr int kWarpBytes = (FUSED ? 2 : 1) * 32 * VPT * 16;
   static bool attr_done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostWarps * kWarpBytes);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         (BLOCKS == 2 ? kPairWarps : kMostWarps) * kWarpBytes);
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
-  const int64_t grid = std::min<int64_t>(a.rows, std::max(1, 16 / warps) * sm_count());
+  const int64_t grid = std::min<int64_t>(a.rows, BLOCKS * sm_count());
   kernel<<<static_cast<unsigned>(grid), 32 * warps, warps * kWarpBytes, s>>>(a);
 }
 
-constexpr int kStagedWarps = 9;  // rows whose blocks an SM holds one of
+constexpr int kStagedWarps = 9;  // rows whose blocks an SM holds one or two of
+
+template <int VPT, bool ODD, bool FUSED>
+void launch_staged(cudaStream_t s, const ForwardArgs& a, int warps) {
+  if (warps <= kPairWarps) launch_staged<VPT, 2, ODD, FUSED>(s, a, warps);
+  else launch_staged<VPT, 1, ODD, FUSED>(s, a, warps);
+}
 
 template <int VPT, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {

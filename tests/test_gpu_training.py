@@ -320,7 +320,8 @@ def test_norm_long_rows_in_turn(tcx, oracle, rows, cols):
     check_backward(tcx, oracle, dy, want, host(mean), host(rstd), w, x, 0.5, 9, 1)
 
 
-@pytest.mark.parametrize("rows,cols", [(310, 8192), (350, 6001), (1790, 6404), (1801, 1101), (1777, 8403)])
+@pytest.mark.parametrize("rows,cols", [(310, 8192), (350, 6001), (1790, 6404), (1801, 1101), (1777, 8403),
+                                       (1800, 10000), (1790, 17408)])
 def test_norm_many_middling_rows(tcx, oracle, rows, cols):
     """Rows of one block, enough of them that fewer warps take more words of each."""
     test_norm_long_rows_in_turn(tcx, oracle, rows, cols)
