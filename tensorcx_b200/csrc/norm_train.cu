@@ -237,6 +237,18 @@ constexpr int most_threads(int warps) { return 32 * (warps == 1 ? 2 : warps ? wa
 constexpr int resident_threads(int vpt, bool fused) {
   return fused ? (vpt < 4 ? 1024 : vpt < 8 ? 768 : 512) : vpt < 4 ? 1536 : vpt < 8 ? 1024 : 768;
 }
+// What their registers are bounded by. Blocks of any number of warps as if they were as large as
+// that: 64 registers for 8 words of one input, 80 for 16 (an SM holds 3 blocks of 8 warps instead
+// of two: [4096, 16384] 110 -> 98 us), 96 for 8 of two ([9500, 6001] 207 -> 177; 80 are too few).
+constexpr int bound_threads(int vpt, int warps, bool fused, int staged) {
+  if (staged == 2) return 32 * kPairWarps;
+  if (staged || warps) return most_threads(warps);
+  return fused ? 640 : vpt == 8 ? 1024 : 768;
+}
+constexpr int bound_blocks(int vpt, int warps, bool fused, int staged) {
+  if (staged) return staged;
+  return warps ? resident_threads(vpt, fused) / most_threads(warps) : 1;
+}
 
 // One block to a row, VPT words to a thread, as many warps as the row needs. Each element is
 // read once and written once; the statistics take two block reductions. STAGED: the 1 or 2 blocks
@@ -249,8 +261,7 @@ constexpr int resident_threads(int vpt, bool fused) {
 // the starts of the blocks took [500000, 64] to 264 us against 56, [125000, 256] 72 against 47,
 // [600000, 33] with dropout and residual 459 against 117.
 template <int VPT, int WARPS, int LANES, bool ODD, bool FUSED, int STAGED>
-__global__ void __launch_bounds__(STAGED == 2 ? 32 * kPairWarps : most_threads(WARPS),
-                                  STAGED ? STAGED : resident_threads(VPT, FUSED) / most_threads(WARPS))
+__global__ void __launch_bounds__(bound_threads(VPT, WARPS, FUSED, STAGED), bound_blocks(VPT, WARPS, FUSED, STAGED))
 norm_forward_kernel(ForwardArgs a) {
   static_assert(LANES == 32 || (WARPS == 1 && LANES >= 8), "a lane to each loose element");
   constexpr bool SHARED = WARPS == 1;
