@@ -467,8 +467,9 @@ int tcx_sm100_embedding(tcx_stream_t stream, const int32_t* indices, int64_t row
  * p in [0, 1]; p = 0 keeps everything, p = 1 nothing. A kept element is multiplied by
  * 1 / (1 - p) rounded to float32; a dropped one counts as 0 even when it is inf or NaN.
  * step_offset, when not NULL, is a device int64 that is read when the kernels run and
- * added to offset (modulo 2^64): a captured graph whose counter is advanced between
- * replays gets a new mask every time. */
+ * added to offset: a captured graph whose counter is advanced between replays gets a new
+ * mask every time. Places are modulo 2^64 (place 2^64 is place 0, and a counter of -1
+ * starts one place before offset), alike in every call and for buffers of any alignment. */
 
 /* output = dropout(input), or residual + dropout(input) with a residual (the product and
  * the sum rounded one after the other). The gradient with respect to input is the same

@@ -58,9 +58,10 @@ __device__ __forceinline__ float dropped(float x, bool keep, float scale) {
   return keep ? __fmul_rn(x, scale) : 0.0f;
 }
 
-// Bit j: word j of the block is kept.
+// Bit j: word j of the block is kept. Places are taken modulo 2^64, so that blocks are modulo
+// 2^62: the next one after the stream's last is its first.
 __device__ __forceinline__ uint32_t kept_block(uint64_t block, const philox::RoundKeys& rk, uint32_t threshold) {
-  const uint4 w = philox::block_words(block, rk);
+  const uint4 w = philox::block_words(block & (~0ull >> 2), rk);
   return (kept(w.x, threshold) ? 1u : 0u) | (kept(w.y, threshold) ? 2u : 0u) | (kept(w.z, threshold) ? 4u : 0u) |
          (kept(w.w, threshold) ? 8u : 0u);
 }
