@@ -478,9 +478,10 @@ int tcx_sm100_dropout(tcx_stream_t stream, const float* input, const float* resi
                       double p, uint64_t seed, uint64_t offset, const int64_t* step_offset);
 
 /* Layer norm over the last axis of [rows, cols] that keeps what its backward pass needs:
- *   total = residual + dropout(input)        (total may be NULL without both: it is input)
+ *   total = residual + dropout(input)        (without both it is input: total may be NULL)
  *   mean[r] = mean of row r,  rstd[r] = 1 / sqrt(variance of row r + epsilon)
  *   output = (total - mean) * rstd * weight + bias      (weight, bias [cols] or NULL)
+ * A total that is given and equals input is copied there (total may be input itself).
  * The variance is the biased one, computed about the mean; a row's differences from its
  * first element must be representable. A constant finite row of input (without dropout)
  * gives exactly 0 * weight + bias, NaN when epsilon is 0. A row that holds a NaN or an
@@ -493,8 +494,9 @@ int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* input, const f
 
 /* Its gradients. With xhat = (total - mean) * rstd and g = dy * weight:
  *   dresidual = dtotal + rstd * (g - mean(g) - xhat * mean(g * xhat))
- *   dx = dresidual through the dropout      (dx may be NULL when p is 0: it is dresidual)
+ *   dx = dresidual through the dropout      (when p is 0 it is dresidual: dx may be NULL)
  *   dweight[c] = sum over rows of dy * xhat,  dbias[c] = sum over rows of dy
+ * A dx that is given and equals dresidual is copied there (dx may be dresidual itself).
  * dtotal (the gradient that reaches total by other ways) may be NULL; dweight and dbias
  * are both given or both NULL. Sums over rows are added in a fixed order: the same inputs
  * give the same bits. The workspace holds partial column sums. */

@@ -958,6 +958,11 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
 
 int64_t splits_of(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(64, rows / 16)); }
 
+// An output that equals another tensor, where the caller has a buffer of its own for it.
+void copy_output(cudaStream_t s, const float* from, float* to, int64_t count) {
+  if (to && to != from) cudaMemcpyAsync(to, from, count * sizeof(float), cudaMemcpyDeviceToDevice, s);
+}
+
 int check_norm(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 0) return invalid("negative extent");
   if (cols == 0) return invalid("layer norm requires a non-empty last axis");
@@ -982,9 +987,12 @@ extern "C" int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* inp
   if (rows == 0) return TCX_OK;
   if (!input || !output || !mean || !rstd) return invalid("missing buffer");
   if ((residual || a.drop.threshold) && !total) return invalid("dropout or a residual needs a buffer for the total");
-  if (!residual && !a.drop.threshold) a.total = nullptr;  // it is the input
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   TimedLaunch timer("norm_forward", s);
+  if (!residual && !a.drop.threshold) {
+    copy_output(s, input, total, rows * cols);
+    a.total = nullptr;  // the kernels have no other than the input
+  }
   const int64_t words = words_of(cols);
   if (words > 8192 || !aligned(input) || !aligned(residual) || !aligned(output) || !aligned(a.total)) {
     const int grid = static_cast<int>(std::min<int64_t>(rows, 8 * sm_count()));
@@ -1035,7 +1043,7 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
   }
   if (!dy || !total || !mean || !rstd || !dresidual) return invalid("missing buffer");
   if (a.drop.threshold && !dx) return invalid("dropout needs a buffer for the input's gradient");
-  if (!a.drop.threshold) a.dx = nullptr;  // it is the residual's gradient
+  if (!a.drop.threshold) a.dx = nullptr;  // the kernels have no other than the residual's
   if (dweight && (!workspace || workspace_bytes < tcx_sm100_layernorm_backward_workspace_bytes(rows, cols)))
     return invalid("workspace too small for the layer norm gradient");
   TimedLaunch timer("norm_backward", s);
@@ -1044,16 +1052,17 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
   if (plan.vpt && aligned(dy) && aligned(total) && aligned(dtotal) && aligned(dresidual) && aligned(a.dx)) {
     const int64_t splits = launch_backward(s, a, partial, plan, cols % 4 != 0 || !aligned(weight));
     if (partial) join_columns(s, partial, splits, cols, dweight, dbias);
-    return launch_status("layer norm backward");
+  } else {
+    const int grid = static_cast<int>(std::min<int64_t>(rows, 8 * sm_count()));
+    norm_backward_any_kernel<<<grid, kThreads, 0, s>>>(a);
+    if (dweight) {
+      const int64_t splits = splits_of(rows);
+      const unsigned blocks = static_cast<unsigned>(ceil_div(cols, kThreads));
+      norm_columns_kernel<<<dim3(blocks, static_cast<unsigned>(splits)), kThreads, 0, s>>>(a, partial,
+                                                                                           ceil_div(rows, splits));
+      join_columns(s, partial, splits, cols, dweight, dbias);
+    }
   }
-  const int grid = static_cast<int>(std::min<int64_t>(rows, 8 * sm_count()));
-  norm_backward_any_kernel<<<grid, kThreads, 0, s>>>(a);
-  if (dweight) {
-    const int64_t splits = splits_of(rows);
-    const unsigned blocks = static_cast<unsigned>(ceil_div(cols, kThreads));
-    norm_columns_kernel<<<dim3(blocks, static_cast<unsigned>(splits)), kThreads, 0, s>>>(a, partial,
-                                                                                         ceil_div(rows, splits));
-    join_columns(s, partial, splits, cols, dweight, dbias);
-  }
+  if (!a.dx) copy_output(s, dresidual, dx, rows * cols);
   return launch_status("layer norm backward");
 }

@@ -1,4 +1,5 @@
-"""The training operators where their arguments end: places of the random stream at 2^64.
+"""The training operators where their arguments end: places of the random stream at 2^64, outputs
+that a call without dropout need not have.
 
 The masks are compared with the generator's definition in whole-number arithmetic on the host.
 """
@@ -48,3 +49,32 @@ def test_one_mask_past_the_stream_s_end(tcx, rows, cols, before):
             dx, dres, _, _ = tcx.layernorm_backward(dev(dy, shift), got, mean, rstd, dev(w), p=p, seed=seed, offset=at)
             dx, dres = host(dx), host(dres)
             assert dx.tobytes() == np.where(keep, dres * scale_of(p), np.float32(0)).astype(np.float32).tobytes()
+
+
+# ------------------------------------------------------- outputs that are other tensors' copies
+@pytest.mark.parametrize("rows,cols", [(1, 1), (37, 100), (300, 4097), (2, 40000)])
+@pytest.mark.parametrize("shift", [0, 3])
+def test_outputs_given_are_written(tcx, rows, cols, shift):
+    """Without dropout and residual the total is the input, and the input's gradient is the
+    residual's: a C caller may pass NULL for them, and finds them in a buffer that it passes."""
+    from tensorcx_b200 import _abi
+    x, _, w, b = norm_case(rows, cols, False)
+    xd, wd, bd = dev(x, shift), dev(w), dev(b)
+    y, mean, rstd = torch.empty_like(xd), *(torch.empty(rows, device="cuda") for _ in range(2))
+    total, dx, dres = (torch.full_like(xd, float("nan")) for _ in range(3))
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _abi.lib().tcx_sm100_layernorm_forward(
+        stream, xd.data_ptr(), None, wd.data_ptr(), bd.data_ptr(), y.data_ptr(), total.data_ptr(), mean.data_ptr(),
+        rstd.data_ptr(), rows, cols, 1e-5, 0.0, 0, 0, None) == _abi.OK
+    want = tcx.layernorm_forward(xd, wd, bd)
+    assert host(total).tobytes() == x.tobytes()
+    assert all(torch.equal(a, c) for a, c in zip((y, mean, rstd), (want[0], want[2], want[3])))
+    assert _abi.lib().tcx_sm100_layernorm_backward(
+        stream, y.data_ptr(), total.data_ptr(), mean.data_ptr(), rstd.data_ptr(), wd.data_ptr(), None, dres.data_ptr(),
+        dx.data_ptr(), None, None, rows, cols, 0.0, 0, 0, None, None, 0) == _abi.OK
+    assert torch.equal(dx, dres) and torch.isfinite(dx).all()
+    # the input itself as the total's buffer, and the residual's gradient as the input's
+    assert _abi.lib().tcx_sm100_layernorm_forward(
+        stream, xd.data_ptr(), None, wd.data_ptr(), bd.data_ptr(), y.data_ptr(), xd.data_ptr(), mean.data_ptr(),
+        rstd.data_ptr(), rows, cols, 1e-5, 0.0, 0, 0, None) == _abi.OK
+    assert host(xd).tobytes() == x.tobytes() and torch.equal(y, want[0])
