@@ -1,5 +1,5 @@
 """The training operators where their arguments end: places of the random stream at 2^64, outputs
-that a call without dropout need not have.
+that a call without dropout need not have, sums over many rows, buffers at any address.
 
 The masks are compared with the generator's definition in whole-number arithmetic on the host.
 """
@@ -7,9 +7,11 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_training import dev, host, norm_case, scale_of
+from test_gpu_training import check_backward, check_forward, dev, host, keep_of, norm_case, scale_of, within
 
 pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
 
 
 def mask_at(shape, p, seed, offset):
@@ -78,3 +80,62 @@ def test_outputs_given_are_written(tcx, rows, cols, shift):
         stream, xd.data_ptr(), None, wd.data_ptr(), bd.data_ptr(), y.data_ptr(), xd.data_ptr(), mean.data_ptr(),
         rstd.data_ptr(), rows, cols, 1e-5, 0.0, 0, 0, None) == _abi.OK
     assert host(xd).tobytes() == x.tobytes() and torch.equal(y, want[0])
+
+
+# ------------------------------------------------------------------ sums over many rows
+def chain(rows, held):
+    """Roundings that a term of a column's sum goes through: three of its own, the rows of a span
+    of 16 one after the other, the spans' sums of one of the `held` places that work on rows at a
+    time, and those places' sums (a warp to every 8th or more of at most 600, and the warps')."""
+    return 3 + 16 + -(-rows // (16 * held)) + 75 + 5
+
+
+def column_sums(tcx, dy, total, mean, rstd, rows, held):
+    """dweight and dbias against 64 bits; all on the GPU."""
+    w = torch.ones(dy.shape[1], device="cuda")
+    _, _, dw, db = tcx.layernorm_backward(dy, total, mean, rstd, w)
+    exact_w, size_w = (torch.zeros(dy.shape[1], dtype=torch.float64, device="cuda") for _ in range(2))
+    exact_b, size_b = torch.zeros_like(exact_w), torch.zeros_like(exact_w)
+    for i in range(0, rows, 1 << 14):
+        d = dy[i:i + (1 << 14)].double()
+        term = d * (total[i:i + (1 << 14)].double() - mean[i:i + (1 << 14), None]) * rstd[i:i + (1 << 14), None]
+        exact_w += term.sum(0)
+        size_w += term.abs().sum(0)
+        exact_b += d.sum(0)
+        size_b += d.abs().sum(0)
+    k = chain(rows, held)
+    within(host(dw), host(exact_w), k * U * host(size_w), "dweight")
+    within(host(db), host(exact_b), k * U * host(size_b), "dbias")
+
+
+def many_rows(rows, cols, shift, value):
+    """A constant gradient (its roundings all go one way as a sum grows) and random rows."""
+    def at_shift(t):
+        buf = torch.empty(t.numel() + shift, device="cuda")
+        buf[shift:] = t.reshape(-1)
+        return buf[shift:].view(t.shape)
+    make = torch.Generator(device="cuda").manual_seed(rows + cols)
+    total = at_shift(torch.randn(rows, cols, generator=make, device="cuda"))
+    return at_shift(torch.full((rows, cols), value, device="cuda")), total, total.mean(1), 1 / total.std(1, correction=0)
+
+
+@pytest.mark.parametrize("rows,cols,value", [(1000000, 64, 0.1), (700003, 129, 0.7), (1100, 40, 0.1),
+                                             (30000, 4099, 0.3)])
+def test_column_sums_of_many_rows_at_any_address(tcx, rows, cols, value):
+    column_sums(tcx, *many_rows(rows, cols, 1, value), rows, 592 if cols < 256 else 64)
+
+
+@pytest.mark.parametrize("rows,cols", [(3001, 67), (1300, 4097), (1100, 40), (2400, 12)])
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_many_rows_at_any_address(tcx, oracle, rows, cols, shift):
+    """Blocks take several rows in turn, and splits of the rows may be empty."""
+    x, r, w, b = norm_case(rows, cols, True, seed=5)
+    y, total, mean, rstd = tcx.layernorm_forward(dev(x, shift), dev(w), dev(b))
+    check_forward(host(y), host(mean), host(rstd), x, w, b, 1e-5)
+    y, total, mean, rstd = tcx.layernorm_forward(dev(x, shift), dev(w, shift), dev(b), residual=dev(r, shift), p=0.5,
+                                                 seed=2, offset=shift)
+    want = r + np.where(keep_of(oracle, x.shape, 0.5, 2, shift), x * 2, np.float32(0)).astype(np.float32)
+    assert host(total).tobytes() == want.tobytes()
+    check_forward(host(y), host(mean), host(rstd), want, w, b, 1e-5)
+    dy = np.random.default_rng(rows).normal(size=x.shape).astype(np.float32)
+    check_backward(tcx, oracle, dy, want, host(mean), host(rstd), w, x, 0.5, 2, shift, shift=shift)
