@@ -766,7 +766,9 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
         const float* const sum = columns + (i < cols ? i : kMostColumns + i - cols);
         float t = 0.0f;
 #pragma unroll
-        for (int g = 0; g < groups; ++g) t += sum[g * 2 * kMostColumns];
+        for (int g = 0; g < groups; g += 4)
+          t += (sum[g * 2 * kMostColumns] + sum[(g + 1) * 2 * kMostColumns]) +
+               (sum[(g + 2) * 2 * kMostColumns] + sum[(g + 3) * 2 * kMostColumns]);
         partial[at + i] = t;
       }
     }
@@ -774,8 +776,11 @@ norm_backward_kernel(BackwardArgs a, float* partial, int* err) {
 }
 
 // Adds the blocks' column sums: a block to 32 columns, a warp to every WARPS-th of the partial
-// rows, then the warps in order. 32 warps for many partial rows, 8 for few.
-template <int WARPS>
+// rows, then the warps four at a time. 32 warps for many partial rows, 8 for few. LONG: a warp
+// adds 20 of its rows before their sum joins its own, for more than 640 (with that loop the
+// kernel has 46 registers instead of 32: [4096, 8192], 148 partial rows, 76 us against 74).
+constexpr int kTwenty = 20;
+template <int WARPS, bool LONG>
 __global__ void __launch_bounds__(32 * WARPS)
 norm_join_kernel(const float* __restrict__ partial, int splits, int64_t cols, float* dweight, float* dbias) {
   __shared__ float2 sums[WARPS][33];
@@ -783,11 +788,23 @@ norm_join_kernel(const float* __restrict__ partial, int splits, int64_t cols, fl
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   wait_for_prior_grid();
   float2 s = make_float2(0.0f, 0.0f);
+  auto add = [&](float2& t, int i) {
+    t.x += __ldcg(partial + 2 * static_cast<int64_t>(i) * cols + c);
+    t.y += __ldcg(partial + (2 * static_cast<int64_t>(i) + 1) * cols + c);
+  };
   if (c < cols) {
+    if constexpr (LONG) {
+      for (int from = warp; from < splits; from += kTwenty * WARPS) {
+        const int to = min(splits, from + kTwenty * WARPS);
+        float2 t = make_float2(0.0f, 0.0f);
 #pragma unroll 5
-    for (int i = warp; i < splits; i += WARPS) {
-      s.x += __ldcg(partial + 2 * i * cols + c);
-      s.y += __ldcg(partial + (2 * i + 1) * cols + c);
+        for (int i = from; i < to; i += WARPS) add(t, i);
+        s.x += t.x;
+        s.y += t.y;
+      }
+    } else {
+#pragma unroll 5
+      for (int i = warp; i < splits; i += WARPS) add(s, i);
     }
   }
   sums[warp][lane] = s;
@@ -795,15 +812,20 @@ norm_join_kernel(const float* __restrict__ partial, int splits, int64_t cols, fl
   if (warp < 2 && c < cols) {  // a warp to each gradient
     float t = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) t += warp ? sums[w][lane].y : sums[w][lane].x;
+    for (int w = 0; w < WARPS; w += 4) {
+      const float2 q0 = sums[w][lane], q1 = sums[w + 1][lane], q2 = sums[w + 2][lane], q3 = sums[w + 3][lane];
+      t += warp ? (q0.y + q1.y) + (q2.y + q3.y) : (q0.x + q1.x) + (q2.x + q3.x);
+    }
     (warp ? dbias : dweight)[c] = t;
   }
 }
 
 void join_columns(cudaStream_t s, const float* partial, int64_t splits, int64_t cols, float* dweight, float* dbias) {
   const dim3 grid(static_cast<unsigned>(ceil_div(cols, 32)));
-  if (splits > 64) launch_after(norm_join_kernel<32>, grid, dim3(1024), s, 0, partial, splits, cols, dweight, dbias);
-  else launch_after(norm_join_kernel<8>, grid, dim3(256), s, 0, partial, splits, cols, dweight, dbias);
+  auto* kernel = splits > kTwenty * 32 ? norm_join_kernel<32, true>
+                 : splits > 64         ? norm_join_kernel<32, false>
+                                       : norm_join_kernel<8, false>;
+  launch_after(kernel, grid, dim3(splits > 64 ? 1024 : 256), s, 0, partial, splits, cols, dweight, dbias);
 }
 
 // ------------------------------------------------------------------------- launches
@@ -877,11 +899,19 @@ void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool od
   else if constexpr (!FUSED) launch_forward<16, FUSED>(s, a, words, odd);
 }
 
-// Blocks (or clusters) that the backward kernel runs as: what the machine holds at a time, no
-// more than there are rows for; where rows start anywhere in a word, a multiple of
-// 4 (the rows of a group are that far apart).
-int64_t backward_blocks(int64_t rows, int64_t cols, int groups, int resident) {
-  const int64_t want = std::min<int64_t>(ceil_div(rows, groups), resident);
+// Blocks (or clusters) that the backward kernel runs as: what the machine holds at a time, or as
+// many times that as leave a group no more than 128 rows (but for the rounding below): a thread
+// adds its columns over them one after the other, and each row is a rounding of the sum so far
+// ([190000, 8192], a constant gradient: off by 1.9e-5 of the sum with 1284 rows to a block). It
+// costs nothing where an SM holds several blocks ([800000, 1024] 1477 us against 1525 with one
+// round, 1468 with at most 64 rows), the blocks' starts where it holds one ([100000, 8192] 1558
+// against 1505, 1587 with 64; a block of [16384, 4096] has 55 rows). No more blocks than there
+// are rows for; where rows start anywhere in a word, a multiple of 4 (the rows of a group are
+// that far apart).
+constexpr int64_t kMostRows = 128;
+int64_t backward_blocks(int64_t rows, int64_t cols, int groups, int64_t resident) {
+  const int64_t blocks = ceil_div(rows, groups);
+  const int64_t want = std::min(blocks, resident * ceil_div(blocks, resident * kMostRows));
   return cols % 4 == 0 ? want : std::max<int64_t>(4, want / 4 * 4);
 }
 
@@ -902,6 +932,14 @@ BackwardPlan backward_plan(int64_t cols) {
   plan.groups = plan.warps == 1 || plan.warps == 2 || plan.warps == 4 ? 256 / (plan.warps * plan.lanes) : 1;
   plan.per_sm = std::max(1, warps_per_sm(plan.vpt) * 32 / (plan.warps * plan.lanes * plan.groups));
   return plan;
+}
+
+// As many at most, whatever the device holds at a time up to what its registers and memory say:
+// whole rounds of that are fewer than the blocks that kMostRows asks for and one round more.
+int64_t most_blocks(int64_t rows, int64_t cols, const BackwardPlan& plan) {
+  const int64_t places = plan.per_sm * sm_count() / plan.cluster, blocks = ceil_div(rows, plan.groups);
+  const int64_t most = std::min(blocks, ceil_div(blocks, kMostRows) + places);
+  return cols % 4 == 0 ? most : std::max<int64_t>(4, most);
 }
 
 template <int VPT, int WARPS, int LANES, int CLUSTER, bool ODD, bool FUSED>
@@ -1033,7 +1071,7 @@ extern "C" size_t tcx_sm100_layernorm_backward_workspace_bytes(int64_t rows, int
   const BackwardPlan plan = backward_plan(cols);
   int64_t splits = splits_of(rows, cols);
   if (plan.vpt)
-    splits = std::max(splits, backward_blocks(rows, cols, plan.groups, plan.per_sm * sm_count() / plan.cluster));
+    splits = std::max(splits, most_blocks(rows, cols, plan));
   return static_cast<size_t>(splits) * 2 * cols * sizeof(float);
 }
 

@@ -84,13 +84,21 @@ def test_outputs_given_are_written(tcx, rows, cols, shift):
 
 # ------------------------------------------------------------------ sums over many rows
 def chain(rows, held):
-    """Roundings that a term of a column's sum goes through: three of its own, the rows of a span
-    of 16 one after the other, the spans' sums of one of the `held` places that work on rows at a
-    time, and those places' sums (a warp to every 8th or more of at most 600, and the warps')."""
-    return 3 + 16 + -(-rows // (16 * held)) + 75 + 5
+    """Roundings that a term of a column's sum goes through where the sums are a pass of their own:
+    three of its own, the rows of a span of 16 one after the other, the spans' sums of one of the
+    `held` parts of the rows, and the parts' sums (at most 592, by 32 warps, then theirs)."""
+    return 3 + 16 + -(-rows // (16 * held)) + 19 + 10
 
 
-def column_sums(tcx, dy, total, mean, rstd, rows, held):
+def chain_in_registers(rows, held):
+    """The same where they are added on the way: three of its own, a group of warps' 128 rows (144
+    where the blocks are a multiple of four), the sums of up to 32 groups, and the blocks' (20 of
+    a warp's every 32nd, the twenties, and the warps')."""
+    blocks = max(600, rows // 128 + 600)
+    return 3 + min(144, -(-rows // held)) + 10 + 20 + -(-blocks // 640) + 10
+
+
+def column_sums(tcx, dy, total, mean, rstd, rows, k):
     """dweight and dbias against 64 bits; all on the GPU."""
     w = torch.ones(dy.shape[1], device="cuda")
     _, _, dw, db = tcx.layernorm_backward(dy, total, mean, rstd, w)
@@ -103,7 +111,6 @@ def column_sums(tcx, dy, total, mean, rstd, rows, held):
         size_w += term.abs().sum(0)
         exact_b += d.sum(0)
         size_b += d.abs().sum(0)
-    k = chain(rows, held)
     within(host(dw), host(exact_w), k * U * host(size_w), "dweight")
     within(host(db), host(exact_b), k * U * host(size_b), "dbias")
 
@@ -122,7 +129,7 @@ def many_rows(rows, cols, shift, value):
 @pytest.mark.parametrize("rows,cols,value", [(1000000, 64, 0.1), (700003, 129, 0.7), (1100, 40, 0.1),
                                              (30000, 4099, 0.3)])
 def test_column_sums_of_many_rows_at_any_address(tcx, rows, cols, value):
-    column_sums(tcx, *many_rows(rows, cols, 1, value), rows, 592 if cols < 256 else 64)
+    column_sums(tcx, *many_rows(rows, cols, 1, value), rows, chain(rows, 592 if cols < 256 else 64))
 
 
 @pytest.mark.parametrize("rows,cols", [(3001, 67), (1300, 4097), (1100, 40), (2400, 12)])
@@ -139,3 +146,13 @@ def test_many_rows_at_any_address(tcx, oracle, rows, cols, shift):
     check_forward(host(y), host(mean), host(rstd), want, w, b, 1e-5)
     dy = np.random.default_rng(rows).normal(size=x.shape).astype(np.float32)
     check_backward(tcx, oracle, dy, want, host(mean), host(rstd), w, x, 0.5, 2, shift, shift=shift)
+
+
+@pytest.mark.parametrize("rows,cols,held,value", [
+    (18000000, 8, 14208, 0.8738095), (6000000, 100, 4736, 0.8738095), (3000001, 509, 2368, 0.8738095),
+    (1500000, 1024, 1184, 0.8738095), (750000, 2050, 592, 0.8738095), (190001, 4100, 148, 0.8738095),
+    (190000, 8192, 148, 0.8738095), (70000, 16388, 32, 0.8738095), (2369, 512, 2368, 0.1), (20000, 4097, 148, 0.7)])
+def test_column_sums_of_many_rows(tcx, rows, cols, held, value):
+    """More than a thousand rows to each place that the GPU has for them, and a few."""
+    column_sums(tcx, *many_rows(rows, cols, 0, value), rows, chain_in_registers(rows, held))
+    torch.cuda.empty_cache()
