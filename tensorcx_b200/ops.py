@@ -817,11 +817,12 @@ def layernorm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias:
 
 def layernorm_backward(dy: torch.Tensor, total: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
                        weight: torch.Tensor | None = None, *, dtotal: torch.Tensor | None = None, p: float = 0.0,
-                       seed: int | None = None, offset=0):
+                       seed: int | None = None, offset=0, params: bool | None = None):
     """The gradients of layernorm_forward from what it returned: (dx, dresidual, dweight,
     dbias). dresidual is the gradient of total (dtotal, what reaches total by other ways,
-    added), and dx the same through the dropout: with p = 0 both are one tensor. Without a
-    weight dweight and dbias are None. Sums over rows have a fixed order."""
+    added), and dx the same through the dropout: with p = 0 both are one tensor. dweight and
+    dbias come with a weight, or as `params` says: True for both without a weight too (a norm
+    with a bias alone), False for None in their places. Sums over rows have a fixed order."""
     index = _leading("total", total)
     shape = total.shape
     if not shape or shape[-1] == 0:
@@ -831,6 +832,10 @@ def layernorm_backward(dy: torch.Tensor, total: torch.Tensor, mean: torch.Tensor
         raise TypeError("layernorm_backward needs dy, mean and rstd")
     _floats(index, shape, "dy", dy, "dtotal", dtotal)
     _floats(index, shape[:-1], "mean", mean, "rstd", rstd)
+    if params is None:
+        params = weight is not None
+    elif not isinstance(params, bool):
+        raise TypeError("params must be a bool or None")
     p, seed, offset, step = _dropout_stream(p, seed, offset, index)
     rows = total.numel() // cols
     dresidual = _new_like(total)
@@ -839,7 +844,9 @@ def layernorm_backward(dy: torch.Tensor, total: torch.Tensor, mean: torch.Tensor
     ws_bytes = 0
     if weight is not None:
         _floats(index, (cols,), "weight", weight)
-        dweight, dbias = _new_like(weight), _new_like(weight)
+    if params:
+        dweight = total.new_empty(cols) if weight is None else _new_like(weight)
+        dbias = _new_like(dweight)
         ws_bytes = lib().tcx_sm100_layernorm_backward_workspace_bytes(rows, cols)
         keep, ws = _workspace(ws_bytes, total.device)
     check(lib().tcx_sm100_layernorm_backward(

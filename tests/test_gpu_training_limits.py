@@ -156,3 +156,30 @@ def test_column_sums_of_many_rows(tcx, rows, cols, held, value):
     """More than a thousand rows to each place that the GPU has for them, and a few."""
     column_sums(tcx, *many_rows(rows, cols, 0, value), rows, chain_in_registers(rows, held))
     torch.cuda.empty_cache()
+
+
+# -------------------------------------------------------------- gradients of a bias alone
+@pytest.mark.parametrize("rows,cols,shift", [(300, 260, 0), (37, 4096, 0), (90, 33, 1), (0, 12, 0)])
+def test_parameter_gradients_are_a_choice(tcx, rows, cols, shift):
+    """params=True gives both sums without a weight (a norm with a bias alone), the same as with
+    a weight of ones; params=False leaves them out (frozen parameters)."""
+    x, _, w, b = norm_case(rows, cols, False)
+    xd, wd, bd = dev(x, shift), dev(w), dev(b)
+    dy = dev(np.random.default_rng(rows).normal(size=x.shape).astype(np.float32), shift)
+    y, total, mean, rstd = tcx.layernorm_forward(xd, None, bd)
+    ones = torch.ones(cols, device="cuda")
+    want = tcx.layernorm_backward(dy, total, mean, rstd, ones)
+    got = tcx.layernorm_backward(dy, total, mean, rstd, params=True)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    hat = (x.astype(np.float64) - host(mean)[:, None]) * host(rstd)[:, None]
+    d = host(dy).astype(np.float64)
+    within(host(got[2]), (d * hat).sum(0), (rows + 8) * U * np.abs(d * hat).sum(0), "dweight")
+    within(host(got[3]), d.sum(0), (rows + 8) * U * np.abs(d).sum(0), "dbias")
+    none = tcx.layernorm_backward(dy, total, mean, rstd)
+    assert none[2] is None and none[3] is None and torch.equal(none[0], got[0])
+    frozen = tcx.layernorm_backward(dy, total, mean, rstd, wd, params=False)
+    with_them = tcx.layernorm_backward(dy, total, mean, rstd, wd)
+    assert frozen[2] is None and frozen[3] is None and torch.equal(frozen[0], with_them[0])
+    assert with_them[2] is not None and with_them[3] is not None
+    with pytest.raises(TypeError, match="params"):
+        tcx.layernorm_backward(dy, total, mean, rstd, wd, params=1)
