@@ -853,8 +853,9 @@ void launch_staged(cudaStream_t s, const ForwardArgs& a, int warps) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         (BLOCKS == 2 ? kPairWarps : kMostWarps) * kWarpBytes);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (BLOCKS == 2 ? kPairWarps : kMostWarps) * kWarpBytes) != cudaSuccess)
+      return;  // the call's error
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
   const int64_t grid = std::min<int64_t>(a.rows, BLOCKS * sm_count());
@@ -961,13 +962,17 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64) held = resident[dev][plan.warps];
   if (held == 0) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         Places<VPT, WARPS, ODD, FUSED>::bytes(kMostWarps * 32));
+    // a lookup that fails is not kept, and its error is the call's: nothing is launched
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Places<VPT, WARPS, ODD, FUSED>::bytes(kMostWarps * 32)) != cudaSuccess)
+      return 0;
     held = plan.per_sm * sm_count() / CLUSTER;
-    cfg.gridDim = dim3(static_cast<unsigned>(held * CLUSTER));
-    int clusters = 0;
-    if (CLUSTER > 1 && cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0)
-      held = std::min(held, clusters);
+    if (CLUSTER > 1) {
+      cfg.gridDim = dim3(static_cast<unsigned>(held * CLUSTER));
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) return 0;
+      held = std::max(1, std::min(held, clusters));
+    }
     if (dev >= 0 && dev < 64) resident[dev][plan.warps] = held;
   }
   const int64_t blocks = backward_blocks(a.rows, a.cols, plan.groups, held);
@@ -986,7 +991,7 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
                : launch_backward<VPT, WARPS, LANES, CLUSTER, false, false>(s, a, partial, plan);
 }
 
-// Returns the partial rows that it leaves.
+// Returns the partial rows that it leaves, or 0 with the runtime's error set.
 int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, const BackwardPlan& plan, bool odd) {
   switch (plan.cluster) {
     case 4: return launch_backward<4, 0, 32, 4>(s, a, partial, plan, odd);
@@ -1105,6 +1110,7 @@ extern "C" int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy
   const BackwardPlan plan = backward_plan(cols);
   if (plan.vpt && aligned(dy) && aligned(total) && aligned(dtotal) && aligned(dresidual) && aligned(a.dx)) {
     const int64_t splits = launch_backward(s, a, partial, plan, cols % 4 != 0 || !aligned(weight));
+    if (splits == 0) return launch_status("layer norm backward");
     if (partial) join_columns(s, partial, splits, cols, dweight, dbias);
   } else {
     const int grid = static_cast<int>(std::min<int64_t>(rows, 8 * sm_count()));
