@@ -26,6 +26,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "dropout.cuh"
@@ -849,14 +850,14 @@ template <int VPT, int BLOCKS, bool ODD, bool FUSED>
 void launch_staged(cudaStream_t s, const ForwardArgs& a, int warps) {
   auto* kernel = norm_forward_kernel<VPT, 0, 32, ODD, FUSED, BLOCKS>;
   constexpr int kWarpBytes = (FUSED ? 2 : 1) * 32 * VPT * 16;
-  static bool attr_done[64] = {false};
+  static std::atomic<bool> attr_done[64];  // host threads may meet here
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+  if (dev < 0 || dev >= 64 || !attr_done[dev].load(std::memory_order_relaxed)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (BLOCKS == 2 ? kPairWarps : kMostWarps) * kWarpBytes) != cudaSuccess)
       return;  // the call's error
-    if (dev >= 0 && dev < 64) attr_done[dev] = true;
+    if (dev >= 0 && dev < 64) attr_done[dev].store(true, std::memory_order_relaxed);
   }
   const int64_t grid = std::min<int64_t>(a.rows, BLOCKS * sm_count());
   kernel<<<static_cast<unsigned>(grid), 32 * warps, warps * kWarpBytes, s>>>(a);
@@ -956,11 +957,12 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
   attr[0].val.clusterDim = {CLUSTER, 1, 1};
   cfg.attrs = attr;
   cfg.numAttrs = CLUSTER > 1 ? 1 : 0;
-  // how many blocks or clusters the device holds at a time, looked up once for each size
-  static int resident[64][kMostWarps + 1] = {};
+  // how many blocks or clusters the device holds at a time, looked up once for each size (or by
+  // each of two host threads that meet here)
+  static std::atomic<int> resident[64][kMostWarps + 1];
   int dev = 0, held = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64) held = resident[dev][plan.warps];
+  if (dev >= 0 && dev < 64) held = resident[dev][plan.warps].load(std::memory_order_relaxed);
   if (held == 0) {
     // a lookup that fails is not kept, and its error is the call's: nothing is launched
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -973,7 +975,7 @@ int64_t launch_backward(cudaStream_t s, const BackwardArgs& a, float* partial, c
       if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) return 0;
       held = std::max(1, std::min(held, clusters));
     }
-    if (dev >= 0 && dev < 64) resident[dev][plan.warps] = held;
+    if (dev >= 0 && dev < 64) resident[dev][plan.warps].store(held, std::memory_order_relaxed);
   }
   const int64_t blocks = backward_blocks(a.rows, a.cols, plan.groups, held);
   cfg.gridDim = dim3(static_cast<unsigned>(blocks * CLUSTER));

@@ -28,6 +28,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -878,13 +879,13 @@ int launch_scan(cudaStream_t s, const Args& a, int threads, int bytes, int per_s
   sc.tiles = static_cast<unsigned>(tiles);
   sc.records = whole ? nullptr : static_cast<Record*>(workspace);
   sc.ticket = whole ? nullptr : reinterpret_cast<unsigned*>(sc.records + tiles * kWide);
-  static bool attr_done[64] = {false};
+  static std::atomic<bool> attr_done[64];  // host threads may meet here
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+  if (dev < 0 || dev >= 64 || !attr_done[dev].load(std::memory_order_relaxed)) {
     if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return launch_status("recurrence shared memory attribute");
-    if (dev >= 0 && dev < 64) attr_done[dev] = true;
+    if (dev >= 0 && dev < 64) attr_done[dev].store(true, std::memory_order_relaxed);
   }
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(whole ? sc.chains : tiles, per_sm * sm_count())));
   if (whole) {

@@ -1,8 +1,11 @@
 """The training operators where their arguments end: places of the random stream at 2^64, outputs
-that a call without dropout need not have, sums over many rows, buffers at any address.
+that a call without dropout need not have, sums over many rows, buffers at any address,
+host threads and streams.
 
 The masks are compared with the generator's definition in whole-number arithmetic on the host.
 """
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -183,3 +186,43 @@ def test_parameter_gradients_are_a_choice(tcx, rows, cols, shift):
     assert with_them[2] is not None and with_them[3] is not None
     with pytest.raises(TypeError, match="params"):
         tcx.layernorm_backward(dy, total, mean, rstd, wd, params=1)
+
+
+# ---------------------------------------------------------------- host threads and streams
+def one_of_each(tcx, seed, cols):
+    """Every operator once, from inputs of the seed; long rows, clusters and scans among them."""
+    make = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=make, device="cuda")
+    x, r, w = normal(61, cols), normal(61, cols), normal(cols)
+    y, total, mean, rstd = tcx.layernorm_forward(x, w, w, residual=r, p=0.2, seed=seed)
+    out = [tcx.dropout(x, 0.3, seed), y, total, mean, rstd, *tcx.layernorm_forward(x, w)[::2]]
+    out += tcx.layernorm_backward(y, total, mean, rstd, w, dtotal=r, p=0.2, seed=seed)
+    gate, xs, dh = (normal(2, 700, cols // 64) for _ in range(3))
+    h, state = tcx.gated_recurrence(gate, xs, form="sigmoid")
+    return out + [h, state, *tcx.gated_recurrence_backward(dh, gate, xs, h, form="sigmoid")[:2]]
+
+
+def test_host_threads_on_streams_of_their_own(tcx):
+    """Four threads at a time, each on a side stream, get what one gets on the usual stream."""
+    cols = [520, 9001, 12288, 17000]
+    got, errors = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[i] = [one_of_each(tcx, 10 * i + j, cols[(i + j) % 4]) for j in range(8)]
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 (a thread's failure is the test's)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i in range(4):
+        for j in range(8):
+            want = one_of_each(tcx, 10 * i + j, cols[(i + j) % 4])
+            assert all(torch.equal(a, b) for a, b in zip(got[i][j], want)), (i, j)
