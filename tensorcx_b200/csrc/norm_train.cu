@@ -874,12 +874,14 @@ void launch_staged(cudaStream_t s, const ForwardArgs& a, int warps) {
 template <int VPT, bool FUSED>
 void launch_forward(cudaStream_t s, const ForwardArgs& a, int64_t words, bool odd) {
   const int warps = static_cast<int>(ceil_div(words, 32 * VPT));
-  if (warps >= kStagedWarps && odd) launch_staged<VPT, true, FUSED>(s, a, warps);
-  else if (warps >= kStagedWarps) launch_staged<VPT, false, FUSED>(s, a, warps);
-  else if (warps == 1) launch_forward<VPT, 1, 32, FUSED>(s, a, warps, odd);
-  else if (warps == 2) launch_forward<VPT, 2, 32, FUSED>(s, a, warps, odd);
-  else if (warps == 4) launch_forward<VPT, 4, 32, FUSED>(s, a, warps, odd);
-  else launch_forward<VPT, 0, 32, FUSED>(s, a, warps, odd);
+  if (warps >= kStagedWarps && odd) return launch_staged<VPT, true, FUSED>(s, a, warps);
+  if (warps >= kStagedWarps) return launch_staged<VPT, false, FUSED>(s, a, warps);
+  if (warps == 1) return launch_forward<VPT, 1, 32, FUSED>(s, a, warps, odd);
+  if constexpr (VPT < 16) {  // 513 to 1024 words are never 16 to a thread
+    if (warps == 2) return launch_forward<VPT, 2, 32, FUSED>(s, a, warps, odd);
+  }
+  if (warps == 4) return launch_forward<VPT, 4, 32, FUSED>(s, a, warps, odd);
+  launch_forward<VPT, 0, 32, FUSED>(s, a, warps, odd);
 }
 
 // 32 values to a thread, of each of two inputs where there are two. Where there are rows to
