@@ -482,11 +482,13 @@ int tcx_sm100_dropout(tcx_stream_t stream, const float* input, const float* resi
  *   mean[r] = mean of row r,  rstd[r] = 1 / sqrt(variance of row r + epsilon)
  *   output = (total - mean) * rstd * weight + bias      (weight, bias [cols] or NULL)
  * A total that is given and equals input is copied there (total may be input itself).
- * The variance is the biased one, computed about the mean; a row's differences from its
- * first element must be representable. A constant finite row of input (without dropout)
- * gives exactly 0 * weight + bias, NaN when epsilon is 0. A row that holds a NaN or an
- * infinity is NaN, and no other is. With cols a multiple of 4 a row's bits do not depend
- * on its place among the rows. */
+ * The variance is the biased one, computed about the mean in float32: a row's differences
+ * from its first element, their sum and the sum of the squared deviations from the mean
+ * must be representable (the root of that sum below 1.8e19), else mean, rstd and output of
+ * the row are inf, NaN or 0 * weight + bias. A constant finite row of input (without
+ * dropout) gives exactly 0 * weight + bias, NaN when epsilon is 0. A row that holds a NaN
+ * or an infinity is NaN, and no row within that range is. With cols a multiple of 4 a
+ * row's bits do not depend on its place among the rows. */
 int tcx_sm100_layernorm_forward(tcx_stream_t stream, const float* input, const float* residual, const float* weight,
                                 const float* bias, float* output, float* total, float* mean, float* rstd,
                                 int64_t rows, int64_t cols, float epsilon, double p, uint64_t seed, uint64_t offset,

@@ -794,7 +794,8 @@ def layernorm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias:
     """Layer norm over the last axis for training, in one pass with what stands in front of
     it: total = residual + dropout(x), y = (total - mean) * rstd * weight + bias. Returns
     (y, total, mean, rstd); mean and rstd have x's shape without its last axis, and total
-    is x itself without a residual and with p = 0. p, seed and offset as for dropout."""
+    is x itself without a residual and with p = 0. p, seed and offset as for dropout. Sums
+    are float32: the root of a row's summed squared deviations must stay below 1.8e19."""
     index = _leading("x", x)
     shape = x.shape
     if not shape or shape[-1] == 0:

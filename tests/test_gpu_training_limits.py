@@ -1,5 +1,5 @@
 """The training operators where their arguments end: places of the random stream at 2^64, outputs
-that a call without dropout need not have, sums over many rows, buffers at any address,
+that a call without dropout need not have, sums over many rows, rows of the widest spread, buffers at any address,
 host threads and streams.
 
 The masks are compared with the generator's definition in whole-number arithmetic on the host.
@@ -159,6 +159,22 @@ def test_column_sums_of_many_rows(tcx, rows, cols, held, value):
     """More than a thousand rows to each place that the GPU has for them, and a few."""
     column_sums(tcx, *many_rows(rows, cols, 0, value), rows, chain_in_registers(rows, held))
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------- wide rows
+@pytest.mark.parametrize("cols", [2, 40, 1024, 5000, 16384, 40000])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_norm_of_rows_of_the_widest_spread(tcx, cols, shift):
+    """Deviations whose squares sum to half of what a float32 holds, about levels near and far,
+    next to an ordinary row."""
+    t = np.random.default_rng(cols).normal(size=(4, cols))
+    t -= t.mean(1, keepdims=True)
+    t *= np.sqrt(1.7e38) / np.sqrt((t * t).sum(1, keepdims=True))
+    t[1] += 1e19
+    t[2] *= 1e-19
+    t = t.astype(np.float32)
+    y, _, mean, rstd = tcx.layernorm_forward(dev(t, shift))
+    check_forward(host(y), host(mean), host(rstd), t, None, None, 1e-5)
 
 
 # -------------------------------------------------------------- gradients of a bias alone
