@@ -515,9 +515,12 @@ int tcx_sm100_layernorm_backward(tcx_stream_t stream, const float* dy, const flo
  * from initial [batch, channels] (NULL: zeros). lengths (NULL, or batch device int32, taken
  * as clamped to [0, time]): steps at and beyond a sequence's length hold its state,
  * h_t = h_(t-1), whatever gate and x hold there. h receives every state; state (NULL or
- * [batch, channels]) the last one. Long sequences are cut into parts that are joined by
- * (product of gates, state from zero): the products must be representable, as they are
- * for gates of magnitude up to 1. */
+ * [batch, channels]) the last one. Sequences of more than 16 steps may be cut into parts
+ * of up to 128 that are joined by (product of gates, state from zero), by a rule on batch,
+ * time and channels. So for more than 16 steps the products of up to 128 consecutive gates
+ * must be representable, here and in the gradient: those of gates of magnitude below 2
+ * are. Where one is not, later states may be inf or NaN although each h_t would be finite.
+ * Calls of up to 16 steps multiply no gates with one another. */
 enum { TCX_RECURRENCE_DECAY = 0, TCX_RECURRENCE_SIGMOID = 1 };
 size_t tcx_sm100_recurrence_workspace_bytes(int64_t batch, int64_t time, int64_t channels);
 int tcx_sm100_recurrence_forward(tcx_stream_t stream, int form, const float* gate, const float* x,

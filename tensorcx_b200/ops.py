@@ -890,7 +890,9 @@ def gated_recurrence(gate: torch.Tensor, x: torch.Tensor, initial: torch.Tensor 
     (zeros without one). `lengths` (int32 [batch], clamped to [0, time]): steps that a
     sequence does not have hold its state, whatever gate and x hold there. Returns (h,
     state): every state, and the last one to go on from. With one step (a token of each
-    running sequence) state is a view of h."""
+    running sequence) state is a view of h: change h in place only when the state has been
+    used. Over more than 16 steps the products of up to 128 consecutive gates must be
+    representable, as those of gates of magnitude below 2 are."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a tensor")
     index, kind, shape, ends = _recurrence_args(gate, form, lengths, "x", x)

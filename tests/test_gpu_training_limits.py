@@ -1,6 +1,6 @@
 """The training operators where their arguments end: places of the random stream at 2^64, outputs
-that a call without dropout need not have, sums over many rows, rows of the widest spread, buffers at any address,
-host threads and streams.
+that a call without dropout need not have, sums over many rows, rows of the widest spread, the largest gates,
+buffers at any address, host threads and streams.
 
 The masks are compared with the generator's definition in whole-number arithmetic on the host.
 """
@@ -10,7 +10,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_training import check_backward, check_forward, dev, host, keep_of, norm_case, scale_of, within
+from test_gpu_training import (check_backward, check_forward, dev, host, keep_of, norm_case,
+                               recurrence_case, roundings, scale_of, scan, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -202,6 +203,33 @@ def test_parameter_gradients_are_a_choice(tcx, rows, cols, shift):
     assert with_them[2] is not None and with_them[3] is not None
     with pytest.raises(TypeError, match="params"):
         tcx.layernorm_backward(dy, total, mean, rstd, wd, params=1)
+
+
+# ---------------------------------------------------------------------------- large gates
+@pytest.mark.parametrize("batch,time,channels", [(2, 512, 33), (1, 700, 128), (400, 128, 512), (300, 256, 32)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_recurrence_gates_of_the_largest_products(tcx, batch, time, channels, sign):
+    """128 gates of 1.99 in a row, in one chunk or across two, whose product (1.8e38) a float32
+    just holds; the states around them are tiny. h, dx and dinitial (a gate's gradient is a
+    product of two such numbers, and leaves float32's range)."""
+    gate, x, init, dh, dstate = recurrence_case(batch, time, channels, "decay", seed=11)
+    gate *= np.float32(0.5)
+    first = (time - 128) // 256 * 128  # a chunk's first step forward, within two backward
+    gate[:, first:first + 128, ::2] = sign * np.float32(1.99)
+    gate[:, (time - 128) // 2:(time - 128) // 2 + 128, 1::2] = sign * np.float32(1.99)
+    x, init, dh, dstate = (v * np.float32(1e-25) for v in (x, init, dh, dstate))
+    a, kappa, every = gate.astype(np.float64), roundings(gate, "decay"), np.ones((batch, time), bool)
+    want, bound = scan(a, x.astype(np.float64), init, every, kappa)
+    h, state = tcx.gated_recurrence(dev(gate), dev(x), dev(init))
+    within(host(h), want, bound, "h")
+    within(host(state), want[:, -1], bound[:, -1], "state")
+    _, dx, dinit = tcx.gated_recurrence_backward(dev(dh), dev(gate), None, h, dev(init), dstate=dev(dstate))
+    back, d = slice(None, None, -1), dh.astype(np.float64)
+    c, off = (v[:, back] for v in scan(a[:, back], (a * d)[:, back], dstate, every, kappa))
+    after = np.concatenate([c[:, 1:], dstate[:, None].astype(np.float64)], 1)
+    off_after = np.concatenate([off[:, 1:], np.zeros((batch, 1, channels))], 1)
+    within(host(dx), d + after, off_after + 2 * U * (np.abs(d) + np.abs(after)), "dx")
+    within(host(dinit), c[:, 0], off[:, 0] + U * np.abs(c[:, 0]), "dinitial")
 
 
 # ---------------------------------------------------------------- host threads and streams
