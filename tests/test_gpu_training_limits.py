@@ -10,8 +10,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_training import (check_backward, check_forward, dev, host, keep_of, norm_case,
-                               recurrence_case, roundings, scale_of, scan, within)
+from test_gpu_training import (check_backward, check_forward, check_recurrence, dev, host, keep_of,
+                               live_steps, norm_case, recurrence_case, roundings, scale_of, scan, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -230,6 +230,48 @@ def test_recurrence_gates_of_the_largest_products(tcx, batch, time, channels, si
     off_after = np.concatenate([off[:, 1:], np.zeros((batch, 1, channels))], 1)
     within(host(dx), d + after, off_after + 2 * U * (np.abs(d) + np.abs(after)), "dx")
     within(host(dinit), c[:, 0], off[:, 0] + U * np.abs(c[:, 0]), "dinitial")
+
+
+# ------------------------------------------------- sequences in buffers at any address
+@pytest.mark.parametrize("form", ["decay", "sigmoid"])
+@pytest.mark.parametrize("batch,time,channels,shift", [(250, 140, 21, 1), (1, 5000, 40, 1), (300, 300, 32, 2),
+                                                       (5, 1700, 33, 3), (700, 100, 301, 1), (2, 40, 64, 1)])
+def test_sequences_at_any_address(tcx, form, batch, time, channels, shift):
+    """Whole chains to a block, a walk back over more than 8 chunks, a thread to a channel, with
+    lengths that end anywhere, none, or past the end."""
+    gate, x, init, dh, dstate = recurrence_case(batch, time, channels, form, seed=12)
+    lengths = np.random.default_rng(time).integers(-1, time + 2, batch)
+    lengths[:1] = time - 1
+    pad = ~live_steps(batch, time, lengths)
+    gate[pad], x[pad] = np.nan, np.inf
+    check_recurrence(tcx, gate, x, init, dh, dstate, form, lengths, shift=shift)
+    h, _ = tcx.gated_recurrence(dev(gate, shift), dev(x, shift), dev(init, shift), form=form,
+                                lengths=dev(lengths.astype(np.int32)))
+    h = host(h)
+    for b, n in enumerate(np.clip(lengths, 0, time)):
+        assert (h[b, n:] == (h[b, n - 1] if n else init[b])).all()
+
+
+# --------------------------------------------------------------- NaN in front of a norm
+@pytest.mark.parametrize("rows,cols,shift", [(40, 36, 0), (12, 1000, 0), (9, 4099, 0), (7, 10000, 0), (5, 20000, 0),
+                                             (6, 100, 1)])
+def test_norm_of_rows_with_nan_under_dropout(tcx, rows, cols, shift):
+    """A NaN or an infinity makes its row NaN where it is kept and nothing where it is dropped."""
+    p, seed = 0.5, 31
+    x, r, w, b = norm_case(rows, cols, True)
+    keep = mask_at(x.shape, p, seed, 3)
+    hit = [(i, [0, cols // 2, cols - 1][i % 3]) for i in range(0, rows, 2)]
+    for i, c in hit:
+        x[i, c] = [np.nan, np.inf, -np.inf][i % 3]
+    bad = np.array([any(i == j and keep[i, c] for i, c in hit) for j in range(rows)])
+    for res in (None, r):
+        y, total, mean, rstd = tcx.layernorm_forward(dev(x, shift), dev(w), dev(b), p=p, seed=seed, offset=3,
+                                                     residual=None if res is None else dev(res, shift))
+        with np.errstate(invalid="ignore"):
+            want = np.where(keep, x * scale_of(p), np.float32(0)).astype(np.float32)
+        want = want if res is None else res + want
+        assert np.isnan(host(y)[bad]).all()
+        check_forward(host(y)[~bad], host(mean)[~bad], host(rstd)[~bad], want[~bad], w, b, 1e-5)
 
 
 # ---------------------------------------------------------------- host threads and streams
