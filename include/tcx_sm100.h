@@ -458,7 +458,9 @@ int tcx_sm100_embedding(tcx_stream_t stream, const int32_t* indices, int64_t row
 /* ----------------------------------------------------------------- training --- */
 /* Operators that a model learns with; the reference, an inference runtime, has no
  * counterpart of them. float32; statistics, sums and states are held in 32 bits.
- * Outputs must not overlap inputs unless a declaration says so.
+ * Outputs must not overlap inputs unless a declaration says so. Buffers may start anywhere;
+ * those that do not start on a 16-byte boundary are taken element by element, some 2 to 30
+ * times slower.
  *
  * Random masks: element e of a call takes place offset + e of the seed's uniform stream
  * (tcx_sm100_random, UNIFORM on [0, 1)) and is kept when its value is at least p, a

@@ -1,8 +1,9 @@
 // The dropout map shared by the elementwise kernel (dropout.cu) and the norm kernels that
 // apply it on the way (norm_train.cu). Element e of a call is kept when the uniform value of
 // place start + e in the seed's stream, a whole number w of 24 bits times 2^-24, is at least
-// p: w >= threshold = ceil(p * 2^24), so the mask equals rand_uniform(...) >= p exactly. The
-// mask is a function of (seed, place): nothing stores it, the backward pass makes it again.
+// p: w >= threshold = ceil(p * 2^24), so the mask equals rand_uniform(...) >= p with p as the
+// 64-bit number that it is (rounded to 32 bits first, a p above 1/2 may move by one of the 2^24
+// values). The mask is a function of (seed, place): nothing stores it, the backward pass makes it again.
 // A kept element is multiplied by scale = 1 / (1 - p) rounded to float32; a dropped one is 0
 // whatever it held (infinities and NaN included).
 #pragma once

@@ -16,11 +16,13 @@
 // dropout in front f is the residual's first element.) All sums are float32.
 //
 // Bound by memory: 8 bytes an element forward and 12 backward, 16 and 20 with the dropout and
-// the residual. Measured on one B200 (those bytes over the call's time, against a copy's 6.55
-// TB/s): [16384, 4096] forward 88 us (0.93), with dropout and residual 170 us (0.96), backward
-// 131 us (0.94; its first kernel 120 us), with dropout and residual 216 us (0.95); [16383, 4095]
-// with both forward 202 us (0.81), backward plain 162 us (0.76); [2048, 32768] backward 157 us
-// (0.78), forward 119 us (0.69); [65536, 256] backward 42 us (0.73).
+// the residual. Measured on one B200, calls back to back on changing inputs (those bytes over the
+// call's time, against a copy's 6.55 TB/s): [16384, 4096] forward 90 us (0.91), with dropout and
+// residual 182 us (0.90), backward 131 us (0.94; its first kernel 120 us), with dropout and residual
+// 229 us (0.89); [16383, 4095] with both forward 214 us (0.76), backward plain 159 us (0.77);
+// [2048, 32768] backward 167 us (0.74), forward 118 us (0.69), with both 243 us (0.67); [65536, 256]
+// backward 39 us (0.78). Where a comment below gives two figures for a choice, they were taken side
+// by side when it was made.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -41,7 +43,10 @@ using rowmath::Block;
 // ------------------------------------------------------------------------ any row
 // For buffers that are not 16-byte aligned and rows longer than the kernels below hold (32768
 // forward, 65536 backward): an element to a thread, a row's block reading it again for each
-// of its sums and once more for its outputs, and the columns' sums in a pass of their own.
+// of its sums and once more for its outputs, and the columns' sums in a pass of their own. One
+// element off the alignment [16384, 4096] takes 155 us forward and 516 with dropout and residual,
+// 301 and 636 backward; [500000, 64], a block to each short row, 1634 and 1575 us; [2048, 70001],
+// aligned or not, 638 and 1138.
 constexpr int kThreads = 256;
 
 struct ForwardArgs {
@@ -252,6 +257,9 @@ constexpr int resident_threads(int vpt, bool fused) {
 // What their registers are bounded by. Blocks of any number of warps as if they were as large as
 // that: 64 registers for 8 words of one input, 80 for 16 (an SM holds 3 blocks of 8 warps instead
 // of two: [4096, 16384] 110 -> 98 us), 96 for 8 of two ([9500, 6001] 207 -> 177; 80 are too few).
+// Some kernels spill 4 to 36 bytes a thread for it. Fused short rows, with the registers not to
+// (512 threads to an SM for 4 words, 768 for fewer): [200000, 100] 74 us against 62, [100000, 401]
+// 160 against 150, [500000, 64] 105 against 94, [600000, 33] 107 against 103.
 constexpr int bound_threads(int vpt, int warps, bool fused, int staged) {
   if (staged == 2) return 32 * kPairWarps;
   if (staged || warps) return most_threads(warps);
@@ -440,8 +448,11 @@ norm_forward_kernel(ForwardArgs a) {
 // rows to a block at a time where they are short, a group of warps to each. A group's rows are
 // a multiple of 4 apart, so that they all start at the same place of a word and a thread's
 // columns are the same in each: the weight's and the bias's gradients add up in its registers
-// over the group's rows, the groups' in shared memory, and the blocks' in a second kernel, each
-// in a fixed order.
+// over the group's rows (at most 128: see kMostRows), the groups' in shared memory, and the blocks'
+// in a second kernel, each in a fixed order. A chain of additions that long is what the sums' error
+// is: 1.6e-7 (2-norm) with 55 rows at [16384, 4096], where torch's sum over the rows has 1.4e-7, and
+// half of torch's at [65536, 256]. Joining spans of 16 rows on the way costs more than it gives:
+// through the workspace 146 us against 138 at [16384, 4096], through tensor memory 149.
 //
 // dy and total come through a ring of places in shared memory (cp.async; a thread copies and
 // reads its own words only, so that needs no barrier): a place is copied into again as soon as
@@ -460,6 +471,8 @@ norm_forward_kernel(ForwardArgs a) {
 // 32768]; 4 blocks of 16 warps took 179).
 
 // Warps to an SM: 128 registers a thread, or 85 where it holds one word of each array.
+// Odd rows with dropout or dtotal spill 32 to 68 bytes a thread at that, with more registers an SM
+// would hold half the warps.
 constexpr int warps_per_sm(int vpt) { return vpt == 1 ? 24 : 16; }
 
 template <int VPT, int WARPS, bool ODD, bool FUSED>

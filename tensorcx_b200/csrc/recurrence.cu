@@ -19,10 +19,13 @@
 // States, gradients and the parts' products are float32; the sigmoid's exponential is the
 // hardware's base-2 one (2 ulp, plus the rounding of its argument).
 //
-// Measured on one B200 (bytes that the form cannot do without over the call's time, against a
-// copy's 6.55 TB/s): [1, 65536, 1024] decay forward 137 us (5.9 TB/s, 0.90), [4, 8192, 2048]
-// sigmoid forward 133 us (0.92), [2, 16384, 2048] sigmoid backward 250 us (6.4 TB/s, 0.98),
-// [2, 16384, 2049] 341 us (0.72) and forward 189 us (0.65), [64, 32, 4096] forward 24 us (0.67).
+// Measured on one B200, calls back to back on changing inputs (bytes that the form cannot do without
+// over the call's time, against a copy's 6.55 TB/s): [1, 65536, 1024] decay forward 140 us (5.8
+// TB/s, 0.88), [4, 8192, 2048] sigmoid forward 143 us (0.86), [2, 16384, 2048] sigmoid backward
+// 261 us (6.2 TB/s, 0.94), decay 215 us (0.95), [2, 16384, 2049] 374 us (0.66) and forward 207 us
+// (0.59), [64, 32, 4096] sigmoid forward 18.5 us and backward 31 to 36 (some of it from the second-
+// level cache). Where a comment below gives two figures for a choice, they were taken side by side
+// when it was made.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -125,7 +128,8 @@ __device__ __forceinline__ void backward_step(const float (&gate)[VEC], const fl
 // Four steps' loads of 4 channels in flight: [64, 32, 4096] forward 24 us, 28 with two, 26 with
 // eight; eight of one channel: [100, 100, 1001] forward 35 us against 39. A call of one step
 // has its own kernel, of which an SM holds more threads ([4096, 1, 4096]: forward 59 us before
-// and 43 so, sigmoid backward 150 and 92).
+// and 43 so, sigmoid backward 150 and 92). Its forward one is held to 32 registers and spills 24 to
+// 76 bytes a thread: with 40 (4 to 40 bytes, 6 blocks to an SM) 41.2 us against 41.0.
 template <int VEC>
 constexpr int kAhead = VEC == 4 ? 4 : 8;
 
@@ -209,7 +213,9 @@ __global__ void __launch_bounds__(256) walk_backward_kernel(Args a) {
 // the product of its gates and its last state from zero. The groups' parts meet by shuffles,
 // the warps' in shared memory and the chunks' in the workspace, as records: a block publishes
 // its chunk's (A, B), walks back over its chain's published parts to the nearest chunk whose
-// last state is known, advances that state through the parts between, and publishes its own.
+// last state is known, advances that state through the parts between, and publishes its own
+// (the method of Merrill and Garland, "Single-pass parallel prefix scan with decoupled
+// look-back", 2016).
 // Blocks stay on their SM and take chunks in order of a ticket, each in the order it got
 // them, so what a block waits for has always begun; the waits are bounded all the same.
 //
@@ -357,7 +363,8 @@ __device__ Tile tile_of(const Args& a, const Scan& sc, unsigned i) {
 // of an aligned array, so a warp copies the 16-byte words that hold its rows, 9 to a row, and a
 // lane reads its channel at the row's own distance (shift) from the first word's start, which is
 // the same in every array. VEC = 1 alone: arrays at any address, copied element by element (an
-// instruction that copies 4 bytes a lane takes the load unit some 30 cycles: only where needed).
+// instruction that copies 4 bytes a lane takes the load unit some 30 cycles: only where needed;
+// one element off the alignment [2, 16384, 2048] takes 226 to 243 us forward and 285 to 357 backward).
 template <int VEC, bool SHIFTED>
 struct Rows {
   static constexpr int kWarps = VEC == 4 ? 4 : 8;           // that work on a chunk

@@ -768,8 +768,8 @@ def _dropout_stream(p, seed, offset, index):
 
 def dropout(x: torch.Tensor, p: float, seed: int, *, offset=0, residual: torch.Tensor | None = None) -> torch.Tensor:
     """dropout(x), or residual + dropout(x) in one pass. Element i is kept when element
-    offset + i of rand_uniform's stream of `seed` is at least p, and then multiplied by
-    1 / (1 - p); a dropped element is 0 even when it is inf or NaN. The mask is never
+    offset + i (modulo 2**64) of rand_uniform's stream of `seed` is at least p, both as 64-bit
+    numbers, and then multiplied by 1 / (1 - p); a dropped element is 0 even when it is inf or NaN. The mask is never
     stored: dropout_backward makes it again from the same seed and offset. `offset` is an
     integer, or a CUDA int64 tensor of one element that is read when the kernel runs
     (advance it between the replays of a captured graph)."""

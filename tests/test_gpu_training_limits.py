@@ -127,7 +127,8 @@ def many_rows(rows, cols, shift, value):
         return buf[shift:].view(t.shape)
     make = torch.Generator(device="cuda").manual_seed(rows + cols)
     total = at_shift(torch.randn(rows, cols, generator=make, device="cuda"))
-    return at_shift(torch.full((rows, cols), value, device="cuda")), total, total.mean(1), 1 / total.std(1, correction=0)
+    rstd = 1 / total.std(1, correction=0)
+    return at_shift(torch.full((rows, cols), value, device="cuda")), total, total.mean(1), rstd
 
 
 @pytest.mark.parametrize("rows,cols,value", [(1000000, 64, 0.1), (700003, 129, 0.7), (1100, 40, 0.1),
