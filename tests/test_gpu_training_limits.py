@@ -163,6 +163,26 @@ def test_column_sums_of_many_rows(tcx, rows, cols, held, value):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("rows,cols", [(160004, 1001), (20004, 8190), (5000, 16385)])
+def test_rounds_of_blocks_are_one_call(tcx, rows, cols):
+    """More rows than one round of blocks takes, with dropout and dtotal: the last rows (from a
+    multiple of 4 on) are those of a call on them alone, the sums the parts' sums."""
+    make = torch.Generator(device="cuda").manual_seed(cols)
+    dy, total, extra = (torch.randn(rows, cols, generator=make, device="cuda") for _ in range(3))
+    mean, rstd, w = total.mean(1), 1 / total.std(1, correction=0), torch.ones(cols, device="cuda")
+    kw = dict(p=0.25, seed=6)
+    dx, dres, dw, db = tcx.layernorm_backward(dy, total, mean, rstd, w, dtotal=extra, offset=9, **kw)
+    cut = rows // 2 // 4 * 4
+    parts = [tcx.layernorm_backward(dy[s], total[s], mean[s].contiguous(), rstd[s].contiguous(), w, dtotal=extra[s],
+                                    offset=9 + s.start * cols, **kw) for s in (slice(0, cut), slice(cut, rows))]
+    assert torch.equal(dx, torch.cat([q[0] for q in parts])) and torch.equal(dres, torch.cat([q[1] for q in parts]))
+    k = 2 * chain_in_registers(rows, 32)
+    size_w, size_b = (dy * (total - mean[:, None]) * rstd[:, None]).abs().sum(0), dy.abs().sum(0)
+    within(host(dw), host(parts[0][2].double() + parts[1][2].double()), k * U * host(size_w), "dweight")
+    within(host(db), host(parts[0][3].double() + parts[1][3].double()), k * U * host(size_b), "dbias")
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------------- wide rows
 @pytest.mark.parametrize("cols", [2, 40, 1024, 5000, 16384, 40000])
 @pytest.mark.parametrize("shift", [0, 1])
